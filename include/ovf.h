@@ -215,6 +215,87 @@ ovf_status ovf_attention_decode_noalloc(const float *q, const void *k_cache, con
                                         int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx,
                                         int32_t seq_len, float scale, void *stream);
 
+/* ------------------------------------------------- 4-bit KV cache */
+/* No counterpart in the reference (its quantized cache is Q8,
+ * Runtime/Q8KvQuant.cs): a cache of 5 bits per element.  Every 32 consecutive
+ * dimensions of a head vector share two fp16 numbers D and M; code c of 0..15
+ * stands for fp16(D * (1 + c/16) + M), rounded once.  D = fp16((max - min) *
+ * 16/15) and M = fp16(min - D) in fp32 steps, and an element gets the code
+ * clamp(rint(((x - M) - D) * (16/D)), 0, 15).  NaN is stored as 0 and
+ * magnitudes above 16384 saturate, so a cache holds finite values only.
+ *
+ * A cache is one side (keys or values) of one layer of one sequence; n_seq of
+ * them lie one behind the other, ovf_kv_q4_bytes apart, 16-byte aligned.
+ * head_dim 32, 64, 128 or 256; max_ctx at most 2^20.  The bytes are
+ * [kv head][tile of 32 positions][20 * head_dim] in the order of the tensor
+ * cores' operands; they are written by ovf_kv_q4_append and read by
+ * ovf_kv_q4_read.
+ *
+ * positions (device, n_seq): what each sequence holds before the call's rows;
+ * negative marks an unused place, for which nothing is read or written.
+ * row_counts (device, n_seq, or NULL for all): how many of its `rows` are
+ * real; the others are not read, and their places in an output are left as
+ * they are.  A sequence whose rows do not fit max_ctx is left out and sets the
+ * error word (ovf_device_error code 4).  Rows are [n_seq][rows][heads *
+ * head_dim] fp32.  Buffers of a call must not overlap unless it says so; calls
+ * on the same cache are ordered by the caller (one stream, or events).
+ *
+ * rope_cos / rope_sin ([max_ctx][head_dim / 2]) rotate keys and queries at
+ * their positions as Rope/RopeKernel.cs:46 does; NULL leaves them as they are. */
+int64_t ovf_kv_q4_bytes(int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx); /* 0: unsupported */
+/* Row r of sequence s is stored at position positions[s] + r (k rotated). */
+ovf_status ovf_kv_q4_append(const float *k, const float *v, void *k_cache, void *v_cache, const int32_t *positions,
+                            const int32_t *row_counts, int32_t n_seq, int32_t rows, int32_t n_kv_heads,
+                            int32_t head_dim, int32_t max_ctx, const float *rope_cos, const float *rope_sin,
+                            int32_t split_half, void *stream);
+/* The values that the cache holds at positions positions[s] + r. */
+ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_t *positions, const int32_t *row_counts,
+                          int32_t n_seq, int32_t rows, int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx, float *k,
+                          float *v, void *stream);
+/* Runtime/CachedAttentionKernel.cs:36 ComputeSingleHead for rows of queries
+ * over 4-bit caches: row r of sequence s attends positions [0, positions[s] +
+ * r] (query head h reads KV head h / (n_heads / n_kv_heads)).  One row is a
+ * decode step, several are a verify batch or a prefill chunk.  The scores, the
+ * softmax's sums and the outputs are fp32, within rounding of the 64-bit
+ * result on the cached values.  Up to OVF_Q4_EXACT_ROWS rows, a row's output
+ * does not depend on the other rows and sequences of the call, bit for bit.
+ * k_new / v_new (or NULL): rows that are appended first, as ovf_kv_q4_append
+ * does.  scratch: ovf_attention_q4_scratch_bytes, 16-byte aligned, for one
+ * call at a time (calls that may overlap, graphs included, need their own). */
+#define OVF_Q4_EXACT_ROWS 64
+int64_t ovf_attention_q4_scratch_bytes(int32_t n_seq, int32_t rows, int32_t n_heads, int32_t n_kv_heads,
+                                       int32_t head_dim, int32_t max_ctx);
+ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_new, void *k_cache, void *v_cache,
+                            float *out, const int32_t *positions, const int32_t *row_counts, int32_t n_seq,
+                            int32_t rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_ctx,
+                            const float *rope_cos, const float *rope_sin, int32_t split_half, float scale,
+                            void *scratch, void *stream);
+
+/* ------------------------------------------------- drafted tokens */
+/* The acceptance of drafted tokens for sampled generation (the reference's
+ * GenerateSpeculative, Runtime/CachedLlamaSession.cs:335, accepts greedily).
+ * All pointers are device memory.  Row j of logits [n_seq][max_drafts + 1]
+ * [vocab] gives p_j = softmax(logits_j / temperature) behind the first j
+ * drafts.  Draft j (drafts [n_seq][max_drafts]) is accepted iff u_j * q_j(d_j)
+ * < p_j(d_j), with q from draft_probs [n_seq][max_drafts][vocab], or NULL for
+ * drafts that are certain (q = 1).  At the first rejected draft the next token
+ * is drawn from max(p_j - q_j, 0), behind the last draft from p_j: the first
+ * index whose cumulative sum exceeds u_{max_drafts} times the sum (the last
+ * index of positive weight where none does, the row's first maximum where
+ * nothing has weight).  uniforms [n_seq][max_drafts + 1] in [0, 1);
+ * temperatures [n_seq]: 0 or less is greedy (a draft is accepted iff it is its
+ * row's first maximum, and the next token is that maximum).  Logits of
+ * -infinity are impossible tokens; a row that has no finite maximum, or a NaN,
+ * accepts nothing and gives token -1.  A draft outside the vocabulary is
+ * rejected.  draft_counts [n_seq] or NULL (max_drafts each): negative marks an
+ * unused place, whose results are left as they are.
+ * accepted [n_seq]: drafts accepted; next_token [n_seq].  max_drafts 0 samples
+ * plainly.  Probabilities and sums are formed in 64 bits. */
+ovf_status ovf_verify_drafts(const float *logits, const float *draft_probs, const int32_t *drafts,
+                             const int32_t *draft_counts, const float *uniforms, const float *temperatures,
+                             int32_t n_seq, int32_t max_drafts, int32_t vocab, int32_t *accepted, int32_t *next_token,
+                             void *stream);
+
 /* ------------------------------------------------------------- sessions */
 typedef struct ovf_model ovf_model;
 typedef struct ovf_session ovf_session;

@@ -82,6 +82,12 @@ SIGNATURES = {
     "ovf_attention_single_head": (I32, [P, P, P, P, I32, I32, I32, I32, I32, F, P]),
     "ovf_attention_single_head_f16": (I32, [P, P, P, P, I32, I32, I32, I32, I32, F, P]),
     "ovf_attention_single_head_q8": (I32, [P, P, P, P, P, P, I32, I32, I32, I32, I32, F, P]),
+    "ovf_kv_q4_bytes": (I64, [I32, I32, I32]),
+    "ovf_kv_q4_append": (I32, [P, P, P, P, P, P, I32, I32, I32, I32, I32, P, P, I32, P]),
+    "ovf_kv_q4_read": (I32, [P, P, P, P, I32, I32, I32, I32, I32, P, P, P]),
+    "ovf_attention_q4_scratch_bytes": (I64, [I32, I32, I32, I32, I32, I32]),
+    "ovf_attention_q4": (I32, [P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, I32, P, P, I32, F, P, P]),
+    "ovf_verify_drafts": (I32, [P, P, P, P, P, P, I32, I32, I32, P, P, P]),
     "ovf_model_create": (I32, [I32, P, P, I32, P]),
     "ovf_model_destroy": (I32, [P]),
     "ovf_model_weight_bytes": (I64, [P]),

@@ -9,6 +9,10 @@ kernel classes (paths relative to ``Sources/Main/LanguageModels/``):
 * ``GgmlQuant`` / ``GgmlDequant`` — Loading/GgmlQuant.cs, Loading/GgmlDequant.cs
 * ``CachedAttentionKernel`` — Runtime/CachedAttentionKernel.cs
 
+and two classes without a counterpart there: ``KvCacheQ4``, the 4-bit KV cache,
+and ``SpeculativeVerifier``, the acceptance of drafted tokens for sampled
+generation.
+
 Buffers are torch CUDA tensors (torch is used for device memory and
 streams only); every call goes through libovf_cuda.so and runs on the
 current torch CUDA stream.  As in the reference the caller owns the
@@ -45,6 +49,14 @@ def _need(t, dtype, n, name):
         raise ValueError(f"{name} must be a contiguous CUDA {dtype} tensor")
     if t.numel() < n:
         raise ValueError(f"{name} span is smaller than {n}")
+
+
+def _same_device(*tensors) -> torch.device:
+    """The device of a call's tensors (None aside); its current stream takes the call."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"tensors are on several devices: {sorted(map(str, devices))}")
+    return devices.pop()
 
 
 @dataclass
@@ -440,3 +452,118 @@ class CachedAttentionKernel:
         check(_lib.load().ovf_attention_decode(_ptr(query), _ptr(k_cache), _ptr(v_cache), _ptr(output), n_heads,
                                                n_kv_heads, head_dim, max_ctx, seq_len, float(scale), _ptr(scratch),
                                                _ptr(counters), _stream()), "ComputeSingleHead")
+
+    @staticmethod
+    def q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim, max_ctx) -> int:
+        return int(_lib.load().ovf_attention_q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim, max_ctx))
+
+    @staticmethod
+    def compute_q4(query, k_cache, v_cache, output, positions, n_heads, n_kv_heads, head_dim, max_ctx, scale, scratch,
+                   rope_cos=None, rope_sin=None, split_half=False, row_counts=None, k_new=None, v_new=None) -> None:
+        """Causal attention of query rows [n_seq, rows, n_heads * head_dim] over
+        4-bit caches (``KvCacheQ4``): row r of sequence s is at positions[s] + r
+        and attends everything up to itself.  ``k_new`` / ``v_new`` [n_seq, rows,
+        n_kv_heads * head_dim] are appended first.  ``scratch``: uint8 of
+        ``q4_scratch_bytes``, for one call at a time."""
+        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, query, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin,
+                                      row_counts, n_heads)
+        _need(output, torch.float32, query.numel(), "output")
+        if (k_new is None) != (v_new is None):
+            raise ValueError("k_new and v_new go together")
+        for t, name in ((k_new, "k_new"), (v_new, "v_new")):
+            if t is not None:
+                _need(t, torch.float32, n_seq * rows * n_kv_heads * head_dim, name)
+        _need(scratch, torch.uint8, CachedAttentionKernel.q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim,
+                                                                           max_ctx), "scratch")
+        device = _same_device(query, k_cache, v_cache, output, positions, scratch, rope_cos, rope_sin, row_counts, k_new, v_new)
+        with torch.cuda.device(device):
+            check(_lib.load().ovf_attention_q4(_ptr(query), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
+                                               _ptr(output), _ptr(positions), _ptr(row_counts), n_seq, rows, n_heads,
+                                               n_kv_heads, head_dim, max_ctx, _ptr(rope_cos), _ptr(rope_sin),
+                                               int(split_half), float(scale), _ptr(scratch), _stream()), "attention_q4")
+
+
+class KvCacheQ4:
+    """The 4-bit KV cache: 32 dimensions share two fp16 numbers D and M, and code
+    c stands for fp16(D * (1 + c/16) + M).  One side (keys or values) of one layer
+    is uint8 of n_seq * ``bytes``; ``positions`` (int32, one a sequence) is what a
+    sequence holds before the rows of a call, negative for an unused place;
+    ``row_counts`` (int32) how many of a sequence's rows are real."""
+
+    @staticmethod
+    def bytes(n_kv_heads, head_dim, max_ctx) -> int:
+        """Bytes of one side of one layer of one sequence."""
+        return int(_lib.load().ovf_kv_q4_bytes(n_kv_heads, head_dim, max_ctx))
+
+    @staticmethod
+    def check(k_cache, v_cache, positions, rows_of, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin, row_counts, n_heads):
+        """The checks that the calls on a cache share; returns (n_seq, rows)."""
+        one = KvCacheQ4.bytes(n_kv_heads, head_dim, max_ctx)
+        if one == 0:
+            raise ValueError(f"no 4-bit cache of {n_kv_heads} heads, head_dim {head_dim} and {max_ctx} positions")
+        if rows_of is None or rows_of.dim() != 3 or rows_of.shape[2] != n_heads * head_dim:
+            raise ValueError(f"rows must be [n_seq, rows, {n_heads * head_dim}]")
+        n_seq, rows = rows_of.shape[:2]
+        _need(rows_of, torch.float32, 0, "rows")
+        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            _need(t, torch.uint8, n_seq * one, name)
+        _need(positions, torch.int32, n_seq, "positions")
+        if row_counts is not None:
+            _need(row_counts, torch.int32, n_seq, "row_counts")
+        if (rope_cos is None) != (rope_sin is None):
+            raise ValueError("rope_cos and rope_sin go together")
+        for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
+            if t is not None:
+                _need(t, torch.float32, max_ctx * head_dim // 2, name)
+        return n_seq, rows
+
+    @staticmethod
+    def append(k, v, k_cache, v_cache, positions, n_kv_heads, head_dim, max_ctx, rope_cos=None, rope_sin=None,
+               split_half=False, row_counts=None) -> None:
+        """Rows k, v [n_seq, rows, n_kv_heads * head_dim] at positions[s] + r, the keys rotated."""
+        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, k, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin,
+                                      row_counts, n_kv_heads)
+        _need(v, torch.float32, k.numel(), "v")
+        with torch.cuda.device(_same_device(k, v, k_cache, v_cache, positions, rope_cos, rope_sin, row_counts)):
+            check(_lib.load().ovf_kv_q4_append(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(positions),
+                                               _ptr(row_counts), n_seq, rows, n_kv_heads, head_dim, max_ctx, _ptr(rope_cos),
+                                               _ptr(rope_sin), int(split_half), _stream()), "kv_q4_append")
+
+    @staticmethod
+    def read(k_cache, v_cache, positions, n_kv_heads, head_dim, max_ctx, k, v, row_counts=None) -> None:
+        """What the caches hold at positions[s] + r, into k, v [n_seq, rows, n_kv_heads * head_dim]."""
+        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, k, n_kv_heads, head_dim, max_ctx, None, None, row_counts,
+                                      n_kv_heads)
+        _need(v, torch.float32, k.numel(), "v")
+        with torch.cuda.device(_same_device(k, v, k_cache, v_cache, positions, row_counts)):
+            check(_lib.load().ovf_kv_q4_read(_ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(row_counts), n_seq, rows,
+                                             n_kv_heads, head_dim, max_ctx, _ptr(k), _ptr(v), _stream()), "kv_q4_read")
+
+
+class SpeculativeVerifier:
+    @staticmethod
+    def verify(logits, drafts, uniforms, temperatures, accepted, next_token, draft_probs=None, draft_counts=None) -> None:
+        """Accepts drafted tokens against the target's distribution and draws the
+        next token: logits [n_seq, max_drafts + 1, vocab], drafts int32 [n_seq,
+        max_drafts], uniforms [n_seq, max_drafts + 1], temperatures [n_seq] (0 or
+        less: greedy), draft_probs [n_seq, max_drafts, vocab] or None for drafts
+        that are certain; accepted and next_token int32 [n_seq]."""
+        if logits is None or logits.dim() != 3 or logits.shape[1] < 1:
+            raise ValueError("logits must be [n_seq, max_drafts + 1, vocab]")
+        n_seq, m, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+        _need(logits, torch.float32, 0, "logits")
+        if m:
+            _need(drafts, torch.int32, n_seq * m, "drafts")
+        _need(uniforms, torch.float32, n_seq * (m + 1), "uniforms")
+        _need(temperatures, torch.float32, n_seq, "temperatures")
+        _need(accepted, torch.int32, n_seq, "accepted")
+        _need(next_token, torch.int32, n_seq, "next_token")
+        if draft_probs is not None:
+            _need(draft_probs, torch.float32, n_seq * m * vocab, "draft_probs")
+        if draft_counts is not None:
+            _need(draft_counts, torch.int32, n_seq, "draft_counts")
+        with torch.cuda.device(_same_device(logits, drafts if m else None, uniforms, temperatures, accepted, next_token,
+                                            draft_probs, draft_counts)):
+            check(_lib.load().ovf_verify_drafts(_ptr(logits), _ptr(draft_probs) if m else None, _ptr(drafts) if m else None,
+                                                _ptr(draft_counts), _ptr(uniforms), _ptr(temperatures), n_seq, m, vocab,
+                                                _ptr(accepted), _ptr(next_token), _stream()), "verify_drafts")
