@@ -11,8 +11,18 @@
 // one.  T <= 0 is greedy: a draft is accepted iff it is its row's first
 // maximum, which is also the next token.
 //
-// Exponentials and sums are formed in 64 bits: a decision that falls the other
-// way because of a rounding changes a token, and a vocabulary has 10^5 borders.
+// A decision must not depend on rounding: a vocabulary has 10^5 borders, and one
+// that falls the other way changes a token.  The rows' sums are first formed from
+// fp32 exponentials, off by less than 2^-16; where a draft's decision is nearer to
+// its border than that (about one in 10^5), its row is summed again in 64 bits.
+// The row that a token is drawn from is summed in 64 bits always.
+//
+// A cluster of 8 or 16 CTAs takes a sequence: every CTA a part of each row, all
+// rows one behind the other, so that memory streams while sums are formed; the
+// partial sums meet in distributed shared memory.  Bound by the logits' bytes for
+// a batch, by the cluster's barriers and the drawing for one sequence.
+#include <float.h>
+
 #include "ovf_internal.cuh"
 
 namespace ovf {
@@ -24,130 +34,404 @@ struct VerifyParams {
     int max_drafts, vocab;
 };
 
-static constexpr int kVerifyThreads = 1024;
+static constexpr int kVfThreads = 512, kVfWarps = kVfThreads / 32;
+static constexpr int kVfRows = 1024;        // max_drafts + 1
+static constexpr int kVfCluster = 16;       // at most
 
-// One CTA per sequence, row after row.
-__global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const VerifyParams p) {
-    __shared__ double sd[32];
-    __shared__ float sf[32];
-    __shared__ int si[32];
-    __shared__ int s_next;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x, V = p.vocab;
+// e^x in 64 bits, off by a few 2^-52: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from
+// the table of 2^(i / 32) that exp_libm (ovf_common.cuh) has.  ln 2 is taken in two parts, the first of 24 bits, so
+// that its product with n is exact.
+__device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
+    if (!(x > -700.0)) return x < -746.0 ? 0.0 : exp(x);  // results below the normal numbers, and NaN
+    const double n = rint(x * (32.0 / 0.693147180559945309417));
+    double r = fma(n, -0x1.62e4300000000p-1 / 32.0, x);
+    r = fma(n, -(-0x1.05c610ca86c39p-29) / 32.0, r);
+    double y = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    y = fma(y, r, 1.0 / 24.0);
+    y = fma(y, r, 1.0 / 6.0);
+    y = fma(y, r, 0.5);
+    y = fma(y, r, 1.0);
+    y = fma(y, r, 1.0);
+    const int k = (int)n;
+    return y * __longlong_as_double((long long)(tab[k & 31] + ((unsigned long long)(long long)k << 47)));
+}
+
+__device__ __forceinline__ float vf_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <class T>
+__device__ __forceinline__ T cluster_read(const T *p, int rank) {
+    T v;
+    const uint32_t at = mapa_shared(smem_u32(p), (uint32_t)rank);
+    if (sizeof(T) == 8) {
+        double d;
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(d) : "r"(at) : "memory");
+        memcpy(&v, &d, sizeof(T));
+    } else {
+        uint32_t u;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(u) : "r"(at) : "memory");
+        memcpy(&v, &u, sizeof(T));
+    }
+    return v;
+}
+
+// Elements 4 g - shift .. + 3 of a row (shift: what its address lies behind a
+// 16-byte boundary); those outside the row are `none`.
+__device__ __forceinline__ float4 vf_load4(const float *row, int V, int shift, int g, float none) {
+    const int i = 4 * g - shift;
+    if (i >= 0 && i + 4 <= V) return __ldg(reinterpret_cast<const float4 *>(row + i));
+    float4 v;
+    v.x = i >= 0 && i < V ? row[i] : none;
+    v.y = i + 1 >= 0 && i + 1 < V ? row[i + 1] : none;
+    v.z = i + 2 >= 0 && i + 2 < V ? row[i + 2] : none;
+    v.w = i + 3 >= 0 && i + 3 < V ? row[i + 3] : none;
+    return v;
+}
+__device__ __forceinline__ int vf_shift(const float *row) { return (int)(reinterpret_cast<uintptr_t>(row) >> 2) & 3; }
+
+struct VfShared {
+    float m[kVfRows];          // this CTA's part of every row: largest logit,
+    int at[kVfRows];           // its first place (greedy),
+    double sum[kVfRows];       // sum of exponentials (NaN: a row with a NaN or +infinity)
+    float row_m[kVfRows];      // the same of the whole rows
+    int row_at[kVfRows];
+    float wm[2][kVfWarps];
+    int wat[2][kVfWarps];
+    double wsum[2][kVfWarps];
+    double part[kVfWarps];               // the drawing: sums of this CTA's warps' parts
+    double all[kVfCluster * kVfWarps];   // of all CTAs'
+    unsigned long long tab[32];
+    int first, token;
+};
+
+// The (largest, first place of it, sum) of N lanes as one, in every lane.
+template <int N>
+__device__ __forceinline__ void vf_join(float &m, int &at, double &sum, bool greedy, double inv,
+                                        const unsigned long long *tab) {
+    float top = m;
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (greedy) {
+        if (m != top) at = 0x7FFFFFFF;
+#pragma unroll
+        for (int o = N / 2; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xFFFFFFFFu, at, o));
+    } else {
+        sum *= vf_exp(((double)m - top) * inv, tab);
+    }
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    m = top;
+}
+
+enum : int { VF_ACCEPT = 0, VF_REJECT = 1, VF_NEAR = 2, VF_BAD = 3 };
+
+// The sum over the cluster of a value of every warp's part, in the order of the parts; all[] holds them.
+__device__ __forceinline__ double vf_gather(VfShared &sh, double mine, int size, int warp, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
+    if (lane == 0) sh.part[warp] = mine;
+    cluster_barrier();
+    for (int i = threadIdx.x; i < size * kVfWarps; i += kVfThreads) sh.all[i] = cluster_read(&sh.part[i % kVfWarps], i / kVfWarps);
+    cluster_barrier();  // (also: part may be written again)
+    double s = 0.0;
+    for (int i = lane; i < size * kVfWarps; i += 32) s += sh.all[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    return s;
+}
+
+__global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const VerifyParams p) {
+    extern __shared__ __align__(16) unsigned char vf_smem[];
+    VfShared &sh = *reinterpret_cast<VfShared *>(vf_smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.vocab;
+    uint32_t rank, size;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    const int s = blockIdx.x / size;
+    if (tid < 32) sh.tab[tid] = kExp2Tab32[tid];
     const int n = p.counts ? min(p.counts[s], p.max_drafts) : p.max_drafts;
-    if (n < 0) return;  // an unused place
+    if (n < 0) return;  // an unused place (all CTAs of the cluster leave)
     const float T = p.temperatures[s];
     const bool greedy = !(T > 0.0f);
-    const int32_t *d = p.drafts ? p.drafts + (size_t)s * p.max_drafts : nullptr;
-    const float *u = p.uniforms ? p.uniforms + (size_t)s * (p.max_drafts + 1) : nullptr;
-    int acc = 0, next = -1;
+    const int32_t *drafts = p.drafts + (size_t)s * p.max_drafts;
+    const float *u = p.uniforms + (size_t)s * (p.max_drafts + 1);
+    const float *logits = p.logits + (size_t)s * (p.max_drafts + 1) * V;
+    const float c = fminf(1.44269504088896340736f / T, FLT_MAX);
+    const double inv = 1.0 / (double)T;
+    __syncthreads();
+
+    // every row's largest logit and sum (greedy: and the first place of it), this CTA's part
     for (int j = 0; j <= n; ++j) {
-        const float *x = p.logits + ((size_t)s * (p.max_drafts + 1) + j) * V;
-        // largest logit and its first place
-        float m = -INFINITY;
-        int at = V;
-        bool bad = false;
-        for (int i = tid; i < V; i += kVerifyThreads) {
-            const float y = x[i];
-            bad |= y != y;
-            if (y > m) m = y, at = i;
+        const float *x = logits + (size_t)j * V;
+        const int shift = vf_shift(x), groups = (V + shift + 3) / 4;
+        float m = -FLT_MAX;
+        int at = 0x7FFFFFFF;
+        double sum = 0.0;
+        if (greedy) {
+            bool bad = false;
+            for (int g = rank * kVfThreads + tid; g < groups; g += size * kVfThreads) {
+                const float4 v = vf_load4(x, V, shift, g, -INFINITY);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bad |= e[i] != e[i];
+                    const int k = 4 * g - shift + i;
+                    if (e[i] > m || (e[i] == m && k < at)) m = e[i], at = k;
+                }
+            }
+            if (bad) sum = __longlong_as_double(0x7ff8000000000000ll);
+        } else {
+            const int step = size * kVfThreads;
+            auto add = [&](const float4 &v) {
+                const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+                if (top > m) {
+                    sum *= vf_exp(((double)m - top) * inv, sh.tab);
+                    m = top;
+                }
+                sum += (double)((vf_ex2((v.x - m) * c) + vf_ex2((v.y - m) * c)) +
+                                (vf_ex2((v.z - m) * c) + vf_ex2((v.w - m) * c)));
+            };
+            int g = rank * kVfThreads + tid;
+            for (; g + 3 * step < groups; g += 4 * step) {
+                float4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = vf_load4(x, V, shift, g + i * step, -INFINITY);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) add(v[i]);
+            }
+            for (; g < groups; g += step) add(vf_load4(x, V, shift, g, -INFINITY));
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m, o);
-            const int a2 = __shfl_xor_sync(0xFFFFFFFFu, at, o);
-            if (m2 > m || (m2 == m && a2 < at)) m = m2, at = a2;
+        vf_join<32>(m, at, sum, greedy, inv, sh.tab);
+        const int b = j & 1;  // two sets: a warp may be a row ahead of the one that joins
+        if (lane == 0) sh.wm[b][warp] = m, sh.wat[b][warp] = at, sh.wsum[b][warp] = sum;
+        __syncthreads();
+        if (warp == (j & (kVfWarps - 1))) {
+            m = lane < kVfWarps ? sh.wm[b][lane] : -FLT_MAX;
+            at = lane < kVfWarps ? sh.wat[b][lane] : 0x7FFFFFFF;
+            sum = lane < kVfWarps ? sh.wsum[b][lane] : 0.0;
+            vf_join<kVfWarps>(m, at, sum, greedy, inv, sh.tab);
+            if (lane == 0) sh.m[j] = m, sh.at[j] = at, sh.sum[j] = sum;
+        }
+    }
+    cluster_barrier();
+
+    // the whole rows, and what becomes of every draft (each CTA forms the same)
+    int state[kVfRows / kVfThreads];
+#pragma unroll
+    for (int i = 0; i < kVfRows / kVfThreads; ++i) {
+        const int j = tid + i * kVfThreads;
+        state[i] = VF_ACCEPT;
+        if (j > n) continue;
+        float m = -FLT_MAX;
+        int at = 0x7FFFFFFF;
+        double sum = 0.0;
+        for (int w = 0; w < (int)size; ++w) m = fmaxf(m, cluster_read(&sh.m[j], w));
+        for (int w = 0; w < (int)size; ++w) {
+            const float m2 = cluster_read(&sh.m[j], w);
+            const double sum2 = cluster_read(&sh.sum[j], w);
+            sum += greedy ? sum2 : sum2 * vf_exp(((double)m2 - m) * inv, sh.tab);
+            if (m2 == m) at = min(at, cluster_read(&sh.at[j], w));
+        }
+        sh.row_m[j] = m;
+        sh.row_at[j] = at;
+        const int d = j < n ? drafts[j] : -1;
+        if (sum != sum || !(m < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0)) {
+            state[i] = VF_BAD;
+        } else if (j == n) {
+            state[i] = VF_REJECT;  // the row behind the last draft
+        } else if (greedy) {
+            state[i] = d == at ? VF_ACCEPT : VF_REJECT;
+        } else if (d < 0 || d >= V) {
+            state[i] = VF_REJECT;
+        } else {
+            const double e = vf_exp(((double)logits[(size_t)j * V + d] - (double)m) * inv, sh.tab);
+            const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + j) * V + d] : 1.0;
+            const double limit = (double)u[j] * q * sum;
+            state[i] = fabs(limit - e) <= 0x1p-16 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
+        }
+    }
+
+    // the first row that is not an accepted draft
+    int k = -1, st = VF_ACCEPT;
+    const int per = (int)(((size_t)V + 3 + size * kVfWarps * 128 - 1) / (size * kVfWarps * 128));  // 128 elements a step
+    const int steps0 = (int)(rank * kVfWarps + warp) * per;  // this warp's part of a row: steps [steps0, steps0 + per)
+    while (true) {
+        __syncthreads();
+        if (tid == 0) sh.first = 0x7FFFFFFF;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kVfRows / kVfThreads; ++i) {
+            const int j = tid + i * kVfThreads;
+            if (j <= n && j > k && state[i] != VF_ACCEPT) atomicMin(&sh.first, j * 4 + state[i]);
         }
         __syncthreads();
-        if (lane == 0) sf[warp] = m, si[warp] = at;
-        bad = __syncthreads_or(bad);
-        for (int w = 0; w < 32; ++w)
-            if (sf[w] > m || (sf[w] == m && si[w] < at)) m = sf[w], at = si[w];
-        bad |= !(fabsf(m) < INFINITY);
-        if (bad) break;  // a row without a distribution: no token
-        const int dj = j < n ? d[j] : -1;
-        if (greedy) {
-            if (dj == at) {
-                ++acc;
-                continue;
-            }
-            next = at;
+        k = sh.first >> 2;
+        st = sh.first & 3;
+        if (st != VF_NEAR) break;
+        // too near to tell: the row's sum in 64 bits
+        const float *x = logits + (size_t)k * V;
+        const double m = (double)sh.row_m[k];
+        const int shift = vf_shift(x);
+        double sum = 0.0;
+        for (int i = steps0; i < steps0 + per; ++i) {
+            const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
+            sum += (vf_exp(((double)v.x - m) * inv, sh.tab) + vf_exp(((double)v.y - m) * inv, sh.tab)) +
+                   (vf_exp(((double)v.z - m) * inv, sh.tab) + vf_exp(((double)v.w - m) * inv, sh.tab));
+        }
+        const double total = vf_gather(sh, sum, size, warp, lane);
+        const int d = drafts[k];
+        const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + k) * V + d] : 1.0;
+        if (!((double)u[k] * q * total < vf_exp(((double)x[d] - m) * inv, sh.tab))) {
+            st = VF_REJECT;
             break;
         }
-        double sum = 0.0;
-        for (int i = tid; i < V; i += kVerifyThreads) sum += exp(((double)x[i] - m) / T);
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        __syncthreads();
-        if (lane == 0) sd[warp] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int w = 0; w < 32; ++w) sum += sd[w];
-        const float *q = p.probs && j < n ? p.probs + ((size_t)s * p.max_drafts + j) * V : nullptr;
-        const bool known = dj >= 0 && dj < V;
-        if (j < n && known) {
-            const double e = exp(((double)x[dj] - m) / T), qd = q ? (double)q[dj] : 1.0;
-            if ((double)u[j] * qd * sum < e) {
-                ++acc;
-                continue;
+    }
+
+    int token = -1;
+    if (st == VF_REJECT && greedy) {
+        token = sh.row_at[k];
+    } else if (st == VF_REJECT) {
+        const float *x = logits + (size_t)k * V;
+        const float *q = p.probs && k < n ? p.probs + ((size_t)s * p.max_drafts + k) * V : nullptr;
+        const int out = !q && k < n ? drafts[k] : -1;  // a certain draft has no weight left
+        const double m = (double)sh.row_m[k];
+        const int shift = vf_shift(x);
+        auto weight4 = [&](int i, double scale, double (&w)[4]) {
+            const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
+            w[0] = vf_exp(((double)v.x - m) * inv, sh.tab) * scale;
+            w[1] = vf_exp(((double)v.y - m) * inv, sh.tab) * scale;
+            w[2] = vf_exp(((double)v.z - m) * inv, sh.tab) * scale;
+            w[3] = vf_exp(((double)v.w - m) * inv, sh.tab) * scale;
+            const int at = 4 * (i * 32 + lane) - shift;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (q && at + b >= 0 && at + b < V) w[b] = fmax(w[b] - (double)q[at + b], 0.0);
+                if (at + b == out) w[b] = 0.0;
             }
-        }
-        // the residual's cumulative sum: every thread takes a run of the row
-        const int per = (V + kVerifyThreads - 1) / kVerifyThreads, i0 = min(V, tid * per), i1 = min(V, i0 + per);
-        auto rest = [&](int i) {
-            const double e = exp(((double)x[i] - m) / T) / sum;
-            if (j >= n) return e;
-            if (q) return fmax(e - (double)q[i], 0.0);
-            return i == dj ? 0.0 : e;
         };
-        double run = 0.0;
-        int last = -1;
-        for (int i = i0; i < i1; ++i) {
-            const double r = rest(i);
-            run += r;
-            if (r > 0.0) last = i;
-        }
-        double before = run;  // inclusive sum over the threads
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xFFFFFFFFu, before, o);
-            if (lane >= o) before += y;
-        }
-        __syncthreads();
-        if (lane == 31) sd[warp] = before;
-        if (tid == 0) s_next = V;
-        for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xFFFFFFFFu, last, o));
-        if (lane == 0) si[warp] = last;
-        __syncthreads();
-        double base = 0.0, total = 0.0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) base += sd[w];
-            total += sd[w];
-        }
-        const double target = (double)u[p.max_drafts] * total;
-        double c = base + before - run;
-        for (int i = i0; i < i1; ++i) {
-            const double r = rest(i);
-            c += r;
-            if (r > 0.0 && c > target) {
-                atomicMin(&s_next, i);
-                break;
+        double scale = 1.0, w[4];
+        if (q) {  // p and q are compared: p needs its sum
+            double sum = 0.0;
+            const float *q0 = q;
+            q = nullptr;
+            for (int i = steps0; i < steps0 + per; ++i) {
+                weight4(i, 1.0, w);
+                sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
+            q = q0;
+            scale = 1.0 / vf_gather(sh, sum, size, warp, lane);
         }
-        __syncthreads();
-        next = s_next;
-        if (next == V) {  // u of 1 or more, or no residual at all
-            next = -1;
-            for (int w = 0; w < 32; ++w) next = max(next, si[w]);
-            if (next < 0) next = at;
+        double sum = 0.0;
+        for (int i = steps0; i < steps0 + per; ++i) {
+            weight4(i, scale, w);
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
         }
-        break;
+        const double rest = vf_gather(sh, sum, size, warp, lane);
+        const double target = (double)u[p.max_drafts] * rest;
+        // the part that holds the token, and what lies before it (every warp finds the same)
+        double before = 0.0, base = 0.0;
+        int part = -1, last = -1;
+        for (int i = 0; i < (int)size * kVfWarps; ++i) {
+            const double y = sh.all[i];
+            if (y > 0.0) {
+                last = i;
+                if (before + y > target) {
+                    part = i;
+                    base = before;
+                    break;
+                }
+            }
+            before += y;
+        }
+        const bool over = part >= 0;
+        if (!over) part = last;  // (u of 1 or more): the last token of any weight
+        if (part == (int)rank * kVfWarps + warp) {
+            int found = -1, some = -1;
+            double run = base;
+            for (int i = steps0; i < steps0 + per && found < 0; ++i) {
+                weight4(i, scale, w);
+                double mine = (w[0] + w[1]) + (w[2] + w[3]), incl = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                    if (lane >= o) incl += y;
+                }
+                double cum = run + (incl - mine);
+                int hit = 0x7FFFFFFF, any = -1;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    cum += w[b];
+                    const int at = 4 * (i * 32 + lane) - shift + b;
+                    if (w[b] > 0.0) {
+                        any = at;
+                        if (over && cum > target) hit = min(hit, at);
+                    }
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    hit = min(hit, __shfl_xor_sync(0xFFFFFFFFu, hit, o));
+                    any = max(any, __shfl_xor_sync(0xFFFFFFFFu, any, o));
+                }
+                some = max(some, any);
+                if (hit != 0x7FFFFFFF) found = hit;
+                run += __shfl_sync(0xFFFFFFFFu, incl, 31);
+            }
+            if (lane == 0) p.token[s] = found >= 0 ? found : some;
+        }
+        token = -2;  // written by the part's warp
+        if (part < 0) {
+            // nothing has weight: the row's first maximum
+            if (tid == 0) sh.token = 0x7FFFFFFF;
+            __syncthreads();
+            for (int i = steps0; i < steps0 + per; ++i) {
+                const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
+                const int at = 4 * (i * 32 + lane) - shift;
+                const float mm = sh.row_m[k];
+                const int hit = v.x == mm ? at : v.y == mm ? at + 1 : v.z == mm ? at + 2 : v.w == mm ? at + 3 : 0x7FFFFFFF;
+                if (hit != 0x7FFFFFFF) atomicMin(&sh.token, hit);
+            }
+            cluster_barrier();
+            token = 0x7FFFFFFF;
+            for (int w2 = 0; w2 < (int)size; ++w2) token = min(token, cluster_read(&sh.token, w2));
+        }
     }
-    if (tid == 0) {
-        p.accepted[s] = acc;
-        p.token[s] = next;
+    if (rank == 0 && tid == 0) {
+        p.accepted[s] = k;
+        if (token != -2) p.token[s] = token;
     }
+    cluster_barrier();  // nobody reads another CTA's memory any more
 }
 
 ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st) {
-    verify_drafts_kernel<<<n_seq, kVerifyThreads, 0, st>>>(p);
-    return cuda_status(cudaGetLastError(), "verify_drafts");
+    static PerDeviceOnce once;
+    const int dev = current_device();
+    if (once.pending(dev)) {
+        cudaError_t e = cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)sizeof(VfShared));
+        if (e != cudaSuccess) return cuda_status(e, "verify_drafts");
+        once.mark(dev);
+    }
+    const int cluster = n_seq * kVfCluster <= sm_count(dev) ? kVfCluster : 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_seq * cluster);
+    cfg.blockDim = dim3(kVfThreads);
+    cfg.dynamicSmemBytes = sizeof(VfShared);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, verify_drafts_kernel, p), "verify_drafts");
 }
 
 }  // namespace ovf

@@ -22,6 +22,7 @@ reference's ArgumentException) before anything is launched.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -51,12 +52,35 @@ def _need(t, dtype, n, name):
         raise ValueError(f"{name} span is smaller than {n}")
 
 
-def _same_device(*tensors) -> torch.device:
-    """The device of a call's tensors (None aside); its current stream takes the call."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors are on several devices: {sorted(map(str, devices))}")
-    return devices.pop()
+# The current stream of a device as a number, without a Stream object around it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _call(name, spans, *args) -> None:
+    """Checks a call's tensors and makes it on their device's current stream.
+    ``spans``: (tensor, dtype, elements needed, name), None where a tensor is
+    optional and absent; ``args`` are the entry point's, tensors among them."""
+    device = -1
+    for t, dtype, n, what in spans:
+        if t is None:
+            continue
+        if not t.is_cuda or t.dtype is not dtype or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous CUDA {dtype} tensor")
+        if t.numel() < n:
+            raise ValueError(f"{what} span is smaller than {n}")
+        if device < 0:
+            device = t.get_device()
+        elif t.get_device() != device:
+            raise ValueError(f"{what} is on another device than the call's other tensors")
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    if device == torch.cuda.current_device():
+        status = getattr(_lib.load(), name)(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(_lib.load(), name)(*args, _raw_stream(device))
+    if status:
+        check(status, name)
 
 
 @dataclass
@@ -454,6 +478,7 @@ class CachedAttentionKernel:
                                                _ptr(counters), _stream()), "ComputeSingleHead")
 
     @staticmethod
+    @lru_cache(maxsize=256)
     def q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim, max_ctx) -> int:
         return int(_lib.load().ovf_attention_q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim, max_ctx))
 
@@ -465,22 +490,17 @@ class CachedAttentionKernel:
         and attends everything up to itself.  ``k_new`` / ``v_new`` [n_seq, rows,
         n_kv_heads * head_dim] are appended first.  ``scratch``: uint8 of
         ``q4_scratch_bytes``, for one call at a time."""
-        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, query, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin,
-                                      row_counts, n_heads)
-        _need(output, torch.float32, query.numel(), "output")
-        if (k_new is None) != (v_new is None):
-            raise ValueError("k_new and v_new go together")
-        for t, name in ((k_new, "k_new"), (v_new, "v_new")):
-            if t is not None:
-                _need(t, torch.float32, n_seq * rows * n_kv_heads * head_dim, name)
-        _need(scratch, torch.uint8, CachedAttentionKernel.q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim,
-                                                                           max_ctx), "scratch")
-        device = _same_device(query, k_cache, v_cache, output, positions, scratch, rope_cos, rope_sin, row_counts, k_new, v_new)
-        with torch.cuda.device(device):
-            check(_lib.load().ovf_attention_q4(_ptr(query), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
-                                               _ptr(output), _ptr(positions), _ptr(row_counts), n_seq, rows, n_heads,
-                                               n_kv_heads, head_dim, max_ctx, _ptr(rope_cos), _ptr(rope_sin),
-                                               int(split_half), float(scale), _ptr(scratch), _stream()), "attention_q4")
+        n_seq, rows, spans = KvCacheQ4.spans(k_cache, v_cache, positions, query, "query", n_kv_heads, head_dim, max_ctx,
+                                             rope_cos, rope_sin, row_counts, n_heads)
+        if output is None or scratch is None or (k_new is None) != (v_new is None):
+            raise ValueError("output and scratch are required, and k_new and v_new go together")
+        new = n_seq * rows * n_kv_heads * head_dim
+        spans += ((output, torch.float32, n_seq * rows * n_heads * head_dim, "output"),
+                  (scratch, torch.uint8, CachedAttentionKernel.q4_scratch_bytes(n_seq, rows, n_heads, n_kv_heads, head_dim,
+                                                                                max_ctx), "scratch"),
+                  (k_new, torch.float32, new, "k_new"), (v_new, torch.float32, new, "v_new"))
+        _call("ovf_attention_q4", spans, query, k_new, v_new, k_cache, v_cache, output, positions, row_counts, n_seq, rows,
+              n_heads, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin, int(split_half), float(scale), scratch)
 
 
 class KvCacheQ4:
@@ -491,53 +511,51 @@ class KvCacheQ4:
     ``row_counts`` (int32) how many of a sequence's rows are real."""
 
     @staticmethod
+    @lru_cache(maxsize=256)
     def bytes(n_kv_heads, head_dim, max_ctx) -> int:
         """Bytes of one side of one layer of one sequence."""
         return int(_lib.load().ovf_kv_q4_bytes(n_kv_heads, head_dim, max_ctx))
 
     @staticmethod
-    def check(k_cache, v_cache, positions, rows_of, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin, row_counts, n_heads):
-        """The checks that the calls on a cache share; returns (n_seq, rows)."""
+    def spans(k_cache, v_cache, positions, rows_of, name, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin, row_counts,
+              n_heads):
+        """What the calls on a cache share: (n_seq, rows, the spans to check)."""
         one = KvCacheQ4.bytes(n_kv_heads, head_dim, max_ctx)
         if one == 0:
             raise ValueError(f"no 4-bit cache of {n_kv_heads} heads, head_dim {head_dim} and {max_ctx} positions")
         if rows_of is None or rows_of.dim() != 3 or rows_of.shape[2] != n_heads * head_dim:
-            raise ValueError(f"rows must be [n_seq, rows, {n_heads * head_dim}]")
-        n_seq, rows = rows_of.shape[:2]
-        _need(rows_of, torch.float32, 0, "rows")
-        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-            _need(t, torch.uint8, n_seq * one, name)
-        _need(positions, torch.int32, n_seq, "positions")
-        if row_counts is not None:
-            _need(row_counts, torch.int32, n_seq, "row_counts")
-        if (rope_cos is None) != (rope_sin is None):
-            raise ValueError("rope_cos and rope_sin go together")
-        for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-            if t is not None:
-                _need(t, torch.float32, max_ctx * head_dim // 2, name)
-        return n_seq, rows
+            raise ValueError(f"{name} must be [n_seq, rows, {n_heads * head_dim}]")
+        if k_cache is None or v_cache is None or positions is None or (rope_cos is None) != (rope_sin is None):
+            raise ValueError("k_cache, v_cache and positions are required, and rope_cos and rope_sin go together")
+        n_seq, rows = rows_of.shape[0], rows_of.shape[1]
+        table = max_ctx * head_dim // 2
+        return n_seq, rows, ((rows_of, torch.float32, 0, name), (k_cache, torch.uint8, n_seq * one, "k_cache"),
+                             (v_cache, torch.uint8, n_seq * one, "v_cache"), (positions, torch.int32, n_seq, "positions"),
+                             (row_counts, torch.int32, n_seq, "row_counts"), (rope_cos, torch.float32, table, "rope_cos"),
+                             (rope_sin, torch.float32, table, "rope_sin"))
 
     @staticmethod
     def append(k, v, k_cache, v_cache, positions, n_kv_heads, head_dim, max_ctx, rope_cos=None, rope_sin=None,
                split_half=False, row_counts=None) -> None:
         """Rows k, v [n_seq, rows, n_kv_heads * head_dim] at positions[s] + r, the keys rotated."""
-        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, k, n_kv_heads, head_dim, max_ctx, rope_cos, rope_sin,
-                                      row_counts, n_kv_heads)
-        _need(v, torch.float32, k.numel(), "v")
-        with torch.cuda.device(_same_device(k, v, k_cache, v_cache, positions, rope_cos, rope_sin, row_counts)):
-            check(_lib.load().ovf_kv_q4_append(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), _ptr(positions),
-                                               _ptr(row_counts), n_seq, rows, n_kv_heads, head_dim, max_ctx, _ptr(rope_cos),
-                                               _ptr(rope_sin), int(split_half), _stream()), "kv_q4_append")
+        n_seq, rows, spans = KvCacheQ4.spans(k_cache, v_cache, positions, k, "k", n_kv_heads, head_dim, max_ctx, rope_cos,
+                                             rope_sin, row_counts, n_kv_heads)
+        if v is None:
+            raise ValueError("v is required")
+        spans += ((v, torch.float32, n_seq * rows * n_kv_heads * head_dim, "v"),)
+        _call("ovf_kv_q4_append", spans, k, v, k_cache, v_cache, positions, row_counts, n_seq, rows, n_kv_heads, head_dim,
+              max_ctx, rope_cos, rope_sin, int(split_half))
 
     @staticmethod
     def read(k_cache, v_cache, positions, n_kv_heads, head_dim, max_ctx, k, v, row_counts=None) -> None:
         """What the caches hold at positions[s] + r, into k, v [n_seq, rows, n_kv_heads * head_dim]."""
-        n_seq, rows = KvCacheQ4.check(k_cache, v_cache, positions, k, n_kv_heads, head_dim, max_ctx, None, None, row_counts,
-                                      n_kv_heads)
-        _need(v, torch.float32, k.numel(), "v")
-        with torch.cuda.device(_same_device(k, v, k_cache, v_cache, positions, row_counts)):
-            check(_lib.load().ovf_kv_q4_read(_ptr(k_cache), _ptr(v_cache), _ptr(positions), _ptr(row_counts), n_seq, rows,
-                                             n_kv_heads, head_dim, max_ctx, _ptr(k), _ptr(v), _stream()), "kv_q4_read")
+        n_seq, rows, spans = KvCacheQ4.spans(k_cache, v_cache, positions, k, "k", n_kv_heads, head_dim, max_ctx, None, None,
+                                             row_counts, n_kv_heads)
+        if v is None:
+            raise ValueError("v is required")
+        spans += ((v, torch.float32, n_seq * rows * n_kv_heads * head_dim, "v"),)
+        _call("ovf_kv_q4_read", spans, k_cache, v_cache, positions, row_counts, n_seq, rows, n_kv_heads, head_dim, max_ctx, k,
+              v)
 
 
 class SpeculativeVerifier:
@@ -551,19 +569,14 @@ class SpeculativeVerifier:
         if logits is None or logits.dim() != 3 or logits.shape[1] < 1:
             raise ValueError("logits must be [n_seq, max_drafts + 1, vocab]")
         n_seq, m, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
-        _need(logits, torch.float32, 0, "logits")
-        if m:
-            _need(drafts, torch.int32, n_seq * m, "drafts")
-        _need(uniforms, torch.float32, n_seq * (m + 1), "uniforms")
-        _need(temperatures, torch.float32, n_seq, "temperatures")
-        _need(accepted, torch.int32, n_seq, "accepted")
-        _need(next_token, torch.int32, n_seq, "next_token")
-        if draft_probs is not None:
-            _need(draft_probs, torch.float32, n_seq * m * vocab, "draft_probs")
-        if draft_counts is not None:
-            _need(draft_counts, torch.int32, n_seq, "draft_counts")
-        with torch.cuda.device(_same_device(logits, drafts if m else None, uniforms, temperatures, accepted, next_token,
-                                            draft_probs, draft_counts)):
-            check(_lib.load().ovf_verify_drafts(_ptr(logits), _ptr(draft_probs) if m else None, _ptr(drafts) if m else None,
-                                                _ptr(draft_counts), _ptr(uniforms), _ptr(temperatures), n_seq, m, vocab,
-                                                _ptr(accepted), _ptr(next_token), _stream()), "verify_drafts")
+        if m == 0:
+            drafts = draft_probs = None
+        if uniforms is None or temperatures is None or accepted is None or next_token is None or (m and drafts is None):
+            raise ValueError("drafts, uniforms, temperatures, accepted and next_token are required")
+        _call("ovf_verify_drafts",
+              ((logits, torch.float32, 0, "logits"), (drafts, torch.int32, n_seq * m, "drafts"),
+               (uniforms, torch.float32, n_seq * (m + 1), "uniforms"), (temperatures, torch.float32, n_seq, "temperatures"),
+               (accepted, torch.int32, n_seq, "accepted"), (next_token, torch.int32, n_seq, "next_token"),
+               (draft_probs, torch.float32, n_seq * m * vocab, "draft_probs"),
+               (draft_counts, torch.int32, n_seq, "draft_counts")),
+              logits, draft_probs, drafts, draft_counts, uniforms, temperatures, n_seq, m, vocab, accepted, next_token)
