@@ -237,8 +237,9 @@ ovf_status ovf_attention_decode_noalloc(const float *q, const void *k_cache, con
  * real; the others are not read, and their places in an output are left as
  * they are.  A sequence whose rows do not fit max_ctx is left out and sets the
  * error word (ovf_device_error code 4).  Rows are [n_seq][rows][heads *
- * head_dim] fp32.  Buffers of a call must not overlap unless it says so; calls
- * on the same cache are ordered by the caller (one stream, or events).
+ * head_dim] fp32, 16-byte aligned; at most 2^22 rows times heads in a call.
+ * Buffers of a call must not overlap; calls on the same cache are ordered by the
+ * caller (one stream, or events).
  *
  * rope_cos / rope_sin ([max_ctx][head_dim / 2]) rotate keys and queries at
  * their positions as Rope/RopeKernel.cs:46 does; NULL leaves them as they are. */

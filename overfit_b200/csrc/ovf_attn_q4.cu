@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kAqThreads, aq_ctas(NG)) attention_q4_kernel(c
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[g][k] = 0.0f;
             }
-            if (it.w.cos) {  // rotated as q4_rotate does
+            if (it.w.cos) {  // Rope/RopeKernel.cs:46-93, each step rounded by itself
                 const int pos = real ? limit : 0;
                 const float *c = it.w.cos + (size_t)pos * (HD / 2), *sn = it.w.sin + (size_t)pos * (HD / 2);
                 if (!src.split_half) {
@@ -570,7 +570,9 @@ ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_n
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (k_new) {
         OVF_CHECK_ARG(k_cache != v_cache, "attention_q4: keys and values need caches of their own");
-        if ((st = launch_kv_q4_append(src, head_dim, k_new, v_new, s))) return st;
+        OVF_CHECK_ARG(aligned16(k_new) && aligned16(v_new) && aligned16(rope_cos) && aligned16(rope_sin),
+                      "attention_q4: new rows and rope tables must be 16-byte aligned");
+        if ((st = launch_kv_q4_append(src, head_dim, k_new, v_new, s, false))) return st;
     }
     return launch_attention_q4(src, n_heads, head_dim, q, out, scale, scratch, s, false);
 }

@@ -1,128 +1,220 @@
 // ovf_kv_q4.cu — rows of keys and values into the 4-bit cache, and back.
 //
 // Append: RoPE of the keys (Rope/RopeKernel.cs:46-93), then every group of 32
-// dimensions is quantised (ovf_q4.cuh).  A value word holds eight positions of
-// one dimension, so a warp owns a block of eight positions of one head: it
-// reads the block's words, replaces the codes of the positions that are
-// appended and writes them once, and no two warps write the same word.
-// Positions outside the rows keep their codes and parameters.
-// Bound by memory: 8 bytes read and 1.25 written per element pair.
+// dimensions is quantised (ovf_q4.cuh).  Keys: a word holds eight dimensions of
+// one position, so a lane takes those, the lanes of a group agree on its range
+// with two shuffles, and nothing else is shared.  Values: a word holds eight
+// positions of one dimension, so a warp takes a group of a block of eight
+// positions, a lane a dimension; the range of each position is one redux.  A
+// block that the rows fill in part keeps the codes of its other positions.  No
+// two warps write the same word.
+// Bound by memory: 4 bytes read and 0.625 written per element (reading back: the
+// other way round).
+#include <algorithm>
+
 #include "ovf_q4.cuh"
 
 namespace ovf {
 
-static constexpr int kKvQ4Warps = 4;
+static constexpr int kKvQ4Threads = 256;
 
-// Rows of sequence `s` that lie in the 8-position block of this warp:
-// positions [p0, p1), block first position b0.
-struct Q4Block {
-    int b0, p0, p1;
+__device__ __forceinline__ float redux_min(float x) {
+    float y;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float redux_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A key word: eight dimensions (32 g + 8 t ..) of one row and head.
+struct Q4KeyWord {
+    int r, h, g, t;
 };
-__device__ __forceinline__ bool q4_block(const Q4View &w, int blk, Q4Block *b) {
-    b->b0 = ((w.pos >> 3) + blk) * 8;
-    b->p0 = max(w.pos, b->b0);
-    b->p1 = min(w.pos + w.count, b->b0 + 8);
-    return b->p0 < b->p1;
+template <int NG>
+__device__ __forceinline__ Q4KeyWord q4_key_of(int i, int KVH) {
+    Q4KeyWord k;
+    k.t = i & 3;
+    k.g = (i >> 2) % NG;
+    const int v = i / (4 * NG);
+    k.h = v % KVH;
+    k.r = v / KVH;
+    return k;
 }
 
 template <int NG>
-__global__ void __launch_bounds__(kKvQ4Warps * 32) kv_q4_append_kernel(const Q4Source src, const float *k,
-                                                                      const float *v) {
+__device__ __forceinline__ void append_key(const Q4Source &src, const float *k, const Q4View &w, int s) {
     constexpr int HD = NG * 32;
-    const int lane = threadIdx.x & 31;
-    const int h = blockIdx.y >> 1, s = blockIdx.z;
-    const bool values = blockIdx.y & 1;
-    Q4View w;
-    Q4Block b;
-    if (!q4_view(src, s, &w) || !q4_block(w, blockIdx.x * kKvQ4Warps + (threadIdx.x >> 5), &b)) return;
-    uint8_t *tile = (values ? w.v : w.k) + ((size_t)h * w.tiles + b.b0 / kQ4Tile) * q4_tile_bytes(HD);
-    uint32_t *words = reinterpret_cast<uint32_t *>(tile);
+    const int i = blockIdx.x * kKvQ4Threads + threadIdx.x;
+    const Q4KeyWord a = q4_key_of<NG>(i, src.KVH);
+    const bool real = a.r < w.count;
+    if (!__any_sync(0xFFFFFFFFu, real)) return;
+    const int pos = w.pos + (real ? a.r : 0);
+    float x[8];
+    if (real) {
+        const float4 *p = reinterpret_cast<const float4 *>(k + ((size_t)s * src.rows * src.KVH * NG * 4 + i) * 8);
+        const float4 u = p[0], v = p[1];
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.0f;
+    }
+    if (w.cos) {
+        const float *c = w.cos + (size_t)pos * (HD / 2), *sn = w.sin + (size_t)pos * (HD / 2);
+        const int d = a.g * 32 + a.t * 8;
+        if (!src.split_half) {
+            const float4 cc = *reinterpret_cast<const float4 *>(c + d / 2), ss = *reinterpret_cast<const float4 *>(sn + d / 2);
+            const float cv[4] = {cc.x, cc.y, cc.z, cc.w}, sv[4] = {ss.x, ss.y, ss.z, ss.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x0 = x[2 * j], x1 = x[2 * j + 1];
+                x[2 * j] = fsub(fmul(x0, cv[j]), fmul(x1, sv[j]));
+                x[2 * j + 1] = fadd(fmul(x0, sv[j]), fmul(x1, cv[j]));
+            }
+        } else {
+            const int at = d % (HD / 2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], NG * 2);  // half a head further
+                const float cc = c[at + j], ss = sn[at + j];
+                x[j] = d < HD / 2 ? fsub(fmul(x[j], cc), fmul(other, ss)) : fadd(fmul(other, ss), fmul(x[j], cc));
+            }
+        }
+    }
+    float lo, hi;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = q4_clean(x[j]);
+        lo = j ? fminf(lo, x[j]) : x[j];
+        hi = j ? fmaxf(hi, x[j]) : x[j];
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+    }
+    const Q4Params q = q4_params(lo, hi);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word |= q4_encode(x[j], q) << (4 * j);
+    if (!real) return;
+    uint8_t *tile = w.k + ((size_t)a.h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
+    reinterpret_cast<uint32_t *>(tile)[q4_key_word(NG, pos & 31, a.t, a.g)] = __funnelshift_l(word, word, 2);
+    if (a.t == 0)
+        *reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(tile + q4_code_bytes(HD)) +
+                                     q4_key_param(NG, pos & 31, a.g)) = __halves2half2(q.D, q.M);
+}
+
+// A group of a block of eight positions: rows r0 .. r0 + 7, of which [0, count) are real.
+struct Q4ValueBlock {
+    int b, h, g, r0;
+};
+template <int NG>
+__device__ __forceinline__ bool q4_value_of(int i, const Q4View &w, int KVH, Q4ValueBlock *v) {
+    v->g = i % NG;
+    v->h = i / NG % KVH;
+    v->b = (w.pos >> 3) + i / (NG * KVH);
+    v->r0 = v->b * 8 - w.pos;
+    return v->r0 < w.count;
+}
+
+template <int NG>
+__device__ __forceinline__ void append_value(const Q4Source &src, const float *v, const Q4View &w, int s) {
+    constexpr int HD = NG * 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Q4ValueBlock a;
+    if (!q4_value_of<NG>(blockIdx.x * (kKvQ4Threads / 32) + warp, w, src.KVH, &a)) return;
+    const int j0 = max(0, -a.r0), j1 = min(8, w.count - a.r0), t = a.b & 3;
+    uint8_t *tile = w.v + ((size_t)a.h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
+    uint32_t *word = reinterpret_cast<uint32_t *>(tile) + q4_value_word(a.g, lane & 7, t, lane >> 3);
     __half *params = reinterpret_cast<__half *>(tile + q4_code_bytes(HD));
-    const int t = (b.b0 & 31) >> 3;
-    const float *x0 = (values ? v : k) + ((size_t)s * src.rows * src.KVH + h) * HD + lane;
-    uint32_t old[NG];
-    if (values) {
+    const float *x0 = v + (((size_t)s * src.rows + a.r0) * src.KVH + a.h) * HD + a.g * 32 + lane;
+    float x[8], lo = 0.0f, hi = 0.0f;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) old[g] = words[q4_value_word(g, lane & 7, t, lane >> 3)];
+    for (int j = 0; j < 8; ++j) x[j] = j >= j0 && j < j1 ? x0[(long long)j * src.KVH * HD] : 0.0f;
+    uint32_t old = 0;
+    if (j0 > 0 || j1 < 8) old = *word;
+    // lane j forms the parameters of position j
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = q4_clean(x[j]);
+        const float l = redux_min(x[j]), h = redux_max(x[j]);
+        if (lane == j) lo = l, hi = h;
     }
-    for (int p = b.p0; p < b.p1; ++p) {
-        float x[NG];
-#pragma unroll
-        for (int g = 0; g < NG; ++g) x[g] = x0[(size_t)(p - w.pos) * src.KVH * HD + g * 32];
-        if (!values && w.cos)
-            q4_rotate<NG>(x, w.cos + (size_t)p * (HD / 2), w.sin + (size_t)p * (HD / 2), src.split_half, lane);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const float y = q4_clean(x[g]);
-            float lo = y, hi = y;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-            }
-            const Q4Params q = q4_params(lo, hi);
-            const uint32_t c = q4_encode(y, q);
-            if (values) {
-                old[g] = q4_with_code(old[g], p & 7, c);
-                if (lane == 0) {
-                    const int i = q4_value_param(g, t, p & 7);
-                    params[i] = q.D;
-                    params[i + 32] = q.M;
-                }
-            } else {
-                // lanes 8 t .. 8 t + 7 hold the codes of one word
-                uint32_t u = __funnelshift_l(c, c, q4_shift(lane & 7));
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) u |= __shfl_xor_sync(0xFFFFFFFFu, u, o);
-                if ((lane & 7) == 0) words[q4_key_word(NG, p & 31, lane >> 3, g)] = u;
-                if (lane == 0) *reinterpret_cast<__half2 *>(params + q4_key_param(NG, p & 31, g)) = __halves2half2(q.D, q.M);
-            }
-        }
+    const Q4Params q = q4_params(lo, hi);
+    if (lane >= j0 && lane < j1) {
+        const int at = q4_value_param(a.g, t, lane);
+        params[at] = q.D;
+        params[at + 32] = q.M;
     }
-    if (values) {
+    uint32_t codes = __funnelshift_r(old, old, 2);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) words[q4_value_word(g, lane & 7, t, lane >> 3)] = old[g];
+    for (int j = 0; j < 8; ++j) {
+        Q4Params p;
+        p.m = __shfl_sync(0xFFFFFFFFu, q.m, j);
+        p.d = __shfl_sync(0xFFFFFFFFu, q.d, j);
+        p.inv = __shfl_sync(0xFFFFFFFFu, q.inv, j);
+        if (j >= j0 && j < j1) codes = (codes & ~(15u << (4 * j))) | q4_encode(x[j], p) << (4 * j);
     }
+    *word = __funnelshift_l(codes, codes, 2);
 }
 
 template <int NG>
-__global__ void __launch_bounds__(kKvQ4Warps * 32) kv_q4_read_kernel(const Q4Source src, float *k, float *v) {
-    constexpr int HD = NG * 32;
-    const int lane = threadIdx.x & 31;
-    const int h = blockIdx.y >> 1, s = blockIdx.z;
-    const bool values = blockIdx.y & 1;
+__global__ void __launch_bounds__(kKvQ4Threads) kv_q4_append_kernel(const Q4Source src, const float *k, const float *v) {
     Q4View w;
-    Q4Block b;
-    if (!q4_view(src, s, &w) || !q4_block(w, blockIdx.x * kKvQ4Warps + (threadIdx.x >> 5), &b)) return;
-    const uint8_t *tile = (values ? w.v : w.k) + ((size_t)h * w.tiles + b.b0 / kQ4Tile) * q4_tile_bytes(HD);
-    const uint32_t *words = reinterpret_cast<const uint32_t *>(tile);
-    const __half *params = reinterpret_cast<const __half *>(tile + q4_code_bytes(HD));
-    const int t = (b.b0 & 31) >> 3;
-    float *y0 = (values ? v : k) + ((size_t)s * src.rows * src.KVH + h) * HD + lane;
-    for (int p = b.p0; p < b.p1; ++p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (!q4_view(src, blockIdx.z, &w)) return;
+    if (blockIdx.y) append_value<NG>(src, v, w, blockIdx.z);
+    else append_key<NG>(src, k, w, blockIdx.z);
+}
+
+template <int NG>
+__global__ void __launch_bounds__(kKvQ4Threads) kv_q4_read_kernel(const Q4Source src, float *k, float *v) {
+    constexpr int HD = NG * 32;
+    const int s = blockIdx.z;
+    Q4View w;
+    if (!q4_view(src, s, &w)) return;
+    if (blockIdx.y == 0) {
+        const int i = blockIdx.x * kKvQ4Threads + threadIdx.x;
+        const Q4KeyWord a = q4_key_of<NG>(i, src.KVH);
+        if (a.r >= w.count) return;
+        const int p = (w.pos + a.r) & 31;
+        const uint8_t *tile = w.k + ((size_t)a.h * w.tiles + (w.pos + a.r) / kQ4Tile) * q4_tile_bytes(HD);
+        const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[q4_key_word(NG, p, a.t, a.g)];
+        const __half2 dm = *reinterpret_cast<const __half2 *>(reinterpret_cast<const __half *>(tile + q4_code_bytes(HD)) +
+                                                              q4_key_param(NG, p, a.g));
+        float x[8];
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            uint32_t c;
-            __half D, M;
-            if (values) {
-                c = q4_code(words[q4_value_word(g, lane & 7, t, lane >> 3)], p & 7);
-                D = params[q4_value_param(g, t, p & 7)];
-                M = params[q4_value_param(g, t, p & 7) + 32];
-            } else {
-                c = q4_code(words[q4_key_word(NG, p & 31, lane >> 3, g)], lane & 7);
-                D = params[q4_key_param(NG, p & 31, g)];
-                M = params[q4_key_param(NG, p & 31, g) + 1];
-            }
-            y0[(size_t)(p - w.pos) * src.KVH * HD + g * 32] = q4_value(c, D, M);
-        }
+        for (int j = 0; j < 8; ++j) x[j] = q4_value(q4_code(word, j), __low2half(dm), __high2half(dm));
+        float4 *y = reinterpret_cast<float4 *>(k + ((size_t)s * src.rows * src.KVH * NG * 4 + i) * 8);
+        y[0] = make_float4(x[0], x[1], x[2], x[3]);
+        y[1] = make_float4(x[4], x[5], x[6], x[7]);
+        return;
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Q4ValueBlock a;
+    if (!q4_value_of<NG>(blockIdx.x * (kKvQ4Threads / 32) + warp, w, src.KVH, &a)) return;
+    const int t = a.b & 3;
+    const uint8_t *tile = w.v + ((size_t)a.h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
+    const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[q4_value_word(a.g, lane & 7, t, lane >> 3)];
+    const __half *params = reinterpret_cast<const __half *>(tile + q4_code_bytes(HD));
+    float *y = v + (((size_t)s * src.rows + a.r0) * src.KVH + a.h) * HD + a.g * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int at = q4_value_param(a.g, t, j);
+        if (a.r0 + j >= 0 && a.r0 + j < w.count) y[(long long)j * src.KVH * HD] = q4_value(q4_code(word, j), params[at], params[at + 32]);
     }
 }
 
 bool q4_supported(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
-static dim3 kv_q4_grid(const Q4Source &src) {
-    const int blocks = (src.rows + 14) / 8;  // rows that start anywhere in a block
-    return dim3((blocks + kKvQ4Warps - 1) / kKvQ4Warps, src.KVH * 2, src.n_seq);
+static dim3 kv_q4_grid(const Q4Source &src, int hd) {
+    const int64_t keys = (int64_t)src.rows * src.KVH * (hd / 8);  // words
+    const int64_t values = (int64_t)((src.rows + 14) / 8) * src.KVH * (hd / 32) * 32;  // rows may start anywhere in a block
+    return dim3((unsigned)((std::max(keys, values) + kKvQ4Threads - 1) / kKvQ4Threads), 2, src.n_seq);
 }
 
 #define OVF_Q4_HD(hd, CALL)              \
@@ -133,17 +225,18 @@ static dim3 kv_q4_grid(const Q4Source &src) {
         default: CALL(8); break;         \
     }
 
-ovf_status launch_kv_q4_append(const Q4Source &src, int hd, const float *k, const float *v, cudaStream_t st) {
-    const dim3 grid = kv_q4_grid(src);
-#define OVF_CALL(NG) kv_q4_append_kernel<NG><<<grid, kKvQ4Warps * 32, 0, st>>>(src, k, v)
+ovf_status launch_kv_q4_append(const Q4Source &src, int hd, const float *k, const float *v, cudaStream_t st, bool pdl) {
+    cudaError_t e = cudaSuccess;
+#define OVF_CALL(NG) \
+    e = launch_pdl(kv_q4_append_kernel<NG>, kv_q4_grid(src, hd), dim3(kKvQ4Threads), 0, st, pdl, src, k, v)
     OVF_Q4_HD(hd, OVF_CALL)
 #undef OVF_CALL
-    return cuda_status(cudaGetLastError(), "kv_q4_append");
+    return cuda_status(e, "kv_q4_append");
 }
 
 ovf_status launch_kv_q4_read(const Q4Source &src, int hd, float *k, float *v, cudaStream_t st) {
-    const dim3 grid = kv_q4_grid(src);
-#define OVF_CALL(NG) kv_q4_read_kernel<NG><<<grid, kKvQ4Warps * 32, 0, st>>>(src, k, v)
+    const dim3 grid = kv_q4_grid(src, hd);
+#define OVF_CALL(NG) kv_q4_read_kernel<NG><<<grid, kKvQ4Threads, 0, st>>>(src, k, v)
     OVF_Q4_HD(hd, OVF_CALL)
 #undef OVF_CALL
     return cuda_status(cudaGetLastError(), "kv_q4_read");
@@ -160,6 +253,8 @@ ovf_status q4_source(const char *what, const void *k_cache, const void *v_cache,
     OVF_CHECK_ARG(rows >= 0 && rows <= max_ctx, "%s: %d rows do not fit max_ctx %d", what, rows, max_ctx);
     OVF_CHECK_ARG(k_cache && v_cache && positions, "%s: null buffer", what);
     OVF_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "%s: caches must be 16-byte aligned", what);
+    OVF_CHECK_ARG((int64_t)rows * n_kv_heads <= (1 << 22), "%s: %d rows of %d heads in one call (at most 2^22 in all)", what,
+                  rows, n_kv_heads);
     OVF_CHECK_ARG(!rope_cos == !rope_sin, "%s: rope_cos and rope_sin go together", what);
     Q4Source s{};
     s.k = static_cast<uint8_t *>(const_cast<void *>(k_cache));
@@ -197,9 +292,11 @@ ovf_status ovf_kv_q4_append(const float *k, const float *v, void *k_cache, void 
                               head_dim, max_ctx, rope_cos, rope_sin, split_half, &src);
     if (st) return st;
     OVF_CHECK_ARG(k && v, "kv_q4_append: null buffer");
+    OVF_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(rope_cos) && aligned16(rope_sin),
+                  "kv_q4_append: buffers must be 16-byte aligned");
     OVF_CHECK_ARG(k_cache != v_cache, "kv_q4_append: keys and values need caches of their own");
     if (n_seq == 0 || rows == 0) return OVF_OK;
-    return launch_kv_q4_append(src, head_dim, k, v, reinterpret_cast<cudaStream_t>(stream));
+    return launch_kv_q4_append(src, head_dim, k, v, reinterpret_cast<cudaStream_t>(stream), false);
 }
 
 ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_t *positions, const int32_t *row_counts,
@@ -211,6 +308,7 @@ ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_
                               max_ctx, nullptr, nullptr, 0, &src);
     if (st) return st;
     OVF_CHECK_ARG(k && v && k != v, "kv_q4_read: null buffer, or one for both sides");
+    OVF_CHECK_ARG(aligned16(k) && aligned16(v), "kv_q4_read: buffers must be 16-byte aligned");
     if (n_seq == 0 || rows == 0) return OVF_OK;
     return launch_kv_q4_read(src, head_dim, k, v, reinterpret_cast<cudaStream_t>(stream));
 }

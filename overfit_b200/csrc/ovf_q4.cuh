@@ -51,12 +51,6 @@ __device__ __forceinline__ int q4_shift(int i) { return (4 * i + 2) & 31; }
 __device__ __forceinline__ uint32_t q4_code(uint32_t word, int i) {
     return __funnelshift_r(word, word, q4_shift(i)) & 15u;
 }
-// `word` with code i replaced.
-__device__ __forceinline__ uint32_t q4_with_code(uint32_t word, int i, uint32_t c) {
-    const uint32_t r = __funnelshift_r(word, word, q4_shift(i));
-    const uint32_t n = (r & ~15u) | c;
-    return __funnelshift_l(n, n, q4_shift(i));
-}
 __device__ __forceinline__ float q4_value(uint32_t c, __half D, __half M) {
     return __half2float(__hfma(D, __ushort_as_half((unsigned short)(0x3C00u | (c << 6))), M));
 }
@@ -83,39 +77,6 @@ __device__ __forceinline__ Q4Params q4_params(float lo, float hi) {
 __device__ __forceinline__ uint32_t q4_encode(float x, const Q4Params &p) {
     const float c = rintf(fmul(fsub(fsub(x, p.m), p.d), p.inv));
     return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
-}
-
-// One head vector in a warp: lane l holds dimensions 32 g + l in x[g].
-// Rotates it by the cos / sin row [hd / 2] of its position as
-// Rope/RopeKernel.cs:46-93 does (adjacent or split-half pairs).
-template <int NG>
-__device__ __forceinline__ void q4_rotate(float (&x)[NG], const float *cos_row, const float *sin_row, int split_half,
-                                          int lane) {
-    constexpr int HD = NG * 32;
-    float y[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        float other;
-        int i;       // pair
-        bool first;  // this lane holds the pair's first element
-        if (!split_half) {
-            other = __shfl_xor_sync(0xFFFFFFFFu, x[g], 1);
-            i = g * 16 + (lane >> 1);
-            first = (lane & 1) == 0;
-        } else if (NG == 1) {
-            other = __shfl_xor_sync(0xFFFFFFFFu, x[g], 16);
-            i = lane & 15;
-            first = lane < 16;
-        } else {
-            other = x[(g + NG / 2) % NG];
-            i = (g * 32 + lane) % (HD / 2);
-            first = g < NG / 2;
-        }
-        const float c = cos_row[i], s = sin_row[i];
-        y[g] = first ? fsub(fmul(x[g], c), fmul(other, s)) : fadd(fmul(other, s), fmul(x[g], c));
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) x[g] = y[g];
 }
 
 // The cache of one sequence, for a batch of sessions whose caches are apart.
@@ -180,7 +141,7 @@ bool q4_supported(int hd);
 ovf_status q4_source(const char *what, const void *k_cache, const void *v_cache, const int32_t *positions,
                      const int32_t *row_counts, int32_t n_seq, int32_t rows, int32_t n_kv_heads, int32_t head_dim,
                      int32_t max_ctx, const float *rope_cos, const float *rope_sin, int32_t split_half, Q4Source *src);
-ovf_status launch_kv_q4_append(const Q4Source &src, int hd, const float *k, const float *v, cudaStream_t st);
+ovf_status launch_kv_q4_append(const Q4Source &src, int hd, const float *k, const float *v, cudaStream_t st, bool pdl);
 ovf_status launch_kv_q4_read(const Q4Source &src, int hd, float *k, float *v, cudaStream_t st);
 // ovf_attn_q4.cu: rows of queries over the 4-bit cache; `scratch` of
 // attn_q4_scratch_bytes.

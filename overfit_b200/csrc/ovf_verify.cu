@@ -13,9 +13,11 @@
 //
 // A decision must not depend on rounding: a vocabulary has 10^5 borders, and one
 // that falls the other way changes a token.  The rows' sums are first formed from
-// fp32 exponentials, off by less than 2^-16; where a draft's decision is nearer to
-// its border than that (about one in 10^5), its row is summed again in 64 bits.
-// The row that a token is drawn from is summed in 64 bits always.
+// fp32 exponentials.  A lane rescales its sum when it meets a larger logit, at
+// most once per 16 elements, 256 times in the longest row (2^24 over 8 x 512
+// lanes), each time off by 2^-21.4 at most, so a sum is off by less than 2^-12;
+// where a draft's decision is nearer to its border than that, its row is summed
+// again in 64 bits.  The row that a token is drawn from is summed in 64 bits always.
 //
 // A cluster of 8 or 16 CTAs takes a sequence: every CTA a part of each row, all
 // rows one behind the other, so that memory streams while sums are formed; the
@@ -38,21 +40,21 @@ static constexpr int kVfThreads = 512, kVfWarps = kVfThreads / 32;
 static constexpr int kVfRows = 1024;        // max_drafts + 1
 static constexpr int kVfCluster = 16;       // at most
 
-// e^x in 64 bits, off by a few 2^-52: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from
+// e^x in 64 bits, off by about 2^-48: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from
 // the table of 2^(i / 32) that exp_libm (ovf_common.cuh) has.  ln 2 is taken in two parts, the first of 24 bits, so
 // that its product with n is exact.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
     if (!(x > -700.0)) return x < -746.0 ? 0.0 : exp(x);  // results below the normal numbers, and NaN
-    const double n = rint(x * (32.0 / 0.693147180559945309417));
+    const double shift = 0x1.8p52;  // its sum with a number ends in that number's nearest integer
+    const double kd = fma(x, 32.0 / 0.693147180559945309417, shift), n = kd - shift;
     double r = fma(n, -0x1.62e4300000000p-1 / 32.0, x);
-    r = fma(n, -(-0x1.05c610ca86c39p-29) / 32.0, r);
-    double y = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    y = fma(y, r, 1.0 / 24.0);
+    r = fma(n, 0x1.05c610ca86c39p-29 / 32.0, r);
+    double y = fma(r, 1.0 / 120.0, 1.0 / 24.0);
     y = fma(y, r, 1.0 / 6.0);
     y = fma(y, r, 0.5);
     y = fma(y, r, 1.0);
     y = fma(y, r, 1.0);
-    const int k = (int)n;
+    const int k = __double2loint(kd);
     return y * __longlong_as_double((long long)(tab[k & 31] + ((unsigned long long)(long long)k << 47)));
 }
 
@@ -95,16 +97,19 @@ __device__ __forceinline__ float4 vf_load4(const float *row, int V, int shift, i
 }
 __device__ __forceinline__ int vf_shift(const float *row) { return (int)(reinterpret_cast<uintptr_t>(row) >> 2) & 3; }
 
+static constexpr int kVfBlock = 32;         // rows whose warps' results are joined at a time
+static_assert(kVfBlock * kVfWarps == kVfThreads, "a thread joins one warp's result of one row");
+
 struct VfShared {
     float m[kVfRows];          // this CTA's part of every row: largest logit,
     int at[kVfRows];           // its first place (greedy),
-    double sum[kVfRows];       // sum of exponentials (NaN: a row with a NaN or +infinity)
+    float sum[kVfRows];        // sum of exponentials (NaN: a row with a NaN or +infinity)
     float row_m[kVfRows];      // the same of the whole rows
     int row_at[kVfRows];
-    float wm[2][kVfWarps];
-    int wat[2][kVfWarps];
-    double wsum[2][kVfWarps];
-    double part[kVfWarps];               // the drawing: sums of this CTA's warps' parts
+    float wm[kVfBlock][kVfWarps];  // of a block of rows, the warps' parts
+    int wat[kVfBlock][kVfWarps];
+    float wsum[kVfBlock][kVfWarps];
+    double part[2][kVfWarps];            // the drawing: sums of this CTA's warps' parts (two calls of vf_gather)
     double all[kVfCluster * kVfWarps];   // of all CTAs'
     unsigned long long tab[32];
     int first, token;
@@ -112,8 +117,7 @@ struct VfShared {
 
 // The (largest, first place of it, sum) of N lanes as one, in every lane.
 template <int N>
-__device__ __forceinline__ void vf_join(float &m, int &at, double &sum, bool greedy, double inv,
-                                        const unsigned long long *tab) {
+__device__ __forceinline__ void vf_join(float &m, int &at, float &sum, bool greedy, float c) {
     float top = m;
 #pragma unroll
     for (int o = N / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -122,7 +126,7 @@ __device__ __forceinline__ void vf_join(float &m, int &at, double &sum, bool gre
 #pragma unroll
         for (int o = N / 2; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xFFFFFFFFu, at, o));
     } else {
-        sum *= vf_exp(((double)m - top) * inv, tab);
+        sum *= vf_ex2((m - top) * c);
     }
 #pragma unroll
     for (int o = N / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
@@ -132,13 +136,17 @@ __device__ __forceinline__ void vf_join(float &m, int &at, double &sum, bool gre
 enum : int { VF_ACCEPT = 0, VF_REJECT = 1, VF_NEAR = 2, VF_BAD = 3 };
 
 // The sum over the cluster of a value of every warp's part, in the order of the parts; all[] holds them.
-__device__ __forceinline__ double vf_gather(VfShared &sh, double mine, int size, int warp, int lane) {
+// Calls take turns with the two sets of part: a CTA that writes one again has passed a barrier that all its
+// readers have reached behind their reads.
+__device__ __forceinline__ double vf_gather(VfShared &sh, double mine, int size, int warp, int lane, int &turn) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-    if (lane == 0) sh.part[warp] = mine;
+    if (lane == 0) sh.part[turn][warp] = mine;
     cluster_barrier();
-    for (int i = threadIdx.x; i < size * kVfWarps; i += kVfThreads) sh.all[i] = cluster_read(&sh.part[i % kVfWarps], i / kVfWarps);
-    cluster_barrier();  // (also: part may be written again)
+    for (int i = threadIdx.x; i < size * kVfWarps; i += kVfThreads)
+        sh.all[i] = cluster_read(&sh.part[turn][i % kVfWarps], i / kVfWarps);
+    turn ^= 1;
+    __syncthreads();
     double s = 0.0;
     for (int i = lane; i < size * kVfWarps; i += 32) s += sh.all[i];
 #pragma unroll
@@ -166,57 +174,72 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
     const double inv = 1.0 / (double)T;
     __syncthreads();
 
-    // every row's largest logit and sum (greedy: and the first place of it), this CTA's part
-    for (int j = 0; j <= n; ++j) {
-        const float *x = logits + (size_t)j * V;
-        const int shift = vf_shift(x), groups = (V + shift + 3) / 4;
-        float m = -FLT_MAX;
-        int at = 0x7FFFFFFF;
-        double sum = 0.0;
-        if (greedy) {
-            bool bad = false;
-            for (int g = rank * kVfThreads + tid; g < groups; g += size * kVfThreads) {
-                const float4 v = vf_load4(x, V, shift, g, -INFINITY);
-                const float e[4] = {v.x, v.y, v.z, v.w};
+    // Every row's largest logit and sum (greedy: and the first place of it), this CTA's part.  A warp takes its
+    // part of one row behind the other, four loads a lane at a time and the next four under way.
+    {
+        const int step = size * kVfThreads, first = rank * kVfThreads + tid;
+        float4 v[4];
+        auto load = [&](int j, int g) {
+            const float *x = logits + (size_t)j * V;
+            const int shift = vf_shift(x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    bad |= e[i] != e[i];
-                    const int k = 4 * g - shift + i;
-                    if (e[i] > m || (e[i] == m && k < at)) m = e[i], at = k;
+            for (int i = 0; i < 4; ++i) v[i] = vf_load4(x, V, shift, g + i * step, -INFINITY);
+        };
+        load(0, first);
+        for (int j0 = 0; j0 <= n; j0 += kVfBlock) {
+            const int j1 = min(n + 1, j0 + kVfBlock);
+            for (int j = j0; j < j1; ++j) {
+                const int shift = vf_shift(logits + (size_t)j * V), groups = (V + shift + 3) / 4;
+                float m = -FLT_MAX;
+                int at = 0x7FFFFFFF;
+                double sum = 0.0;
+                bool bad = false;
+                for (int g = first; g - first < groups; g += 4 * step) {
+                    float4 w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = v[i];
+                    if (g - first + 4 * step < groups) load(j, g + 4 * step);
+                    else if (j < n) load(j + 1, first);
+                    float top = w[0].x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(w[i].x, w[i].y), fmaxf(w[i].z, w[i].w)));
+                    if (greedy) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float e[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                bad |= e[k] != e[k];
+                                const int place = 4 * (g + i * step) - shift + k;
+                                if (e[k] > m || (e[k] == m && place < at)) m = e[k], at = place;
+                            }
+                        }
+                    } else {
+                        if (top > m) {
+                            sum *= (double)vf_ex2((m - top) * c);
+                            m = top;
+                        }
+                        float part = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            part += (vf_ex2((w[i].x - m) * c) + vf_ex2((w[i].y - m) * c)) +
+                                    (vf_ex2((w[i].z - m) * c) + vf_ex2((w[i].w - m) * c));
+                        sum += (double)part;
+                    }
                 }
+                float fsum = bad ? __int_as_float(0x7fc00000) : (float)sum;
+                vf_join<32>(m, at, fsum, greedy, c);
+                if (lane == 0) sh.wm[j - j0][warp] = m, sh.wat[j - j0][warp] = at, sh.wsum[j - j0][warp] = fsum;
             }
-            if (bad) sum = __longlong_as_double(0x7ff8000000000000ll);
-        } else {
-            const int step = size * kVfThreads;
-            auto add = [&](const float4 &v) {
-                const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-                if (top > m) {
-                    sum *= vf_exp(((double)m - top) * inv, sh.tab);
-                    m = top;
-                }
-                sum += (double)((vf_ex2((v.x - m) * c) + vf_ex2((v.y - m) * c)) +
-                                (vf_ex2((v.z - m) * c) + vf_ex2((v.w - m) * c)));
-            };
-            int g = rank * kVfThreads + tid;
-            for (; g + 3 * step < groups; g += 4 * step) {
-                float4 v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = vf_load4(x, V, shift, g + i * step, -INFINITY);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) add(v[i]);
+            __syncthreads();
+            const int r = tid / kVfWarps, w = tid % kVfWarps;
+            if (j0 + (warp * 32) / kVfWarps < j1) {  // (whole warps: two rows each)
+                float m = sh.wm[r][w], sum = sh.wsum[r][w];
+                int at = sh.wat[r][w];
+                vf_join<kVfWarps>(m, at, sum, greedy, c);
+                if (w == 0 && j0 + r < j1) sh.m[j0 + r] = m, sh.at[j0 + r] = at, sh.sum[j0 + r] = sum;
             }
-            for (; g < groups; g += step) add(vf_load4(x, V, shift, g, -INFINITY));
-        }
-        vf_join<32>(m, at, sum, greedy, inv, sh.tab);
-        const int b = j & 1;  // two sets: a warp may be a row ahead of the one that joins
-        if (lane == 0) sh.wm[b][warp] = m, sh.wat[b][warp] = at, sh.wsum[b][warp] = sum;
-        __syncthreads();
-        if (warp == (j & (kVfWarps - 1))) {
-            m = lane < kVfWarps ? sh.wm[b][lane] : -FLT_MAX;
-            at = lane < kVfWarps ? sh.wat[b][lane] : 0x7FFFFFFF;
-            sum = lane < kVfWarps ? sh.wsum[b][lane] : 0.0;
-            vf_join<kVfWarps>(m, at, sum, greedy, inv, sh.tab);
-            if (lane == 0) sh.m[j] = m, sh.at[j] = at, sh.sum[j] = sum;
+            __syncthreads();
         }
     }
     cluster_barrier();
@@ -228,20 +251,18 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         const int j = tid + i * kVfThreads;
         state[i] = VF_ACCEPT;
         if (j > n) continue;
-        float m = -FLT_MAX;
+        float m = -FLT_MAX, sum = 0.0f;
         int at = 0x7FFFFFFF;
-        double sum = 0.0;
         for (int w = 0; w < (int)size; ++w) m = fmaxf(m, cluster_read(&sh.m[j], w));
         for (int w = 0; w < (int)size; ++w) {
-            const float m2 = cluster_read(&sh.m[j], w);
-            const double sum2 = cluster_read(&sh.sum[j], w);
-            sum += greedy ? sum2 : sum2 * vf_exp(((double)m2 - m) * inv, sh.tab);
-            if (m2 == m) at = min(at, cluster_read(&sh.at[j], w));
+            const float m2 = cluster_read(&sh.m[j], w), sum2 = cluster_read(&sh.sum[j], w);
+            sum += greedy ? sum2 : sum2 * vf_ex2((m2 - m) * c);
+            if (greedy && m2 == m) at = min(at, cluster_read(&sh.at[j], w));
         }
         sh.row_m[j] = m;
         sh.row_at[j] = at;
         const int d = j < n ? drafts[j] : -1;
-        if (sum != sum || !(m < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0)) {
+        if (sum != sum || !(m < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0f)) {
             state[i] = VF_BAD;
         } else if (j == n) {
             state[i] = VF_REJECT;  // the row behind the last draft
@@ -252,13 +273,13 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         } else {
             const double e = vf_exp(((double)logits[(size_t)j * V + d] - (double)m) * inv, sh.tab);
             const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + j) * V + d] : 1.0;
-            const double limit = (double)u[j] * q * sum;
-            state[i] = fabs(limit - e) <= 0x1p-16 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
+            const double limit = (double)u[j] * q * (double)sum;
+            state[i] = fabs(limit - e) <= 0x1p-12 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
         }
     }
 
     // the first row that is not an accepted draft
-    int k = -1, st = VF_ACCEPT;
+    int k = -1, st = VF_ACCEPT, turn = 0;
     const int per = (int)(((size_t)V + 3 + size * kVfWarps * 128 - 1) / (size * kVfWarps * 128));  // 128 elements a step
     const int steps0 = (int)(rank * kVfWarps + warp) * per;  // this warp's part of a row: steps [steps0, steps0 + per)
     while (true) {
@@ -284,7 +305,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             sum += (vf_exp(((double)v.x - m) * inv, sh.tab) + vf_exp(((double)v.y - m) * inv, sh.tab)) +
                    (vf_exp(((double)v.z - m) * inv, sh.tab) + vf_exp(((double)v.w - m) * inv, sh.tab));
         }
-        const double total = vf_gather(sh, sum, size, warp, lane);
+        const double total = vf_gather(sh, sum, size, warp, lane, turn);
         const int d = drafts[k];
         const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + k) * V + d] : 1.0;
         if (!((double)u[k] * q * total < vf_exp(((double)x[d] - m) * inv, sh.tab))) {
@@ -325,30 +346,44 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
                 sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
             q = q0;
-            scale = 1.0 / vf_gather(sh, sum, size, warp, lane);
+            scale = 1.0 / vf_gather(sh, sum, size, warp, lane, turn);
         }
         double sum = 0.0;
         for (int i = steps0; i < steps0 + per; ++i) {
             weight4(i, scale, w);
             sum += (w[0] + w[1]) + (w[2] + w[3]);
         }
-        const double rest = vf_gather(sh, sum, size, warp, lane);
+        const double rest = vf_gather(sh, sum, size, warp, lane, turn);
         const double target = (double)u[p.max_drafts] * rest;
         // the part that holds the token, and what lies before it (every warp finds the same)
-        double before = 0.0, base = 0.0;
-        int part = -1, last = -1;
-        for (int i = 0; i < (int)size * kVfWarps; ++i) {
-            const double y = sh.all[i];
+        const int entries = (int)size * kVfWarps / 32;  // of a lane, one behind the other
+        double own = 0.0, base = 0.0;
+        for (int i = 0; i < entries; ++i) own += sh.all[lane * entries + i];
+        double before = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xFFFFFFFFu, before, o);
+            if (lane >= o) before += y;
+        }
+        before -= own;
+        int part = 0x7FFFFFFF, last = -1;
+        for (int i = 0; i < entries; ++i) {
+            const double y = sh.all[lane * entries + i];
             if (y > 0.0) {
-                last = i;
-                if (before + y > target) {
-                    part = i;
-                    base = before;
-                    break;
-                }
+                last = lane * entries + i;
+                if (part == 0x7FFFFFFF && before + y > target) part = last, base = before;
             }
             before += y;
         }
+        const int mine = part;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            part = min(part, __shfl_xor_sync(0xFFFFFFFFu, part, o));
+            last = max(last, __shfl_xor_sync(0xFFFFFFFFu, last, o));
+        }
+        const unsigned holder = __ballot_sync(0xFFFFFFFFu, mine == part);
+        base = __shfl_sync(0xFFFFFFFFu, base, __ffs(holder) - 1);
+        if (part == 0x7FFFFFFF) part = -1;
         const bool over = part >= 0;
         if (!over) part = last;  // (u of 1 or more): the last token of any weight
         if (part == (int)rank * kVfWarps + warp) {
@@ -356,13 +391,14 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             double run = base;
             for (int i = steps0; i < steps0 + per && found < 0; ++i) {
                 weight4(i, scale, w);
-                double mine = (w[0] + w[1]) + (w[2] + w[3]), incl = mine;
+                const double four = (w[0] + w[1]) + (w[2] + w[3]);
+                double incl = four;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
                     if (lane >= o) incl += y;
                 }
-                double cum = run + (incl - mine);
+                double cum = run + (incl - four);
                 int hit = 0x7FFFFFFF, any = -1;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
