@@ -19,10 +19,13 @@
 // where a draft's decision is nearer to its border than that, its row is summed
 // again in 64 bits.  The row that a token is drawn from is summed in 64 bits always.
 //
-// A cluster of 8 or 16 CTAs takes a sequence: every CTA a part of each row, all
-// rows one behind the other, so that memory streams while sums are formed; the
-// partial sums meet in distributed shared memory.  Bound by the logits' bytes for
-// a batch, by the cluster's barriers and the drawing for one sequence.
+// A cluster of 8 or 16 CTAs takes a sequence.  Its warps cut all rows, one behind
+// the other, into equal runs of steps (128 elements), so that a warp meets one or
+// two rows and reduces as often; the partial sums meet in distributed shared
+// memory, and every CTA forms the same decisions.  For a batch the logits' bytes
+// bound it; for one sequence latency does: three cluster barriers, and code that
+// runs once and comes from memory, which is why its parts are functions, not
+// inlined copies.
 #include <float.h>
 
 #include "ovf_internal.cuh"
@@ -39,12 +42,19 @@ struct VerifyParams {
 static constexpr int kVfThreads = 512, kVfWarps = kVfThreads / 32;
 static constexpr int kVfRows = 1024;        // max_drafts + 1
 static constexpr int kVfCluster = 16;       // at most
+static constexpr int kVfMinCluster = 8;
+static constexpr int kVfStep = 128;         // elements that a warp takes at once
+// rows that a warp's run meets: the run is ceil(rows * steps / warps) steps of `steps` a row
+static constexpr int kVfSlots = kVfRows / (kVfMinCluster * kVfWarps) + 2;
 
-// e^x in 64 bits, off by about 2^-48: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from
-// the table of 2^(i / 32) that exp_libm (ovf_common.cuh) has.  ln 2 is taken in two parts, the first of 24 bits, so
+// What lies below the normal numbers, and NaN.
+__device__ __noinline__ double vf_exp_tail(double x) { return exp(x); }
+
+// e^x in 64 bits, off by about 2^-48: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from the
+// table of 2^(i / 32) that exp_libm (ovf_common.cuh) has.  ln 2 is taken in two parts, the first of 24 bits, so
 // that its product with n is exact.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
-    if (!(x > -700.0)) return x < -746.0 ? 0.0 : exp(x);  // results below the normal numbers, and NaN
+    if (!(x > -700.0)) return x < -746.0 ? 0.0 : vf_exp_tail(x);
     const double shift = 0x1.8p52;  // its sum with a number ends in that number's nearest integer
     const double kd = fma(x, 32.0 / 0.693147180559945309417, shift), n = kd - shift;
     double r = fma(n, -0x1.62e4300000000p-1 / 32.0, x);
@@ -67,248 +77,287 @@ __device__ __forceinline__ float vf_ex2(float x) {
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-template <class T>
-__device__ __forceinline__ T cluster_read(const T *p, int rank) {
-    T v;
-    const uint32_t at = mapa_shared(smem_u32(p), (uint32_t)rank);
-    if (sizeof(T) == 8) {
-        double d;
-        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(d) : "r"(at) : "memory");
-        memcpy(&v, &d, sizeof(T));
-    } else {
-        uint32_t u;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(u) : "r"(at) : "memory");
-        memcpy(&v, &u, sizeof(T));
-    }
+__device__ __forceinline__ float cluster_read(const float *p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(p), (uint32_t)rank)));
+    return v;
+}
+__device__ __forceinline__ int cluster_read(const int *p, int rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), (uint32_t)rank)));
+    return v;
+}
+__device__ __forceinline__ double cluster_read(const double *p, int rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa_shared(smem_u32(p), (uint32_t)rank)));
     return v;
 }
 
-// Elements 4 g - shift .. + 3 of a row (shift: what its address lies behind a
-// 16-byte boundary); those outside the row are `none`.
-__device__ __forceinline__ float4 vf_load4(const float *row, int V, int shift, int g, float none) {
-    const int i = 4 * g - shift;
-    if (i >= 0 && i + 4 <= V) return __ldg(reinterpret_cast<const float4 *>(row + i));
-    float4 v;
-    v.x = i >= 0 && i < V ? row[i] : none;
-    v.y = i + 1 >= 0 && i + 1 < V ? row[i + 1] : none;
-    v.z = i + 2 >= 0 && i + 2 < V ? row[i + 2] : none;
-    v.w = i + 3 >= 0 && i + 3 < V ? row[i + 3] : none;
-    return v;
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
+    return x;
 }
+
+// What a row's address lies behind a 16-byte boundary, in elements.  Lane l's
+// elements of step i are 4 (32 i + l) - shift .. + 3; those outside the row are `none`.
 __device__ __forceinline__ int vf_shift(const float *row) { return (int)(reinterpret_cast<uintptr_t>(row) >> 2) & 3; }
-
-static constexpr int kVfBlock = 32;         // rows whose warps' results are joined at a time
-static_assert(kVfBlock * kVfWarps == kVfThreads, "a thread joins one warp's result of one row");
-
-struct VfShared {
-    float m[kVfRows];          // this CTA's part of every row: largest logit,
-    int at[kVfRows];           // its first place (greedy),
-    float sum[kVfRows];        // sum of exponentials (NaN: a row with a NaN or +infinity)
-    float row_m[kVfRows];      // the same of the whole rows
-    int row_at[kVfRows];
-    float wm[kVfBlock][kVfWarps];  // of a block of rows, the warps' parts
-    int wat[kVfBlock][kVfWarps];
-    float wsum[kVfBlock][kVfWarps];
-    double part[2][kVfWarps];            // the drawing: sums of this CTA's warps' parts (two calls of vf_gather)
-    double all[kVfCluster * kVfWarps];   // of all CTAs'
-    unsigned long long tab[32];
-    int first, token;
-};
-
-// The (largest, first place of it, sum) of N lanes as one, in every lane.
-template <int N>
-__device__ __forceinline__ void vf_join(float &m, int &at, float &sum, bool greedy, float c) {
-    float top = m;
-#pragma unroll
-    for (int o = N / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (greedy) {
-        if (m != top) at = 0x7FFFFFFF;
-#pragma unroll
-        for (int o = N / 2; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(0xFFFFFFFFu, at, o));
-    } else {
-        sum *= vf_ex2((m - top) * c);
-    }
-#pragma unroll
-    for (int o = N / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    m = top;
+__device__ __forceinline__ float4 vf_load4(const float *row, int V, int at, float none) {
+    if (at >= 0 && at + 4 <= V) return __ldg(reinterpret_cast<const float4 *>(row + at));
+    float4 v;
+    v.x = at >= 0 && at < V ? row[at] : none;
+    v.y = at + 1 >= 0 && at + 1 < V ? row[at + 1] : none;
+    v.z = at + 2 >= 0 && at + 2 < V ? row[at + 2] : none;
+    v.w = at + 3 >= 0 && at + 3 < V ? row[at + 3] : none;
+    return v;
 }
 
 enum : int { VF_ACCEPT = 0, VF_REJECT = 1, VF_NEAR = 2, VF_BAD = 3 };
 
-// The sum over the cluster of a value of every warp's part, in the order of the parts; all[] holds them.
-// Calls take turns with the two sets of part: a CTA that writes one again has passed a barrier that all its
-// readers have reached behind their reads.
-__device__ __forceinline__ double vf_gather(VfShared &sh, double mine, int size, int warp, int lane, int &turn) {
+struct VfShared {
+    // this CTA's warps' parts of the rows: largest logit, its first place (greedy), sum of exponentials (NaN: a
+    // row with a NaN or +infinity)
+    float m[kVfWarps][kVfSlots], sum[kVfWarps][kVfSlots];
+    int at[kVfWarps][kVfSlots];
+    // of every row: the drafted token's logit and probability, the whole row's largest logit and its place, the decision
+    float draft_x[kVfRows], draft_q[kVfRows], row_m[kVfRows];
+    int draft[kVfRows], row_at[kVfRows], state[kVfRows];
+    double part[2][kVfWarps];            // the drawing: sums of this CTA's warps' parts (two calls of vf_gather)
+    double all[kVfCluster * kVfWarps];   // of all CTAs'
+    double step[kVfWarps];               // of the steps of the part that holds the token
+    unsigned long long tab[32];
+    int token, last;
+};
+
+// The row that a token is drawn from, or whose sum is formed in 64 bits.
+struct VfRow {
+    const float *x, *q;  // logits; probabilities to take away, or null
+    double m, inv, scale;
+    int V, shift, out;   // `out`: a token without weight, or -1
+};
+struct VfFour {
+    double w[4];
+};
+
+// This lane's four elements of a step: logits and, where they count, probabilities to take away.
+struct VfLoad {
+    float x[4], q[4];
+};
+__device__ __forceinline__ void vf_load(const VfRow &r, int i, VfLoad *l) {
+    const int at = 4 * (32 * i + (threadIdx.x & 31)) - r.shift;
+    const float4 v = vf_load4(r.x, r.V, at, -INFINITY);
+    l->x[0] = v.x, l->x[1] = v.y, l->x[2] = v.z, l->x[3] = v.w;
+    if (r.q) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
+        for (int b = 0; b < 4; ++b) l->q[b] = at + b >= 0 && at + b < r.V ? r.q[at + b] : 0.0f;
+    }
+}
+
+// Their weights: max(scale e^((x - m) / T) - q, 0).
+__device__ __noinline__ VfFour vf_weights(const VfRow r, const VfLoad l, int i, const unsigned long long *tab) {
+    const int at = 4 * (32 * i + (threadIdx.x & 31)) - r.shift;
+    VfFour f;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const double e = vf_exp(((double)l.x[b] - r.m) * r.inv, tab) * r.scale;
+        f.w[b] = at + b == r.out ? 0.0 : r.q ? fmax(e - (double)l.q[b], 0.0) : e;
+    }
+    return f;
+}
+
+// The sum of a row's weights over the cluster.  all[] holds the warps' sums.  Calls
+// take turns with the two sets of part: a CTA that writes one again has passed a barrier that all its readers
+// have reached behind their reads.
+__device__ __noinline__ double vf_gather(VfShared &sh, const VfRow r, int i0, int i1, int size, int turn) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double mine = 0.0;
+    VfLoad next;
+    vf_load(r, i0, &next);
+    for (int i = i0; i < i1; ++i) {
+        const VfLoad now = next;
+        vf_load(r, i + 1, &next);  // (behind the row: nothing is read)
+        const VfFour f = vf_weights(r, now, i, sh.tab);
+        mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
+    }
+    mine = warp_sum(mine);
     if (lane == 0) sh.part[turn][warp] = mine;
     cluster_barrier();
+    const int entries = size * kVfWarps / 32;  // lane l looks through parts entries * l ..: they lie 32 apart
     for (int i = threadIdx.x; i < size * kVfWarps; i += kVfThreads)
-        sh.all[i] = cluster_read(&sh.part[turn][i % kVfWarps], i / kVfWarps);
-    turn ^= 1;
+        sh.all[i % entries * 32 + i / entries] = cluster_read(&sh.part[turn][i % kVfWarps], i / kVfWarps);
     __syncthreads();
     double s = 0.0;
     for (int i = lane; i < size * kVfWarps; i += 32) s += sh.all[i];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    return s;
+    return warp_sum(s);
 }
 
 __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const VerifyParams p) {
     extern __shared__ __align__(16) unsigned char vf_smem[];
     VfShared &sh = *reinterpret_cast<VfShared *>(vf_smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.vocab;
-    uint32_t rank, size;
+    int rank, size;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-    const int s = blockIdx.x / size;
-    if (tid < 32) sh.tab[tid] = kExp2Tab32[tid];
+    const int s = blockIdx.x / size, warps = size * kVfWarps, me = rank * kVfWarps + warp;
     const int n = p.counts ? min(p.counts[s], p.max_drafts) : p.max_drafts;
     if (n < 0) return;  // an unused place (all CTAs of the cluster leave)
     const float T = p.temperatures[s];
     const bool greedy = !(T > 0.0f);
-    const int32_t *drafts = p.drafts + (size_t)s * p.max_drafts;
     const float *u = p.uniforms + (size_t)s * (p.max_drafts + 1);
     const float *logits = p.logits + (size_t)s * (p.max_drafts + 1) * V;
     const float c = fminf(1.44269504088896340736f / T, FLT_MAX);
     const double inv = 1.0 / (double)T;
-    __syncthreads();
+    const float last_u = u[p.max_drafts];
+    if (tid < 32) sh.tab[tid] = kExp2Tab32[tid];
+    for (int j = tid; j < n; j += kVfThreads) sh.draft[j] = p.drafts[(size_t)s * p.max_drafts + j];
 
-    // Every row's largest logit and sum (greedy: and the first place of it), this CTA's part.  A warp takes its
-    // part of one row behind the other, four loads a lane at a time and the next four under way.
-    {
-        const int step = size * kVfThreads, first = rank * kVfThreads + tid;
+    // the warps' runs of the rows' steps
+    const unsigned steps = (V + 3 + kVfStep - 1) / kVfStep;  // of a row, wherever it starts
+    const unsigned all_steps = (unsigned)(n + 1) * steps, run = (all_steps + warps - 1) / warps;  // (below 2^28)
+    const unsigned run1 = min(all_steps, (me + 1) * run);
+    const int first_row = (int)(me * run / steps);
+    for (unsigned st = me * run; st < run1;) {
+        const int j = (int)(st / steps);
+        const unsigned stop = min(run1, (unsigned)(j + 1) * steps);
+        const float *x = logits + (size_t)j * V;
+        int at = 4 * (32 * (int)(st - j * steps) + lane) - vf_shift(x);
+        float m = -FLT_MAX;
+        int place = 0x7FFFFFFF;
+        double sum = 0.0;
+        bool bad = false;
         float4 v[4];
-        auto load = [&](int j, int g) {
-            const float *x = logits + (size_t)j * V;
-            const int shift = vf_shift(x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = vf_load4(x, V, shift, g + i * step, -INFINITY);
-        };
-        load(0, first);
-        for (int j0 = 0; j0 <= n; j0 += kVfBlock) {
-            const int j1 = min(n + 1, j0 + kVfBlock);
-            for (int j = j0; j < j1; ++j) {
-                const int shift = vf_shift(logits + (size_t)j * V), groups = (V + shift + 3) / 4;
-                float m = -FLT_MAX;
-                int at = 0x7FFFFFFF;
-                double sum = 0.0;
-                bool bad = false;
-                for (int g = first; g - first < groups; g += 4 * step) {
-                    float4 w[4];
+        for (int i = 0; i < 4; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY)
+                                                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (; st < stop; st += 4, at += 4 * kVfStep) {
+            float4 w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = v[i];
-                    if (g - first + 4 * step < groups) load(j, g + 4 * step);
-                    else if (j < n) load(j + 1, first);
-                    float top = w[0].x;
+            for (int i = 0; i < 4; ++i) {
+                w[i] = v[i];  // the next four are under way meanwhile
+                v[i] = st + 4 + i < stop ? vf_load4(x, V, at + (4 + i) * kVfStep, -INFINITY)
+                                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            }
+            if (greedy) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(w[i].x, w[i].y), fmaxf(w[i].z, w[i].w)));
-                    if (greedy) {
+                for (int i = 0; i < 4; ++i) {
+                    const float e[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float e[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                bad |= e[k] != e[k];
-                                const int place = 4 * (g + i * step) - shift + k;
-                                if (e[k] > m || (e[k] == m && place < at)) m = e[k], at = place;
-                            }
-                        }
-                    } else {
-                        if (top > m) {
-                            sum *= (double)vf_ex2((m - top) * c);
-                            m = top;
-                        }
-                        float part = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            part += (vf_ex2((w[i].x - m) * c) + vf_ex2((w[i].y - m) * c)) +
-                                    (vf_ex2((w[i].z - m) * c) + vf_ex2((w[i].w - m) * c));
-                        sum += (double)part;
+                    for (int k = 0; k < 4; ++k) {
+                        bad |= e[k] != e[k];
+                        const int here = at + i * kVfStep + k;
+                        if (e[k] > m || (e[k] == m && here < place)) m = e[k], place = here;
                     }
                 }
-                float fsum = bad ? __int_as_float(0x7fc00000) : (float)sum;
-                vf_join<32>(m, at, fsum, greedy, c);
-                if (lane == 0) sh.wm[j - j0][warp] = m, sh.wat[j - j0][warp] = at, sh.wsum[j - j0][warp] = fsum;
+            } else {
+                float top = m;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(w[i].x, w[i].y), fmaxf(w[i].z, w[i].w)));
+                if (top > m) {
+                    sum *= (double)vf_ex2((m - top) * c);
+                    m = top;
+                }
+                float four = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    four += (vf_ex2((w[i].x - m) * c) + vf_ex2((w[i].y - m) * c)) +
+                            (vf_ex2((w[i].z - m) * c) + vf_ex2((w[i].w - m) * c));
+                sum += (double)four;
             }
-            __syncthreads();
-            const int r = tid / kVfWarps, w = tid % kVfWarps;
-            if (j0 + (warp * 32) / kVfWarps < j1) {  // (whole warps: two rows each)
-                float m = sh.wm[r][w], sum = sh.wsum[r][w];
-                int at = sh.wat[r][w];
-                vf_join<kVfWarps>(m, at, sum, greedy, c);
-                if (w == 0 && j0 + r < j1) sh.m[j0 + r] = m, sh.at[j0 + r] = at, sh.sum[j0 + r] = sum;
-            }
-            __syncthreads();
+        }
+        st = stop;
+        float top = m, part = bad ? __int_as_float(0x7fc00000) : (float)sum;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        if (!greedy) part *= vf_ex2((m - top) * c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
+        if (greedy) place = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)place : 0x7FFFFFFFu);
+        if (lane == 0) {
+            sh.m[warp][j - first_row] = top;
+            sh.sum[warp][j - first_row] = part;
+            sh.at[warp][j - first_row] = place;
         }
     }
     cluster_barrier();
 
-    // the whole rows, and what becomes of every draft (each CTA forms the same)
-    int state[kVfRows / kVfThreads];
-#pragma unroll
-    for (int i = 0; i < kVfRows / kVfThreads; ++i) {
-        const int j = tid + i * kVfThreads;
-        state[i] = VF_ACCEPT;
-        if (j > n) continue;
+    // the whole rows, and what becomes of every draft: a warp a row, a lane a part of it
+    for (int j = warp; j <= n; j += kVfWarps) {
+        const int w0 = (int)(j * steps / run), w1 = (int)(((j + 1) * steps - 1) / run);
+        const int d = j < n ? sh.draft[j] : -1;
+        float draft_x = -INFINITY, draft_q = 1.0f, draft_u = 0.0f;
+        if (lane == 0 && d >= 0 && d < V) {
+            draft_x = logits[(size_t)j * V + d];
+            draft_u = u[j];
+            if (p.probs) draft_q = p.probs[((size_t)s * p.max_drafts + j) * V + d];
+        }
         float m = -FLT_MAX, sum = 0.0f;
         int at = 0x7FFFFFFF;
-        for (int w = 0; w < (int)size; ++w) m = fmaxf(m, cluster_read(&sh.m[j], w));
-        for (int w = 0; w < (int)size; ++w) {
-            const float m2 = cluster_read(&sh.m[j], w), sum2 = cluster_read(&sh.sum[j], w);
-            sum += greedy ? sum2 : sum2 * vf_ex2((m2 - m) * c);
-            if (greedy && m2 == m) at = min(at, cluster_read(&sh.at[j], w));
+        for (int w = w0 + lane; w - lane <= w1; w += 32) {
+            float m2 = -FLT_MAX, sum2 = 0.0f;
+            int at2 = 0x7FFFFFFF;
+            if (w <= w1) {
+                const int slot = j - (int)(w * run / steps), from = w / kVfWarps;
+                m2 = cluster_read(&sh.m[w % kVfWarps][slot], from);
+                sum2 = cluster_read(&sh.sum[w % kVfWarps][slot], from);
+                at2 = cluster_read(&sh.at[w % kVfWarps][slot], from);
+            }
+            const float top = fmaxf(m, m2);
+            sum = greedy ? sum + sum2 : sum * vf_ex2((m - top) * c) + sum2 * vf_ex2((m2 - top) * c);
+            if (m2 > m || (m2 == m && at2 < at)) at = at2;
+            m = top;
         }
-        sh.row_m[j] = m;
-        sh.row_at[j] = at;
-        const int d = j < n ? drafts[j] : -1;
-        if (sum != sum || !(m < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0f)) {
-            state[i] = VF_BAD;
-        } else if (j == n) {
-            state[i] = VF_REJECT;  // the row behind the last draft
-        } else if (greedy) {
-            state[i] = d == at ? VF_ACCEPT : VF_REJECT;
-        } else if (d < 0 || d >= V) {
-            state[i] = VF_REJECT;
-        } else {
-            const double e = vf_exp(((double)logits[(size_t)j * V + d] - (double)m) * inv, sh.tab);
-            const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + j) * V + d] : 1.0;
-            const double limit = (double)u[j] * q * (double)sum;
-            state[i] = fabs(limit - e) <= 0x1p-12 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
-        }
-    }
-
-    // the first row that is not an accepted draft
-    int k = -1, st = VF_ACCEPT, turn = 0;
-    const int per = (int)(((size_t)V + 3 + size * kVfWarps * 128 - 1) / (size * kVfWarps * 128));  // 128 elements a step
-    const int steps0 = (int)(rank * kVfWarps + warp) * per;  // this warp's part of a row: steps [steps0, steps0 + per)
-    while (true) {
-        __syncthreads();
-        if (tid == 0) sh.first = 0x7FFFFFFF;
-        __syncthreads();
+        float top = m;
 #pragma unroll
-        for (int i = 0; i < kVfRows / kVfThreads; ++i) {
-            const int j = tid + i * kVfThreads;
-            if (j <= n && j > k && state[i] != VF_ACCEPT) atomicMin(&sh.first, j * 4 + state[i]);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        if (!greedy) sum *= vf_ex2((m - top) * c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        at = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)at : 0x7FFFFFFFu);
+        if (lane) continue;
+        sh.row_m[j] = top;
+        sh.row_at[j] = at;
+        int state = VF_REJECT;  // (the row behind the last draft, a draft that is no token)
+        if (sum != sum || !(top < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0f)) {
+            state = VF_BAD;
+        } else if (greedy) {
+            if (j < n && d == at) state = VF_ACCEPT;
+        } else if (d >= 0 && d < V) {
+            const double e = vf_exp(((double)draft_x - (double)top) * inv, sh.tab);
+            const double limit = (double)draft_u * (double)draft_q * (double)sum;
+            sh.draft_x[j] = draft_x;
+            sh.draft_q[j] = draft_q;
+            state = fabs(limit - e) <= 0x1p-12 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
         }
-        __syncthreads();
-        k = sh.first >> 2;
-        st = sh.first & 3;
+        sh.state[j] = state;
+    }
+    __syncthreads();
+
+    // the first row that is not an accepted draft (every warp of the cluster finds the same)
+    const int per = ((int)steps + warps - 1) / warps, i0 = min((int)steps, me * per), i1 = min((int)steps, i0 + per);
+    int k = -1, st, turn = 0;
+    VfRow row;
+    row.inv = inv;
+    row.V = V;
+    while (true) {
+        for (int j = k + 1;; j += 32) {
+            const unsigned stop = __ballot_sync(0xFFFFFFFFu, j + lane <= n && sh.state[min(j + lane, n)] != VF_ACCEPT);
+            if (stop) {
+                k = j + __ffs(stop) - 1;
+                break;
+            }
+        }
+        st = sh.state[k];
+        row.x = logits + (size_t)k * V;
+        row.q = nullptr;
+        row.m = (double)sh.row_m[k];
+        row.scale = 1.0;
+        row.shift = vf_shift(row.x);
+        row.out = -1;
         if (st != VF_NEAR) break;
         // too near to tell: the row's sum in 64 bits
-        const float *x = logits + (size_t)k * V;
-        const double m = (double)sh.row_m[k];
-        const int shift = vf_shift(x);
-        double sum = 0.0;
-        for (int i = steps0; i < steps0 + per; ++i) {
-            const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
-            sum += (vf_exp(((double)v.x - m) * inv, sh.tab) + vf_exp(((double)v.y - m) * inv, sh.tab)) +
-                   (vf_exp(((double)v.z - m) * inv, sh.tab) + vf_exp(((double)v.w - m) * inv, sh.tab));
-        }
-        const double total = vf_gather(sh, sum, size, warp, lane, turn);
-        const int d = drafts[k];
-        const double q = p.probs ? (double)p.probs[((size_t)s * p.max_drafts + k) * V + d] : 1.0;
-        if (!((double)u[k] * q * total < vf_exp(((double)x[d] - m) * inv, sh.tab))) {
+        const double total = vf_gather(sh, row, i0, i1, size, turn);
+        turn ^= 1;
+        if (!((double)u[k] * (double)sh.draft_q[k] * total < vf_exp(((double)sh.draft_x[k] - row.m) * inv, sh.tab))) {
             st = VF_REJECT;
             break;
         }
@@ -318,47 +367,18 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
     if (st == VF_REJECT && greedy) {
         token = sh.row_at[k];
     } else if (st == VF_REJECT) {
-        const float *x = logits + (size_t)k * V;
-        const float *q = p.probs && k < n ? p.probs + ((size_t)s * p.max_drafts + k) * V : nullptr;
-        const int out = !q && k < n ? drafts[k] : -1;  // a certain draft has no weight left
-        const double m = (double)sh.row_m[k];
-        const int shift = vf_shift(x);
-        auto weight4 = [&](int i, double scale, double (&w)[4]) {
-            const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
-            w[0] = vf_exp(((double)v.x - m) * inv, sh.tab) * scale;
-            w[1] = vf_exp(((double)v.y - m) * inv, sh.tab) * scale;
-            w[2] = vf_exp(((double)v.z - m) * inv, sh.tab) * scale;
-            w[3] = vf_exp(((double)v.w - m) * inv, sh.tab) * scale;
-            const int at = 4 * (i * 32 + lane) - shift;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                if (q && at + b >= 0 && at + b < V) w[b] = fmax(w[b] - (double)q[at + b], 0.0);
-                if (at + b == out) w[b] = 0.0;
-            }
-        };
-        double scale = 1.0, w[4];
-        if (q) {  // p and q are compared: p needs its sum
-            double sum = 0.0;
-            const float *q0 = q;
-            q = nullptr;
-            for (int i = steps0; i < steps0 + per; ++i) {
-                weight4(i, 1.0, w);
-                sum += (w[0] + w[1]) + (w[2] + w[3]);
-            }
-            q = q0;
-            scale = 1.0 / vf_gather(sh, sum, size, warp, lane, turn);
+        if (k < n && p.probs) {  // p and q are compared: p needs its sum
+            row.scale = 1.0 / vf_gather(sh, row, i0, i1, size, turn);
+            turn ^= 1;
+            row.q = p.probs + ((size_t)s * p.max_drafts + k) * V;
+        } else if (k < n) {
+            row.out = sh.draft[k];  // a certain draft has no weight left
         }
-        double sum = 0.0;
-        for (int i = steps0; i < steps0 + per; ++i) {
-            weight4(i, scale, w);
-            sum += (w[0] + w[1]) + (w[2] + w[3]);
-        }
-        const double rest = vf_gather(sh, sum, size, warp, lane, turn);
-        const double target = (double)u[p.max_drafts] * rest;
-        // the part that holds the token, and what lies before it (every warp finds the same)
-        const int entries = (int)size * kVfWarps / 32;  // of a lane, one behind the other
+        const double target = (double)last_u * vf_gather(sh, row, i0, i1, size, turn);
+        // the part that holds the token, and what lies before it
+        const int entries = warps / 32;  // of a lane, one behind the other
         double own = 0.0, base = 0.0;
-        for (int i = 0; i < entries; ++i) own += sh.all[lane * entries + i];
+        for (int i = 0; i < entries; ++i) own += sh.all[i * 32 + lane];
         double before = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -368,7 +388,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         before -= own;
         int part = 0x7FFFFFFF, last = -1;
         for (int i = 0; i < entries; ++i) {
-            const double y = sh.all[lane * entries + i];
+            const double y = sh.all[i * 32 + lane];
             if (y > 0.0) {
                 last = lane * entries + i;
                 if (part == 0x7FFFFFFF && before + y > target) part = last, base = before;
@@ -376,65 +396,75 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             before += y;
         }
         const int mine = part;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            part = min(part, __shfl_xor_sync(0xFFFFFFFFu, part, o));
-            last = max(last, __shfl_xor_sync(0xFFFFFFFFu, last, o));
-        }
-        const unsigned holder = __ballot_sync(0xFFFFFFFFu, mine == part);
-        base = __shfl_sync(0xFFFFFFFFu, base, __ffs(holder) - 1);
-        if (part == 0x7FFFFFFF) part = -1;
-        const bool over = part >= 0;
+        part = (int)__reduce_min_sync(0xFFFFFFFFu, (unsigned)part);
+        last = __reduce_max_sync(0xFFFFFFFFu, last);
+        base = __shfl_sync(0xFFFFFFFFu, base, __ffs(__ballot_sync(0xFFFFFFFFu, mine == part)) - 1);
+        const bool over = part != 0x7FFFFFFF;
         if (!over) part = last;  // (u of 1 or more): the last token of any weight
-        if (part == (int)rank * kVfWarps + warp) {
+        token = -2;              // written by the part's CTA
+        if (part >= 0 && part / kVfWarps == rank) {
+            // this CTA has the part: its warps take its steps side by side
+            const int p0 = min((int)steps, part * per), p1 = min((int)steps, p0 + per);
             int found = -1, some = -1;
-            double run = base;
-            for (int i = steps0; i < steps0 + per && found < 0; ++i) {
-                weight4(i, scale, w);
-                const double four = (w[0] + w[1]) + (w[2] + w[3]);
+            for (int i = p0; i < p1 && found < 0; i += kVfWarps) {
+                VfLoad l;
+                vf_load(row, min(i + warp, p1), &l);
+                VfFour f = vf_weights(row, l, i + warp, sh.tab);
+                if (i + warp >= p1) f.w[0] = f.w[1] = f.w[2] = f.w[3] = 0.0;
+                const double four = (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
                 double incl = four;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
                     if (lane >= o) incl += y;
                 }
-                double cum = run + (incl - four);
-                int hit = 0x7FFFFFFF, any = -1;
+                __syncthreads();
+                if (lane == 31) sh.step[warp] = incl;
+                if (tid == 0) sh.token = 0x7FFFFFFF, sh.last = -1;
+                __syncthreads();
+                double cum = base;
+#pragma unroll
+                for (int w = 0; w < kVfWarps; ++w) {
+                    if (w < warp) cum += sh.step[w];
+                    base += sh.step[w];
+                }
+                cum += incl - four;
+                unsigned hit = 0x7FFFFFFFu;
+                int any = -1;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    cum += w[b];
-                    const int at = 4 * (i * 32 + lane) - shift + b;
-                    if (w[b] > 0.0) {
+                    cum += f.w[b];
+                    const int at = 4 * (32 * (i + warp) + lane) - row.shift + b;
+                    if (f.w[b] > 0.0) {
                         any = at;
-                        if (over && cum > target) hit = min(hit, at);
+                        if (over && cum > target) hit = min(hit, (unsigned)at);
                     }
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    hit = min(hit, __shfl_xor_sync(0xFFFFFFFFu, hit, o));
-                    any = max(any, __shfl_xor_sync(0xFFFFFFFFu, any, o));
+                hit = __reduce_min_sync(0xFFFFFFFFu, hit);
+                any = __reduce_max_sync(0xFFFFFFFFu, any);
+                if (lane == 0) {
+                    atomicMin(&sh.token, (int)hit);
+                    atomicMax(&sh.last, any);
                 }
-                some = max(some, any);
-                if (hit != 0x7FFFFFFF) found = hit;
-                run += __shfl_sync(0xFFFFFFFFu, incl, 31);
+                __syncthreads();
+                if (sh.token != 0x7FFFFFFF) found = sh.token;
+                some = max(some, sh.last);
             }
-            if (lane == 0) p.token[s] = found >= 0 ? found : some;
-        }
-        token = -2;  // written by the part's warp
-        if (part < 0) {
+            if (tid == 0) p.token[s] = found >= 0 ? found : some;
+        } else if (part < 0) {
             // nothing has weight: the row's first maximum
             if (tid == 0) sh.token = 0x7FFFFFFF;
             __syncthreads();
-            for (int i = steps0; i < steps0 + per; ++i) {
-                const float4 v = vf_load4(x, V, shift, i * 32 + lane, -INFINITY);
-                const int at = 4 * (i * 32 + lane) - shift;
-                const float mm = sh.row_m[k];
-                const int hit = v.x == mm ? at : v.y == mm ? at + 1 : v.z == mm ? at + 2 : v.w == mm ? at + 3 : 0x7FFFFFFF;
+            for (int i = i0; i < i1; ++i) {
+                const int at = 4 * (32 * i + lane) - row.shift;
+                const float4 v = vf_load4(row.x, V, at, -INFINITY);
+                const float top = sh.row_m[k];
+                const int hit = v.x == top ? at : v.y == top ? at + 1 : v.z == top ? at + 2 : v.w == top ? at + 3 : 0x7FFFFFFF;
                 if (hit != 0x7FFFFFFF) atomicMin(&sh.token, hit);
             }
             cluster_barrier();
             token = 0x7FFFFFFF;
-            for (int w2 = 0; w2 < (int)size; ++w2) token = min(token, cluster_read(&sh.token, w2));
+            for (int w = 0; w < size; ++w) token = min(token, cluster_read(&sh.token, w));
         }
     }
     if (rank == 0 && tid == 0) {
@@ -455,7 +485,7 @@ ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t s
         if (e != cudaSuccess) return cuda_status(e, "verify_drafts");
         once.mark(dev);
     }
-    const int cluster = n_seq * kVfCluster <= sm_count(dev) ? kVfCluster : 8;
+    const int cluster = n_seq * kVfCluster <= sm_count(dev) ? kVfCluster : kVfMinCluster;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_seq * cluster);
     cfg.blockDim = dim3(kVfThreads);
