@@ -11,21 +11,18 @@
 // one.  T <= 0 is greedy: a draft is accepted iff it is its row's first
 // maximum, which is also the next token.
 //
-// A decision must not depend on rounding: a vocabulary has 10^5 borders, and one
-// that falls the other way changes a token.  The rows' sums are first formed from
-// fp32 exponentials.  A lane rescales its sum when it meets a larger logit, at
-// most once per 16 elements, 256 times in the longest row (2^24 over 8 x 512
-// lanes), each time off by 2^-21.4 at most, so a sum is off by less than 2^-12;
-// where a draft's decision is nearer to its border than that, its row is summed
-// again in 64 bits.  The row that a token is drawn from is summed in 64 bits always.
+// All exponentials and sums are formed in 64 bits: a decision must not depend on
+// rounding, a vocabulary has 10^5 borders, and one that falls the other way changes
+// a token.  The device does 64 such products a clock and SM, so an exponential of
+// ten of them (a table and a short series) keeps pace with memory.
 //
 // A cluster of 8 or 16 CTAs takes a sequence.  Its warps cut all rows, one behind
 // the other, into equal runs of steps (128 elements), so that a warp meets one or
 // two rows and reduces as often; the partial sums meet in distributed shared
-// memory, and every CTA forms the same decisions.  For a batch the logits' bytes
-// bound it; for one sequence latency does: three cluster barriers, and code that
-// runs once and comes from memory, which is why its parts are functions, not
-// inlined copies.
+// memory, and every CTA forms the same decisions.  Where the drawn row's weights
+// are its exponentials, the partial sums serve the drawing too; where a draft's
+// distribution is taken away, the row is passed once more.  For a batch the
+// logits' bytes and the exponentials bound it alike; for one sequence latency does.
 #include <float.h>
 
 #include "ovf_internal.cuh"
@@ -47,31 +44,36 @@ static constexpr int kVfStep = 128;         // elements that a warp takes at onc
 // rows that a warp's run meets: the run is ceil(rows * steps / warps) steps of `steps` a row
 static constexpr int kVfSlots = kVfRows / (kVfMinCluster * kVfWarps) + 2;
 
-// What lies below the normal numbers, and NaN.
-__device__ __noinline__ double vf_exp_tail(double x) { return exp(x); }
-
-// e^x in 64 bits, off by about 2^-48: x = n ln 2 / 32 + r, the series of e^r (|r| < 0.011), and 2^(n / 32) from the
-// table of 2^(i / 32) that exp_libm (ovf_common.cuh) has.  ln 2 is taken in two parts, the first of 24 bits, so
-// that its product with n is exact.
+// e^x in 64 bits for x of -700 to 700, off by less than 2^-44: x = n ln 2 / 64 + r, the series of e^r to r^4
+// (|r| < 0.0055), and 2^(n / 64) from `tab`: entry i holds the bits of 2^(i / 64) less i << 46.  NaN stays NaN.
+// A branch for other x would double its time (3.8 clocks a warp and SM): its callers raise smaller logits to
+// a floor of weight e^-690 instead, in 32 bits.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
-    if (!(x > -700.0)) return x < -746.0 ? 0.0 : vf_exp_tail(x);
     const double shift = 0x1.8p52;  // its sum with a number ends in that number's nearest integer
-    const double kd = fma(x, 32.0 / 0.693147180559945309417, shift), n = kd - shift;
-    double r = fma(n, -0x1.62e4300000000p-1 / 32.0, x);
-    r = fma(n, 0x1.05c610ca86c39p-29 / 32.0, r);
-    double y = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    y = fma(y, r, 1.0 / 6.0);
+    const double kd = fma(x, 64.0 / 0.693147180559945309417, shift), n = kd - shift;
+    const double r = fma(n, -0.693147180559945309417 / 64.0, x);  // (n < 2^17: off by less than 2^-46)
+    double y = fma(r, 1.0 / 24.0, 1.0 / 6.0);
     y = fma(y, r, 0.5);
     y = fma(y, r, 1.0);
     y = fma(y, r, 1.0);
     const int k = __double2loint(kd);
-    return y * __longlong_as_double((long long)(tab[k & 31] + ((unsigned long long)(long long)k << 47)));
+    return y * __longlong_as_double((long long)(tab[k & 63] + ((unsigned long long)(long long)k << 46)));
 }
-
-__device__ __forceinline__ float vf_ex2(float x) {
+// The same for any x up to 0 (0 below e^-690).
+__device__ __forceinline__ double vf_exp0(double x, const unsigned long long *tab) {
+    return x < -690.0 ? 0.0 : vf_exp(x, tab);
+}
+__device__ __forceinline__ float vf_floor(float m, float T) { return fmaxf(m - 690.0f * T, -FLT_MAX); }
+__device__ __forceinline__ float vf_raise(float x, float floor) {  // the larger; NaN stays NaN
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(floor));
     return y;
+}
+// The table from that of 2^(i / 32) which exp_libm (ovf_common.cuh) has.
+__device__ __forceinline__ unsigned long long vf_tab(int i) {
+    const unsigned long long half = kExp2Tab32[i >> 1] + ((unsigned long long)(i >> 1) << 47);  // bits of 2^((i >> 1) / 32)
+    const double v = __longlong_as_double((long long)half) * (i & 1 ? 0x1.02c9a3e778061p+0 : 1.0);  // 2^(1 / 64)
+    return (unsigned long long)__double_as_longlong(v) - ((unsigned long long)i << 46);
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -112,27 +114,30 @@ __device__ __forceinline__ float4 vf_load4(const float *row, int V, int at, floa
     return v;
 }
 
-enum : int { VF_ACCEPT = 0, VF_REJECT = 1, VF_NEAR = 2, VF_BAD = 3 };
+enum : int { VF_ACCEPT = 0, VF_REJECT = 1, VF_BAD = 2 };
 
 struct VfShared {
     // this CTA's warps' parts of the rows: largest logit, its first place (greedy), sum of exponentials (NaN: a
     // row with a NaN or +infinity)
-    float m[kVfWarps][kVfSlots], sum[kVfWarps][kVfSlots];
+    double sum[kVfWarps][kVfSlots];
+    float m[kVfWarps][kVfSlots];
     int at[kVfWarps][kVfSlots];
-    // of every row: the drafted token's logit and probability, the whole row's largest logit and its place, the decision
-    float draft_x[kVfRows], draft_q[kVfRows], row_m[kVfRows];
+    // of every row: the drafted token, the whole row's sum, largest logit and its place, the decision
+    double row_sum[kVfRows];
+    float row_m[kVfRows];
     int draft[kVfRows], row_at[kVfRows], state[kVfRows];
-    double part[2][kVfWarps];            // the drawing: sums of this CTA's warps' parts (two calls of vf_gather)
-    double all[kVfCluster * kVfWarps];   // of all CTAs'
+    double part[kVfWarps];               // the drawing: sums of this CTA's warps' parts
+    double all[kVfCluster * kVfWarps];   // of all parts
     double step[kVfWarps];               // of the steps of the part that holds the token
-    unsigned long long tab[32];
+    unsigned long long tab[64];
     int token, last;
 };
 
-// The row that a token is drawn from, or whose sum is formed in 64 bits.
+// The row that a token is drawn from.
 struct VfRow {
     const float *x, *q;  // logits; probabilities to take away, or null
     double m, inv, scale;
+    float floor;         // logits up to here have no weight
     int V, shift, out;   // `out`: a token without weight, or -1
 };
 struct VfFour {
@@ -154,41 +159,15 @@ __device__ __forceinline__ void vf_load(const VfRow &r, int i, VfLoad *l) {
 }
 
 // Their weights: max(scale e^((x - m) / T) - q, 0).
-__device__ __noinline__ VfFour vf_weights(const VfRow r, const VfLoad l, int i, const unsigned long long *tab) {
+__device__ __forceinline__ VfFour vf_weights(const VfRow &r, const VfLoad &l, int i, const unsigned long long *tab) {
     const int at = 4 * (32 * i + (threadIdx.x & 31)) - r.shift;
     VfFour f;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-        const double e = vf_exp(((double)l.x[b] - r.m) * r.inv, tab) * r.scale;
-        f.w[b] = at + b == r.out ? 0.0 : r.q ? fmax(e - (double)l.q[b], 0.0) : e;
+        const double e = vf_exp(((double)fmaxf(l.x[b], r.floor) - r.m) * r.inv, tab) * r.scale;
+        f.w[b] = at + b == r.out || !(l.x[b] > r.floor) ? 0.0 : r.q ? fmax(e - (double)l.q[b], 0.0) : e;
     }
     return f;
-}
-
-// The sum of a row's weights over the cluster.  all[] holds the warps' sums.  Calls
-// take turns with the two sets of part: a CTA that writes one again has passed a barrier that all its readers
-// have reached behind their reads.
-__device__ __noinline__ double vf_gather(VfShared &sh, const VfRow r, int i0, int i1, int size, int turn) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    double mine = 0.0;
-    VfLoad next;
-    vf_load(r, i0, &next);
-    for (int i = i0; i < i1; ++i) {
-        const VfLoad now = next;
-        vf_load(r, i + 1, &next);  // (behind the row: nothing is read)
-        const VfFour f = vf_weights(r, now, i, sh.tab);
-        mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
-    }
-    mine = warp_sum(mine);
-    if (lane == 0) sh.part[turn][warp] = mine;
-    cluster_barrier();
-    const int entries = size * kVfWarps / 32;  // lane l looks through parts entries * l ..: they lie 32 apart
-    for (int i = threadIdx.x; i < size * kVfWarps; i += kVfThreads)
-        sh.all[i % entries * 32 + i / entries] = cluster_read(&sh.part[turn][i % kVfWarps], i / kVfWarps);
-    __syncthreads();
-    double s = 0.0;
-    for (int i = lane; i < size * kVfWarps; i += 32) s += sh.all[i];
-    return warp_sum(s);
 }
 
 __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const VerifyParams p) {
@@ -205,11 +184,12 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
     const bool greedy = !(T > 0.0f);
     const float *u = p.uniforms + (size_t)s * (p.max_drafts + 1);
     const float *logits = p.logits + (size_t)s * (p.max_drafts + 1) * V;
-    const float c = fminf(1.44269504088896340736f / T, FLT_MAX);
     const double inv = 1.0 / (double)T;
     const float last_u = u[p.max_drafts];
-    if (tid < 32) sh.tab[tid] = kExp2Tab32[tid];
+    if (tid < 64) sh.tab[tid] = vf_tab(tid);
     for (int j = tid; j < n; j += kVfThreads) sh.draft[j] = p.drafts[(size_t)s * p.max_drafts + j];
+
+    __syncthreads();
 
     // the warps' runs of the rows' steps
     const unsigned steps = (V + 3 + kVfStep - 1) / kVfStep;  // of a row, wherever it starts
@@ -225,56 +205,57 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         int place = 0x7FFFFFFF;
         double sum = 0.0;
         bool bad = false;
-        float4 v[4];
+        const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        float4 v[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY)
-                                                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        for (; st < stop; st += 4, at += 4 * kVfStep) {
-            float4 w[4];
+        for (int i = 0; i < 2; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY) : none;
+        for (; st < stop; st += 2, at += 2 * kVfStep) {
+            float4 w[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = v[i];  // the next four are under way meanwhile
-                v[i] = st + 4 + i < stop ? vf_load4(x, V, at + (4 + i) * kVfStep, -INFINITY)
-                                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            for (int i = 0; i < 2; ++i) {
+                w[i] = v[i];  // the next two are under way meanwhile
+                v[i] = st + 2 + i < stop ? vf_load4(x, V, at + (2 + i) * kVfStep, -INFINITY) : none;
             }
+            const float e[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
             if (greedy) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float e[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        bad |= e[k] != e[k];
-                        const int here = at + i * kVfStep + k;
-                        if (e[k] > m || (e[k] == m && here < place)) m = e[k], place = here;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    bad |= e[i] != e[i];
+                    const int here = at + (i >> 2) * kVfStep + (i & 3);
+                    if (e[i] > m || (e[i] == m && here < place)) m = e[i], place = here;
                 }
             } else {
                 float top = m;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fmaxf(w[i].x, w[i].y), fmaxf(w[i].z, w[i].w)));
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, e[i]);
                 if (top > m) {
-                    sum *= (double)vf_ex2((m - top) * c);
+                    sum *= vf_exp0(((double)m - (double)top) * inv, sh.tab);
                     m = top;
                 }
-                float four = 0.0f;
+                const double md = (double)m;
+                const float floor = vf_floor(m, T);
+                double part[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    four += (vf_ex2((w[i].x - m) * c) + vf_ex2((w[i].y - m) * c)) +
-                            (vf_ex2((w[i].z - m) * c) + vf_ex2((w[i].w - m) * c));
-                sum += (double)four;
+                for (int i = 0; i < 8; ++i) {
+                    const double y = vf_exp(((double)vf_raise(e[i], floor) - md) * inv, sh.tab);
+                    part[i & 3] = i < 4 ? y : part[i & 3] + y;
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
             }
         }
         st = stop;
-        float top = m, part = bad ? __int_as_float(0x7fc00000) : (float)sum;
+        float top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        if (!greedy) part *= vf_ex2((m - top) * c);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xFFFFFFFFu, part, o);
-        if (greedy) place = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)place : 0x7FFFFFFFu);
+        if (greedy) {
+            place = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)place : 0x7FFFFFFFu);
+            if (__any_sync(0xFFFFFFFFu, bad)) sum = __longlong_as_double(0x7ff8000000000000ll);
+        } else {
+            sum = warp_sum(sum * vf_exp0(((double)m - (double)top) * inv, sh.tab));
+        }
         if (lane == 0) {
             sh.m[warp][j - first_row] = top;
-            sh.sum[warp][j - first_row] = part;
+            sh.sum[warp][j - first_row] = sum;
             sh.at[warp][j - first_row] = place;
         }
     }
@@ -290,93 +271,123 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             draft_u = u[j];
             if (p.probs) draft_q = p.probs[((size_t)s * p.max_drafts + j) * V + d];
         }
-        float m = -FLT_MAX, sum = 0.0f;
+        float m = -FLT_MAX;
+        double sum = 0.0;
         int at = 0x7FFFFFFF;
-        for (int w = w0 + lane; w - lane <= w1; w += 32) {
-            float m2 = -FLT_MAX, sum2 = 0.0f;
-            int at2 = 0x7FFFFFFF;
-            if (w <= w1) {
-                const int slot = j - (int)(w * run / steps), from = w / kVfWarps;
-                m2 = cluster_read(&sh.m[w % kVfWarps][slot], from);
-                sum2 = cluster_read(&sh.sum[w % kVfWarps][slot], from);
-                at2 = cluster_read(&sh.at[w % kVfWarps][slot], from);
-            }
+        for (int w = w0 + lane; w <= w1; w += 32) {
+            const int slot = j - (int)(w * run / steps), from = w / kVfWarps;
+            const float m2 = cluster_read(&sh.m[w % kVfWarps][slot], from);
+            const double sum2 = cluster_read(&sh.sum[w % kVfWarps][slot], from);
+            const int at2 = cluster_read(&sh.at[w % kVfWarps][slot], from);
             const float top = fmaxf(m, m2);
-            sum = greedy ? sum + sum2 : sum * vf_ex2((m - top) * c) + sum2 * vf_ex2((m2 - top) * c);
+            sum = greedy ? sum + sum2
+                         : sum * vf_exp0(((double)m - (double)top) * inv, sh.tab) +
+                               sum2 * vf_exp0(((double)m2 - (double)top) * inv, sh.tab);
             if (m2 > m || (m2 == m && at2 < at)) at = at2;
             m = top;
         }
         float top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        if (!greedy) sum *= vf_ex2((m - top) * c);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (!greedy) sum *= vf_exp0(((double)m - (double)top) * inv, sh.tab);
+        sum = warp_sum(sum);
         at = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)at : 0x7FFFFFFFu);
         if (lane) continue;
-        sh.row_m[j] = top;
-        sh.row_at[j] = at;
         int state = VF_REJECT;  // (the row behind the last draft, a draft that is no token)
-        if (sum != sum || !(top < INFINITY) || (greedy ? at == 0x7FFFFFFF : sum == 0.0f)) {
+        if (sum != sum || !(top < INFINITY) || top == -FLT_MAX) {
             state = VF_BAD;
         } else if (greedy) {
             if (j < n && d == at) state = VF_ACCEPT;
         } else if (d >= 0 && d < V) {
-            const double e = vf_exp(((double)draft_x - (double)top) * inv, sh.tab);
-            const double limit = (double)draft_u * (double)draft_q * (double)sum;
-            sh.draft_x[j] = draft_x;
-            sh.draft_q[j] = draft_q;
-            state = fabs(limit - e) <= 0x1p-12 * fmax(limit, e) ? VF_NEAR : limit < e ? VF_ACCEPT : VF_REJECT;
+            const double e = vf_exp0(((double)draft_x - (double)top) * inv, sh.tab);
+            if ((double)draft_u * (double)draft_q * sum < e) state = VF_ACCEPT;
         }
+        sh.row_sum[j] = sum;
+        sh.row_m[j] = top;
+        sh.row_at[j] = at;
         sh.state[j] = state;
     }
     __syncthreads();
 
     // the first row that is not an accepted draft (every warp of the cluster finds the same)
-    const int per = ((int)steps + warps - 1) / warps, i0 = min((int)steps, me * per), i1 = min((int)steps, i0 + per);
-    int k = -1, st, turn = 0;
-    VfRow row;
-    row.inv = inv;
-    row.V = V;
-    while (true) {
-        for (int j = k + 1;; j += 32) {
-            const unsigned stop = __ballot_sync(0xFFFFFFFFu, j + lane <= n && sh.state[min(j + lane, n)] != VF_ACCEPT);
-            if (stop) {
-                k = j + __ffs(stop) - 1;
-                break;
-            }
-        }
-        st = sh.state[k];
-        row.x = logits + (size_t)k * V;
-        row.q = nullptr;
-        row.m = (double)sh.row_m[k];
-        row.scale = 1.0;
-        row.shift = vf_shift(row.x);
-        row.out = -1;
-        if (st != VF_NEAR) break;
-        // too near to tell: the row's sum in 64 bits
-        const double total = vf_gather(sh, row, i0, i1, size, turn);
-        turn ^= 1;
-        if (!((double)u[k] * (double)sh.draft_q[k] * total < vf_exp(((double)sh.draft_x[k] - row.m) * inv, sh.tab))) {
-            st = VF_REJECT;
+    int k = 0;
+    for (int j = 0;; j += 32) {
+        const unsigned stop = __ballot_sync(0xFFFFFFFFu, j + lane <= n && sh.state[min(j + lane, n)] != VF_ACCEPT);
+        if (stop) {
+            k = j + __ffs(stop) - 1;
             break;
         }
     }
-
     int token = -1;
-    if (st == VF_REJECT && greedy) {
+    if (sh.state[k] == VF_REJECT && greedy) {
         token = sh.row_at[k];
-    } else if (st == VF_REJECT) {
-        if (k < n && p.probs) {  // p and q are compared: p needs its sum
-            row.scale = 1.0 / vf_gather(sh, row, i0, i1, size, turn);
-            turn ^= 1;
-            row.q = p.probs + ((size_t)s * p.max_drafts + k) * V;
-        } else if (k < n) {
-            row.out = sh.draft[k];  // a certain draft has no weight left
+    } else if (sh.state[k] == VF_REJECT) {
+        VfRow row;
+        row.x = logits + (size_t)k * V;
+        row.q = nullptr;
+        row.m = (double)sh.row_m[k];
+        row.inv = inv;
+        row.scale = 1.0;
+        row.floor = vf_floor(sh.row_m[k], T);
+        row.V = V;
+        row.shift = vf_shift(row.x);
+        row.out = -1;
+        double drafted = 0.0;  // the weight of a certain draft, which is taken away
+        if (k < n && !p.probs && sh.draft[k] >= 0 && sh.draft[k] < V) {
+            row.out = sh.draft[k];
+            drafted = vf_exp0(((double)row.x[row.out] - row.m) * inv, sh.tab);
         }
-        const double target = (double)last_u * vf_gather(sh, row, i0, i1, size, turn);
+        // The row's parts and their weights.  Without a distribution to take away they are the runs above and their
+        // sums (less a draft's, unless little were left: a difference of nearly equal sums would be inexact); else
+        // the row is passed once more.
+        int parts, part0, per = 0;
+        const bool again = (k < n && p.probs) || drafted > 0.99 * sh.row_sum[k];
+        if (again) {
+            if (k < n && p.probs) {
+                row.q = p.probs + ((size_t)s * p.max_drafts + k) * V;
+                row.scale = 1.0 / sh.row_sum[k];
+            }
+            parts = warps, part0 = 0, per = ((int)steps + warps - 1) / warps;
+            const int i0 = min((int)steps, me * per), i1 = min((int)steps, i0 + per);
+            double mine = 0.0;
+            VfLoad a, b;
+            vf_load(row, i0, &a);
+            vf_load(row, i0 + 1, &b);  // (behind the row nothing is read)
+            for (int i = i0; i < i1; ++i) {
+                const VfLoad now = a;
+                a = b;
+                vf_load(row, i + 2, &b);
+                const VfFour f = vf_weights(row, now, i, sh.tab);
+                mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
+            }
+            mine = warp_sum(mine);
+            if (lane == 0) sh.part[warp] = mine;
+            cluster_barrier();
+        } else {
+            part0 = (int)(k * steps / run);
+            parts = (int)(((k + 1) * steps - 1) / run) - part0 + 1;
+        }
+        const int entries = (parts + 31) / 32;  // of a lane, one behind the other: they lie 32 apart
+        for (int i = tid; i < entries * 32; i += kVfThreads) {
+            double y = 0.0;
+            if (i < parts) {
+                const int w = part0 + i, from = w / kVfWarps;
+                if (again) {
+                    y = cluster_read(&sh.part[w % kVfWarps], from);
+                } else {
+                    const int slot = k - (int)(w * run / steps);
+                    const double m2 = (double)cluster_read(&sh.m[w % kVfWarps][slot], from);
+                    y = cluster_read(&sh.sum[w % kVfWarps][slot], from) * vf_exp0((m2 - row.m) * inv, sh.tab);
+                    if (row.out >= 0 && (unsigned)((row.out + row.shift) / kVfStep + k * steps) / run == (unsigned)w) {
+                        y -= drafted;
+                        if (y < 1e-12 * sh.row_sum[k]) y = 0.0;  // rounding, if the part had nothing else
+                    }
+                }
+            }
+            sh.all[i % entries * 32 + i / entries] = y;
+        }
+        __syncthreads();
         // the part that holds the token, and what lies before it
-        const int entries = warps / 32;  // of a lane, one behind the other
         double own = 0.0, base = 0.0;
         for (int i = 0; i < entries; ++i) own += sh.all[i * 32 + lane];
         double before = own;
@@ -385,6 +396,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             const double y = __shfl_up_sync(0xFFFFFFFFu, before, o);
             if (lane >= o) before += y;
         }
+        const double target = (double)last_u * __shfl_sync(0xFFFFFFFFu, before, 31);
         before -= own;
         int part = 0x7FFFFFFF, last = -1;
         for (int i = 0; i < entries; ++i) {
@@ -402,9 +414,11 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         const bool over = part != 0x7FFFFFFF;
         if (!over) part = last;  // (u of 1 or more): the last token of any weight
         token = -2;              // written by the part's CTA
-        if (part >= 0 && part / kVfWarps == rank) {
+        if (part >= 0 && (part0 + part) / kVfWarps == rank) {
             // this CTA has the part: its warps take its steps side by side
-            const int p0 = min((int)steps, part * per), p1 = min((int)steps, p0 + per);
+            const int w = part0 + part, at0 = again ? w * per : (int)max(w * run, k * steps) - (int)(k * steps),
+                      at1 = again ? at0 + per : (int)min((w + 1) * run, (k + 1) * steps) - (int)(k * steps);
+            const int p0 = min((int)steps, at0), p1 = min((int)steps, at1);
             int found = -1, some = -1;
             for (int i = p0; i < p1 && found < 0; i += kVfWarps) {
                 VfLoad l;
@@ -455,7 +469,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             // nothing has weight: the row's first maximum
             if (tid == 0) sh.token = 0x7FFFFFFF;
             __syncthreads();
-            for (int i = i0; i < i1; ++i) {
+            for (int i = me; i < (int)steps; i += warps) {
                 const int at = 4 * (32 * i + lane) - row.shift;
                 const float4 v = vf_load4(row.x, V, at, -INFINITY);
                 const float top = sh.row_m[k];
