@@ -8,19 +8,23 @@
 // Both products run on the tensor cores (m16n8k16, fp16 operands, fp32 sums)
 // without losing the query's or the weights' precision: the cached values are
 // fp16 numbers by definition, and an fp32 operand x enters as two fp16 numbers,
-// hi = fp16(x) and lo = fp16(x - hi), which together hold 22 bits.  The 16 rows
-// of an operand are the hi and the lo parts of 8 query rows (the heads of one KV
-// head, row after row), so a decode step of up to 8 heads per KV head needs no
-// product twice; the two halves of a result are added in fp32.  Queries are
-// scaled by a power of two into fp16's range, weights by 2^14, both exactly.
+// hi = fp16(x) and lo = fp16(x - hi), which together hold 22 bits.  The cache is
+// the 16-row operand, straight from its codes (keys: 16 positions, values: 16
+// dimensions), the query rows the 8-column one: 4 rows (the heads of one KV head,
+// row after row) as hi and lo columns, whose two results a lane holds side by
+// side and adds in fp32.  Queries are scaled by a power of two into fp16's range,
+// weights by 2^14, both exactly.  (With the query as the 16-row operand, 8 rows
+// times hi and lo, a decode step of 4 heads a KV head left half of it empty: 1037
+// instructions a tile of 32 positions and warp, now about half.)
 //
-// Work is cut into chunks of 256 positions, each one softmax pass with a running
-// maximum: a CTA's four warps take two tiles of 32 positions each, their partial
+// Work is cut into chunks of 256 positions, 64 (two tiles) a warp: scores, their
+// maximum, weights, weighted values, with no rescaling.  A CTA's four warps'
 // results (maximum, sum, weighted values) are joined in shared memory, and a
 // second kernel joins the chunks of a row.  Chunks, tiles and the order of every
 // sum go by position alone, so a row's result does not depend on what else is in
 // the call, bit for bit.  CTAs stay resident and take equal runs of the chunks
-// of all sequences, so that unequal lengths cost nothing.
+// of all sequences, so that unequal lengths cost nothing; a warp's keys of the
+// next chunk load while it weights values, and the values while it scores.
 #include "ovf_q4.cuh"
 
 namespace ovf {
@@ -28,22 +32,23 @@ namespace ovf {
 static constexpr int kAqWarps = 4;
 static constexpr int kAqThreads = kAqWarps * 32;
 static constexpr int kAqChunk = 256;               // positions of a chunk: kAqWarps warps x 2 tiles
-static constexpr int kAqRows = 8;                  // query rows of an operand (hi and lo parts)
 static constexpr float kAqLift = 14.0f;            // weights are held times 2^14: lo parts stay normal fp16 numbers
 static_assert(kAqChunk == kAqWarps * 2 * kQ4Tile, "two tiles a warp");
 
-// CTAs per SM and stages of the tile ring of a warp, by head_dim.
-__host__ __device__ constexpr int aq_ctas(int ng) { return ng <= 4 ? 3 : 2; }
-__host__ __device__ constexpr int aq_stages(int ng) { return ng <= 2 ? 4 : ng == 4 ? 2 : 2; }
-
-template <int NG>
-struct AqSmem {
+// A call's shape in the template: NG groups of 32 dimensions, NT operands of 4
+// query rows that share the cache's operand.
+template <int NG, int NT>
+struct AqShape {
     static constexpr int HD = NG * 32;
-    static constexpr int kTile = 2 * q4_tile_bytes(HD);  // keys, then values
-    static constexpr int kRing = kAqWarps * aq_stages(NG) * kTile;
+    static constexpr int kRows = 4 * NT;                 // query rows of an item
+    static constexpr int kTile = q4_tile_bytes(HD);
+    static constexpr int kSide = 2 * kTile;              // a warp's keys (or values) of a chunk
     static constexpr int MD = HD < 128 ? HD : 128;       // dimensions joined at a time
-    static constexpr int kMerge = kAqWarps * kAqRows * MD * 4;
-    static constexpr int kTotal = kRing + kMerge + kAqWarps * kAqRows * 8 + kAqWarps * aq_stages(NG) * 8;
+    static constexpr int kPad = MD + 8;                  // (rows of the join: no two lanes on one bank)
+    static constexpr int kRing = kAqWarps * 2 * kSide;
+    static constexpr int kMerge = kAqWarps * kRows * kPad * 4;
+    static constexpr int kTotal = kRing + kMerge + kAqWarps * kRows * 8 + kAqWarps * 2 * 8;
+    static constexpr int kCtas = NG == 8 ? 2 : NT == 2 ? 3 : 4;  // per SM
 };
 
 struct AqParams {
@@ -64,11 +69,18 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The transpose of an 8 x 8 matrix of fp16: lane 4 e + t gives and gets row e, columns 2 t and 2 t + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 // Pair i (codes i and i + 4) of a word as two fp16 numbers 1 + c / 16.
@@ -80,32 +92,41 @@ __device__ __forceinline__ __half2 q4_pair(uint32_t w) {
     return bits_h2(r);
 }
 
-// x and y as hi and lo parts, each a pair of fp16.
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+// hi and lo part of x, as a pair.
+__device__ __forceinline__ uint32_t split1(float x) {
+    const __half h = __float2half_rn(x);
+    return h2_bits(__halves2half2(h, __float2half_rn(x - __half2float(h))));
 }
 
-// The sequences' chunks as one list: per sequence [kv head][operand of 8 rows][chunk].
+// The values of eight codes that share D and M (keys) or have a pair each (values).
+__device__ __forceinline__ void q4_values(uint32_t w, __half2 d0, __half2 m0, __half2 d1, __half2 m1, __half2 d2, __half2 m2,
+                                          __half2 d3, __half2 m3, uint32_t (&v)[4]) {
+    v[0] = h2_bits(__hfma2(d0, q4_pair<0>(w), m0));
+    v[1] = h2_bits(__hfma2(d1, q4_pair<1>(w), m1));
+    v[2] = h2_bits(__hfma2(d2, q4_pair<2>(w), m2));
+    v[3] = h2_bits(__hfma2(d3, q4_pair<3>(w), m3));
+}
+
+// The sequences' chunks as one list: per sequence [kv head][KR query rows][chunk].
 struct AqItem {
     Q4View w;
     int s, left;               // items of this sequence behind this one
-    int chunks, tiles8, chunk, mt, h;  // chunks and operands of the sequence; this item's
+    int chunks, groups, chunk, mt, h;  // chunks and groups of KR rows of the sequence; this item's
 };
 
+template <int KR>
 __device__ __forceinline__ int aq_count(const Q4Source &src, int s, int G) {
     Q4View w;
     if (s >= src.n_seq || !q4_view(src, s, &w)) return 0;
-    return src.KVH * ((w.count * G + kAqRows - 1) / kAqRows) * ((w.pos + w.count + kAqChunk - 1) / kAqChunk);
+    return src.KVH * ((w.count * G + KR - 1) / KR) * ((w.pos + w.count + kAqChunk - 1) / kAqChunk);
 }
 
 // Item `target` of the list that starts with sequence `from`; false if it has fewer.
+template <int KR>
 __device__ __forceinline__ bool aq_locate(const Q4Source &src, int G, int from, long long target, AqItem *it) {
     const int lane = threadIdx.x & 31;
     for (int s0 = from; s0 < src.n_seq; s0 += 32) {
-        const int n = aq_count(src, s0 + lane, G);
+        const int n = aq_count<KR>(src, s0 + lane, G);
         long long sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -123,22 +144,23 @@ __device__ __forceinline__ bool aq_locate(const Q4Source &src, int G, int from, 
         it->s = s0 + l;
         q4_view(src, it->s, &it->w);
         it->chunks = (it->w.pos + it->w.count + kAqChunk - 1) / kAqChunk;
-        it->tiles8 = (it->w.count * G + kAqRows - 1) / kAqRows;
+        it->groups = (it->w.count * G + KR - 1) / KR;
         it->left = items - 1 - local;
         it->chunk = local % it->chunks;
-        it->mt = local / it->chunks % it->tiles8;
-        it->h = local / it->chunks / it->tiles8;
+        it->mt = local / it->chunks % it->groups;
+        it->h = local / it->chunks / it->groups;
         return true;
     }
     return false;
 }
 
+template <int KR>
 __device__ __forceinline__ bool aq_next(const Q4Source &src, int G, AqItem *it) {
-    if (it->left == 0) return aq_locate(src, G, it->s + 1, 0, it);
+    if (it->left == 0) return aq_locate<KR>(src, G, it->s + 1, 0, it);
     --it->left;
     if (++it->chunk == it->chunks) {
         it->chunk = 0;
-        if (++it->mt == it->tiles8) {
+        if (++it->mt == it->groups) {
             it->mt = 0;
             ++it->h;
         }
@@ -147,22 +169,24 @@ __device__ __forceinline__ bool aq_next(const Q4Source &src, int G, AqItem *it) 
 }
 
 // Positions of the item that any of its rows attends: [256 chunk, end).
+template <int KR>
 __device__ __forceinline__ int aq_end(const AqItem &it, int G) {
-    const int last_row = min(it.w.count - 1, (it.mt * kAqRows + kAqRows - 1) / G);
+    const int last_row = min(it.w.count - 1, (it.mt * KR + KR - 1) / G);
     return min((it.chunk + 1) * kAqChunk, it.w.pos + last_row + 1);
 }
 
-template <int NG>
-__global__ void __launch_bounds__(kAqThreads, aq_ctas(NG)) attention_q4_kernel(const AqParams p) {
-    constexpr int HD = NG * 32, NS = aq_stages(NG), TB = q4_tile_bytes(HD), MD = AqSmem<NG>::MD;
+template <int NG, int NT>
+__global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_q4_kernel(const AqParams p) {
+    using S = AqShape<NG, NT>;
+    constexpr int HD = NG * 32, KR = S::kRows, TB = S::kTile, MD = S::MD, PAD = S::kPad;
     extern __shared__ __align__(128) uint8_t smem[];
     const Q4Source &src = p.src;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = lane >> 2, t = lane & 3, G = p.H / src.KVH;
-    uint8_t *ring = smem + warp * NS * 2 * TB;
-    float *merge = reinterpret_cast<float *>(smem + AqSmem<NG>::kRing);                   // [warp][row][MD]
-    float2 *merge_ml = reinterpret_cast<float2 *>(merge + kAqWarps * kAqRows * MD);       // [warp][row]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(merge_ml + kAqWarps * kAqRows) + warp * NS;
-    if (lane < NS) mbar_init(&bars[lane], 1);
+    uint8_t *keys = smem + warp * 2 * S::kSide, *values = keys + S::kSide;
+    float *merge = reinterpret_cast<float *>(smem + S::kRing);                             // [warp][row][PAD]
+    float2 *merge_ml = reinterpret_cast<float2 *>(merge + kAqWarps * KR * PAD);            // [warp][row]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(merge_ml + kAqWarps * KR) + warp * 2;    // keys, values
+    if (lane < 2) mbar_init(&bars[lane], 1);
     fence_mbar_init();
     __syncwarp();
     pdl_wait();
@@ -171,263 +195,308 @@ __global__ void __launch_bounds__(kAqThreads, aq_ctas(NG)) attention_q4_kernel(c
     // this CTA's run of the list
     long long total = 0;
     for (int s0 = 0; s0 < src.n_seq; s0 += 32) {
-        int n = aq_count(src, s0 + lane, G);
+        int n = aq_count<KR>(src, s0 + lane, G);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
         total += n;
     }
     const long long lo = total * blockIdx.x / gridDim.x;
-    int left = (int)(total * (blockIdx.x + 1) / gridDim.x - lo);  // items to compute
-    AqItem it, ahead;
-    if (left <= 0 || !aq_locate(src, G, 0, lo, &it)) return;
-    ahead = it;
-    int ahead_left = left, ahead_tile = warp * 2, issued = 0, used = 0;
-    bool dead = false;
+    int left = (int)(total * (blockIdx.x + 1) / gridDim.x - lo);
+    AqItem it, next;
+    if (left <= 0 || !aq_locate<KR>(src, G, 0, lo, &it)) return;
 
-    // requests this warp's next tile, if its run has one
-    auto request = [&]() {
-        while (ahead_left > 0) {
-            const int p0 = ahead.chunk * kAqChunk + ahead_tile * kQ4Tile;
-            if (ahead_tile < warp * 2 + 2 && p0 < aq_end(ahead, G)) break;
-            ahead_tile = warp * 2;
-            --ahead_left;
-            if (ahead_left > 0 && !aq_next(src, G, &ahead)) ahead_left = 0;
-        }
-        if (ahead_left <= 0) return;
-        const int st = issued % NS;
+    // One side of this warp's part of an item: its tiles that hold attended positions, or none (false).
+    const uint64_t policy = l2_evict_first_policy();
+    auto request = [&](const AqItem &i, bool side) {
+        const int p0 = i.chunk * kAqChunk + warp * 2 * kQ4Tile, tiles = min(2, (aq_end<KR>(i, G) - p0 + kQ4Tile - 1) / kQ4Tile);
+        if (tiles <= 0) return;
         if (lane == 0) {
-            const size_t at = ((size_t)ahead.h * ahead.w.tiles + ahead.chunk * (kAqChunk / kQ4Tile) + ahead_tile) * TB;
-            const uint64_t pol = l2_evict_first_policy();
-            mbar_arrive_expect_tx(&bars[st], 2 * TB);
-            bulk_g2s(ring + st * 2 * TB, ahead.w.k + at, TB, &bars[st], pol);
-            bulk_g2s(ring + st * 2 * TB + TB, ahead.w.v + at, TB, &bars[st], pol);
+            const size_t at = ((size_t)i.h * i.w.tiles + p0 / kQ4Tile) * TB;
+            mbar_arrive_expect_tx(&bars[side], tiles * TB);
+            bulk_g2s(side ? values : keys, (side ? i.w.v : i.w.k) + at, tiles * TB, &bars[side], policy);
         }
-        ++issued;
-        ++ahead_tile;
     };
-#pragma unroll
-    for (int i = 0; i < NS; ++i) request();
+    request(it, false);
+    request(it, true);
 
-    uint32_t a[NG][2][4];  // query operand: [group][step]
-    float factor = 0.0f;   // score of this lane's row from its sum of products
-    int limit = 0;         // last position that the row attends
-    int have_h = -1, have_mt = -1, have_s = -1;
+    uint32_t q[NT][NG][4];  // query operand: pairs (0, 4) (1, 5) (2, 6) (3, 7) of this lane's dimensions
+    float factor[NT];       // a score from its sum of products, of row 4 nt + t
+    int limit[NT];          // last position that the row attends
+    int have_h = -1, have_mt = -1, have_s = -1, phase = 0;
+    bool dead = false;
 
     for (; left > 0; --left) {
         if (it.h != have_h || it.mt != have_mt || it.s != have_s) {
             have_h = it.h, have_mt = it.mt, have_s = it.s;
-            const int i = it.mt * kAqRows + e, r = i / G;
-            const bool real = r < it.w.count;
-            limit = real ? it.w.pos + r : 0x7FFFFFFF;  // (a row that is none: zeros, which nothing reads)
-            float x[NG][8];
-            if (real) {
-                const float4 *q = reinterpret_cast<const float4 *>(
-                    p.q + (((size_t)it.s * src.rows + r) * p.H + it.h * G + i % G) * HD + 8 * t);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float4 u = q[g * 8], v = q[g * 8 + 1];
-                    x[g][0] = u.x, x[g][1] = u.y, x[g][2] = u.z, x[g][3] = u.w;
-                    x[g][4] = v.x, x[g][5] = v.y, x[g][6] = v.z, x[g][7] = v.w;
-                }
-            } else {
+            for (int nt = 0; nt < NT; ++nt) {
+                // column e of the operand: row e / 2, its hi (even) or lo part
+                const int i = it.mt * KR + nt * 4 + (e >> 1), r = i / G;
+                const bool real = r < it.w.count;
+                float x[NG][8];
+                if (real) {
+                    const float4 *src4 = reinterpret_cast<const float4 *>(
+                        p.q + (((size_t)it.s * src.rows + r) * p.H + it.h * G + i % G) * HD + 8 * t);
 #pragma unroll
-                for (int g = 0; g < NG; ++g)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[g][k] = 0.0f;
-            }
-            if (it.w.cos) {  // Rope/RopeKernel.cs:46-93, each step rounded by itself
-                const int pos = real ? limit : 0;
-                const float *c = it.w.cos + (size_t)pos * (HD / 2), *sn = it.w.sin + (size_t)pos * (HD / 2);
-                if (!src.split_half) {
+                    for (int g = 0; g < NG; ++g) {
+                        const float4 u = src4[g * 8], v = src4[g * 8 + 1];
+                        x[g][0] = u.x, x[g][1] = u.y, x[g][2] = u.z, x[g][3] = u.w;
+                        x[g][4] = v.x, x[g][5] = v.y, x[g][6] = v.z, x[g][7] = v.w;
+                    }
+                } else {
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const float cc = c[g * 16 + 4 * t + k], ss = sn[g * 16 + 4 * t + k], x0 = x[g][2 * k],
-                                        x1 = x[g][2 * k + 1];
-                            x[g][2 * k] = fsub(fmul(x0, cc), fmul(x1, ss));
-                            x[g][2 * k + 1] = fadd(fmul(x0, ss), fmul(x1, cc));
-                        }
-                } else if (NG == 1) {
+                        for (int k = 0; k < 8; ++k) x[g][k] = 0.0f;
+                }
+                if (it.w.cos) {  // Rope/RopeKernel.cs:46-93, each step rounded by itself
+                    const int pos = real ? it.w.pos + r : 0;
+                    const float *c = it.w.cos + (size_t)pos * (HD / 2), *sn = it.w.sin + (size_t)pos * (HD / 2);
+                    if (!src.split_half) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float other = __shfl_xor_sync(0xFFFFFFFFu, x[0][k], 2);
-                        const float cc = c[(8 * t + k) & 15], ss = sn[(8 * t + k) & 15];
-                        x[0][k] = t < 2 ? fsub(fmul(x[0][k], cc), fmul(other, ss)) : fadd(fmul(other, ss), fmul(x[0][k], cc));
-                    }
-                } else {
+                        for (int g = 0; g < NG; ++g)
 #pragma unroll
-                    for (int g = 0; g < NG / 2; ++g)
+                            for (int k = 0; k < 4; ++k) {
+                                const float cc = c[g * 16 + 4 * t + k], ss = sn[g * 16 + 4 * t + k], x0 = x[g][2 * k],
+                                            x1 = x[g][2 * k + 1];
+                                x[g][2 * k] = fsub(fmul(x0, cc), fmul(x1, ss));
+                                x[g][2 * k + 1] = fadd(fmul(x0, ss), fmul(x1, cc));
+                            }
+                    } else if (NG == 1) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            const float cc = c[g * 32 + 8 * t + k], ss = sn[g * 32 + 8 * t + k], x0 = x[g][k],
-                                        x1 = x[(g + NG / 2) % NG][k];
-                            x[g][k] = fsub(fmul(x0, cc), fmul(x1, ss));
-                            x[(g + NG / 2) % NG][k] = fadd(fmul(x0, ss), fmul(x1, cc));
+                            const float other = __shfl_xor_sync(0xFFFFFFFFu, x[0][k], 2);
+                            const float cc = c[(8 * t + k) & 15], ss = sn[(8 * t + k) & 15];
+                            x[0][k] = t < 2 ? fsub(fmul(x[0][k], cc), fmul(other, ss)) : fadd(fmul(other, ss), fmul(x[0][k], cc));
                         }
-                }
-            }
-            float top = 0.0f;
+                    } else {
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+                        for (int g = 0; g < NG / 2; ++g)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[g][k]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            // the largest element to [2^14, 2^15), by a power of two
-            const int ex = min(max((__float_as_int(top) >> 23) & 255, 15), 254);
-            const float up = __int_as_float((268 - ex) << 23);
-            factor = p.scale2 * __int_as_float((ex - 14) << 23);
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-#pragma unroll
-                for (int k = 0; k < 4; ++k)  // pair (k, k + 4): registers 0 and 2 of step 0, then of step 1
-                    split2(x[g][k] * up, x[g][k + 4] * up, a[g][k >> 1][2 * (k & 1)], a[g][k >> 1][2 * (k & 1) + 1]);
-        }
-
-        float m = -INFINITY, l = 0.0f, o[NG * 4][4];
-#pragma unroll
-        for (int n = 0; n < NG * 4; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[n][k] = 0.0f;
-        const int end = aq_end(it, G), data_end = it.w.pos + it.w.count;
-        for (int tile = warp * 2; tile < warp * 2 + 2; ++tile) {
-            const int p0 = it.chunk * kAqChunk + tile * kQ4Tile;
-            if (p0 >= end) break;
-            const int st = used % NS;
-            if (!dead && !mbar_wait_sleep_bounded(&bars[st], (used / NS) & 1)) dead = true;
-            uint8_t *kt = ring + st * 2 * TB, *vt = kt + TB;
-            if (p0 + kQ4Tile > data_end) {
-                // what lies behind the sequence's data may be anything: its weights
-                // are 0, and its values must be numbers for that
-                if (p0 + lane >= data_end) {
-                    __half *vp = reinterpret_cast<__half *>(vt + q4_code_bytes(HD));
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        vp[q4_value_param(g, lane >> 3, lane & 7)] = __half(0.0f);
-                        vp[q4_value_param(g, lane >> 3, lane & 7) + 32] = __half(0.0f);
+                            for (int k = 0; k < 8; ++k) {
+                                const float cc = c[g * 32 + 8 * t + k], ss = sn[g * 32 + 8 * t + k], x0 = x[g][k],
+                                            x1 = x[(g + NG / 2) % NG][k];
+                                x[g][k] = fsub(fmul(x0, cc), fmul(x1, ss));
+                                x[(g + NG / 2) % NG][k] = fadd(fmul(x0, ss), fmul(x1, cc));
+                            }
                     }
-                    fence_proxy_async_smem();
                 }
-                __syncwarp();
-            }
-            // scores of this lane's row at positions p0 + 8 t + 2 j and + 1
-            float s[4][2];
+                float top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = 8 * (e >> 1) + 2 * j + (e & 1);
-                uint32_t kw[NG], kp[NG];
-                if (NG == 1) {
-                    kw[0] = *reinterpret_cast<const uint32_t *>(kt + (row * 4 + t) * 4);
-                    kp[0] = *reinterpret_cast<const uint32_t *>(kt + q4_code_bytes(HD) + row * 4);
-                } else if (NG == 2) {
-                    *reinterpret_cast<uint2 *>(kw) = *reinterpret_cast<const uint2 *>(kt + (row * 4 + t) * 8);
-                    *reinterpret_cast<uint2 *>(kp) = *reinterpret_cast<const uint2 *>(kt + q4_code_bytes(HD) + row * 8);
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(x[g][k]));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                // the largest element to [2^14, 2^15), by a power of two
+                const int ex = min(max((__float_as_int(top) >> 23) & 255, 15), 254);
+                const float up = __int_as_float((268 - ex) << 23);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x0 = x[g][k] * up, x1 = x[g][k + 4] * up;
+                        const __half2 hi = __floats2half2_rn(x0, x1);
+                        const float2 f = __half22float2(hi);
+                        q[nt][g][k] = h2_bits(e & 1 ? __floats2half2_rn(x0 - f.x, x1 - f.y) : hi);
+                    }
+                // of row 4 nt + t, whose operand the lanes of column 2 t formed
+                factor[nt] = p.scale2 * __int_as_float((__shfl_sync(0xFFFFFFFFu, ex, 8 * t) - 14) << 23);
+                const int row = (it.mt * KR + nt * 4 + t) / G;
+                limit[nt] = row < it.w.count ? it.w.pos + row : 0x7FFFFFFF;  // (a row that is none: zeros, which nothing reads)
+            }
+        }
+        const bool more = left > 1;
+        next = it;
+        if (more) aq_next<KR>(src, G, &next);
+
+        const int first = it.chunk * kAqChunk + warp * 2 * kQ4Tile, end = aq_end<KR>(it, G), data_end = it.w.pos + it.w.count;
+        const int tiles = min(2, (end - first + kQ4Tile - 1) / kQ4Tile);
+        float m[NT], l[NT], o[NT][NG * 2][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt] = -INFINITY, l[nt] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < NG * 2; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[nt][d][k] = 0.0f;
+        }
+        if (tiles > 0) {
+            // scores of row 4 nt + t at positions first + 32 tile + 8 (e / 2) + 4 (e % 2) + i
+            float s[NT][2][4];
+            if (!dead && !mbar_wait_sleep_bounded(&bars[0], phase)) dead = true;
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile) {
+                if (tile < tiles) {
+                    const uint8_t *kt = keys + tile * TB;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // positions i = 2 half and 2 half + 1: the operand's rows e and e + 8
+                        uint32_t w[2][NG], dm[2][NG];
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int row = 8 * (e >> 1) + 4 * (e & 1) + 2 * half + b;
+                            const uint8_t *wp = kt + (row * 4 + t) * NG * 4, *dp = kt + q4_code_bytes(HD) + row * NG * 4;
+                            if (NG == 1) {
+                                w[b][0] = *reinterpret_cast<const uint32_t *>(wp);
+                                dm[b][0] = *reinterpret_cast<const uint32_t *>(dp);
+                            } else if (NG == 2) {
+                                *reinterpret_cast<uint2 *>(w[b]) = *reinterpret_cast<const uint2 *>(wp);
+                                *reinterpret_cast<uint2 *>(dm[b]) = *reinterpret_cast<const uint2 *>(dp);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < NG / 4; ++i) {
+                                    reinterpret_cast<uint4 *>(w[b])[i] = reinterpret_cast<const uint4 *>(wp)[i];
+                                    reinterpret_cast<uint4 *>(dm[b])[i] = reinterpret_cast<const uint4 *>(dp)[i];
+                                }
+                            }
+                        }
+                        float c[NT][4] = {};
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            uint32_t v0[4], v1[4];
+                            __half2 D = __low2half2(bits_h2(dm[0][g])), M = __high2half2(bits_h2(dm[0][g]));
+                            q4_values(w[0][g], D, M, D, M, D, M, D, M, v0);
+                            D = __low2half2(bits_h2(dm[1][g])), M = __high2half2(bits_h2(dm[1][g]));
+                            q4_values(w[1][g], D, M, D, M, D, M, D, M, v1);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma_f16(c[nt], v0[0], v1[0], v0[1], v1[1], q[nt][g][0], q[nt][g][1]);
+                                mma_f16(c[nt], v0[2], v1[2], v0[3], v1[3], q[nt][g][2], q[nt][g][3]);
+                            }
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            s[nt][tile][2 * half] = (c[nt][0] + c[nt][1]) * factor[nt];
+                            s[nt][tile][2 * half + 1] = (c[nt][2] + c[nt][3]) * factor[nt];
+                        }
+                    }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < NG / 4; ++i) {
-                        reinterpret_cast<uint4 *>(kw)[i] = reinterpret_cast<const uint4 *>(kt + (row * 4 + t) * NG * 4)[i];
-                        reinterpret_cast<uint4 *>(kp)[i] =
-                            reinterpret_cast<const uint4 *>(kt + q4_code_bytes(HD) + row * NG * 4)[i];
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[nt][tile][i] = -INFINITY;
                 }
-                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            uint32_t x[NT][2][4];  // weights as operands
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int at = first + 8 * (e >> 1) + 4 * (e & 1);
+                if (__any_sync(0xFFFFFFFFu, first + 2 * kQ4Tile - 1 > limit[nt])) {
+#pragma unroll
+                    for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (at + tile * kQ4Tile + i > limit[nt]) s[nt][tile][i] = -INFINITY;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, s[nt][tile][i]);
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+                m[nt] = top;
+                const float base = (top == -INFINITY ? 0.0f : top) - kAqLift;  // (nothing attended: weights of 0)
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = ex2(s[nt][tile][i] - base);
+                        l[nt] += w;
+                        x[nt][tile][i] = transpose8(split1(w));
+                    }
+            }
+
+            // (the maxima stand: every read of the keys is behind this warp)
+            if (more) request(next, false);
+            if (!dead && !mbar_wait_sleep_bounded(&bars[1], phase)) dead = true;
+#pragma unroll
+            for (int tile = 0; tile < 2; ++tile) {
+                if (tile >= tiles) break;
+                uint8_t *vt = values + tile * TB;
+                if (first + (tile + 1) * kQ4Tile > data_end) {
+                    // what lies behind the sequence's data may be anything: its weights
+                    // are 0, and its values must be numbers for that
+                    if (first + tile * kQ4Tile + lane >= data_end) {
+                        __half *vp = reinterpret_cast<__half *>(vt + q4_code_bytes(HD));
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            vp[q4_value_param(g, lane >> 3, lane & 7)] = __half(0.0f);
+                            vp[q4_value_param(g, lane >> 3, lane & 7) + 32] = __half(0.0f);
+                        }
+                        fence_proxy_async_smem();
+                    }
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const __half2 dm = bits_h2(kp[g]), D = __low2half2(dm), M = __high2half2(dm);
-                    mma_f16(c, a[g][0], h2_bits(__hfma2(D, q4_pair<0>(kw[g]), M)), h2_bits(__hfma2(D, q4_pair<1>(kw[g]), M)));
-                    mma_f16(c, a[g][1], h2_bits(__hfma2(D, q4_pair<2>(kw[g]), M)), h2_bits(__hfma2(D, q4_pair<3>(kw[g]), M)));
-                }
-                s[j][0] = (c[0] + c[2]) * factor;
-                s[j][1] = (c[1] + c[3]) * factor;
-            }
-            if (__any_sync(0xFFFFFFFFu, p0 + kQ4Tile - 1 > limit)) {
+                    const uint4 d = *reinterpret_cast<const uint4 *>(vt + q4_code_bytes(HD) + g * 128 + t * 16);
+                    const uint4 b = *reinterpret_cast<const uint4 *>(vt + q4_code_bytes(HD) + g * 128 + 64 + t * 16);
+                    const uint4 w = *reinterpret_cast<const uint4 *>(vt + ((g * 8 + e) * 4 + t) * 16);
+                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                    for (int half = 0; half < 2; ++half) {  // dimensions 32 g + 16 half + e and + 8
+                        uint32_t v0[4], v1[4];
+                        q4_values(words[2 * half], bits_h2(d.x), bits_h2(b.x), bits_h2(d.y), bits_h2(b.y), bits_h2(d.z),
+                                  bits_h2(b.z), bits_h2(d.w), bits_h2(b.w), v0);
+                        q4_values(words[2 * half + 1], bits_h2(d.x), bits_h2(b.x), bits_h2(d.y), bits_h2(b.y), bits_h2(d.z),
+                                  bits_h2(b.z), bits_h2(d.w), bits_h2(b.w), v1);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (p0 + 8 * t + 2 * j + i > limit) s[j][i] = -INFINITY;
-            }
-            float top = m;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(s[j][0], s[j][1]));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            const float base = top == -INFINITY ? 0.0f : top;  // nothing attended so far: weights of 0
-            const float keep = ex2(m - base);
-            m = top;
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    s[j][i] = ex2(s[j][i] - base + kAqLift);
-                    sum += s[j][i];
-                }
-            l = l * keep + sum;
-            if (__any_sync(0xFFFFFFFFu, keep != 1.0f)) {
-#pragma unroll
-                for (int n = 0; n < NG * 4; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[n][k] *= keep;
-            }
-            // weights as operands: pairs (0, 4) (1, 5), then (2, 6) (3, 7) of positions 8 t ..
-            uint32_t w0[4], w1[4];
-            split2(s[0][0], s[2][0], w0[0], w0[1]);
-            split2(s[0][1], s[2][1], w0[2], w0[3]);
-            split2(s[1][0], s[3][0], w1[0], w1[1]);
-            split2(s[1][1], s[3][1], w1[2], w1[3]);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const uint4 dw = *reinterpret_cast<const uint4 *>(vt + q4_code_bytes(HD) + g * 128 + t * 16);
-                const uint4 mw = *reinterpret_cast<const uint4 *>(vt + q4_code_bytes(HD) + g * 128 + 64 + t * 16);
-                const uint4 cw = *reinterpret_cast<const uint4 *>(vt + ((g * 8 + e) * 4 + t) * 16);
-                const uint32_t words[4] = {cw.x, cw.y, cw.z, cw.w};
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    mma_f16(o[g * 4 + n], w0, h2_bits(__hfma2(bits_h2(dw.x), q4_pair<0>(words[n]), bits_h2(mw.x))),
-                            h2_bits(__hfma2(bits_h2(dw.y), q4_pair<1>(words[n]), bits_h2(mw.y))));
-                    mma_f16(o[g * 4 + n], w1, h2_bits(__hfma2(bits_h2(dw.z), q4_pair<2>(words[n]), bits_h2(mw.z))),
-                            h2_bits(__hfma2(bits_h2(dw.w), q4_pair<3>(words[n]), bits_h2(mw.w))));
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_f16(o[nt][2 * g + half], v0[0], v1[0], v0[1], v1[1], x[nt][tile][0], x[nt][tile][1]);
+                            mma_f16(o[nt][2 * g + half], v0[2], v1[2], v0[3], v1[3], x[nt][tile][2], x[nt][tile][3]);
+                        }
+                    }
                 }
             }
-            __syncwarp();
-            ++used;
-            request();
+            phase ^= 1;
+        } else if (more) {
+            request(next, false);
         }
 
         // the four warps' results to one
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        if (t == 0) merge_ml[warp * kAqRows + e] = make_float2(m, l);
-        __syncthreads();
-        float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kAqWarps; ++w) top = fmaxf(top, merge_ml[w * kAqRows + e].x);
-        const float share = m == -INFINITY ? 0.0f : ex2(m - top);
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) l[nt] += __shfl_xor_sync(0xFFFFFFFFu, l[nt], w);
+            if (e == 0) merge_ml[warp * KR + nt * 4 + t] = make_float2(m[nt], l[nt]);
+        }
+        __syncthreads();
+        float share[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kAqWarps; ++w) top = fmaxf(top, merge_ml[w * KR + nt * 4 + t].x);
+            share[nt] = m[nt] == -INFINITY ? 0.0f : ex2(m[nt] - top);
+        }
 #pragma unroll
         for (int d0 = 0; d0 < HD; d0 += MD) {
 #pragma unroll
-            for (int n = 0; n < MD / 8; ++n) {
-                // lane 4 e + t: dimensions 8 n + 2 t and + 1 of row e
-                const float(&c)[4] = o[d0 / 8 + n];
-                *reinterpret_cast<float2 *>(&merge[(warp * kAqRows + e) * MD + 8 * n + 2 * t]) =
-                    make_float2((c[0] + c[2]) * share, (c[1] + c[3]) * share);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int d = 0; d < MD / 16; ++d) {
+                    const float(&c)[4] = o[nt][d0 / 16 + d];
+                    float *to = &merge[(warp * KR + nt * 4 + t) * PAD + 16 * d + e];
+                    to[0] = (c[0] + c[1]) * share[nt];
+                    to[8] = (c[2] + c[3]) * share[nt];
+                }
+            // (the last sums are written: every read of the values is behind this warp)
+            if (more && d0 + MD == HD) request(next, true);
             __syncthreads();
-            for (int x = threadIdx.x; x < kAqRows * MD / 4; x += kAqThreads) {
-                const int row = x / (MD / 4), d = x % (MD / 4) * 4, i = it.mt * kAqRows + row, r = i / G;
+            for (int x = threadIdx.x; x < KR * MD / 4; x += kAqThreads) {
+                const int row = x / (MD / 4), d = x % (MD / 4) * 4, i = it.mt * KR + row, r = i / G;
                 const int row_last = it.w.pos + r;
                 if (r >= it.w.count || row_last < it.chunk * kAqChunk) continue;  // no row, or one that ends before
                 float mm = -INFINITY, sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kAqWarps; ++w) mm = fmaxf(mm, merge_ml[w * kAqRows + row].x);
+                for (int w = 0; w < kAqWarps; ++w) mm = fmaxf(mm, merge_ml[w * KR + row].x);
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int w = 0; w < kAqWarps; ++w) {
-                    const float2 ml = merge_ml[w * kAqRows + row];
+                    const float2 ml = merge_ml[w * KR + row];
                     sum += ml.x == -INFINITY ? 0.0f : ml.y * ex2(ml.x - mm);
-                    const float4 u = *reinterpret_cast<const float4 *>(&merge[(w * kAqRows + row) * MD + d]);
+                    const float4 u = *reinterpret_cast<const float4 *>(&merge[(w * KR + row) * PAD + d]);
                     v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
                 }
                 const size_t orow = ((size_t)it.s * src.rows + r) * p.H + it.h * G + i % G;
@@ -443,7 +512,7 @@ __global__ void __launch_bounds__(kAqThreads, aq_ctas(NG)) attention_q4_kernel(c
             }
             __syncthreads();
         }
-        if (left > 1 && !aq_next(src, G, &it)) break;
+        it = next;
     }
 }
 
@@ -500,21 +569,21 @@ int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx) {
     return 256 + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
 }
 
-template <int NG>
+template <int NG, int NT>
 static cudaError_t launch_aq(const AqParams &p, cudaStream_t st, bool pdl) {
-    constexpr int smem = AqSmem<NG>::kTotal;
+    using S = AqShape<NG, NT>;
     static PerDeviceOnce once;
     const int dev = current_device();
     if (once.pending(dev)) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(attention_q4_kernel<NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        const cudaError_t e = cudaFuncSetAttribute(attention_q4_kernel<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   S::kTotal);
         if (e != cudaSuccess) return e;
         once.mark(dev);
     }
-    const int G = p.H / p.src.KVH;
-    const int64_t most = (int64_t)p.src.n_seq * p.src.KVH * ((p.src.rows * (int64_t)G + kAqRows - 1) / kAqRows) * p.max_chunks;
-    const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(dev) * aq_ctas(NG));
-    cudaError_t e = launch_pdl(attention_q4_kernel<NG>, dim3(grid), dim3(kAqThreads), smem, st, pdl, p);
+    const int64_t rows = (int64_t)p.src.rows * (p.H / p.src.KVH);
+    const int64_t most = (int64_t)p.src.n_seq * p.src.KVH * ((rows + S::kRows - 1) / S::kRows) * p.max_chunks;
+    const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(dev) * S::kCtas);
+    cudaError_t e = launch_pdl(attention_q4_kernel<NG, NT>, dim3(grid), dim3(kAqThreads), S::kTotal, st, pdl, p);
     if (e != cudaSuccess || p.max_chunks == 1) return e;
     return launch_pdl(attention_q4_join_kernel<NG * 32>, dim3(p.H, p.src.rows, p.src.n_seq), dim3(kAqJoinThreads), 0, st,
                       true, p);
@@ -532,7 +601,9 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
     p.part = static_cast<float *>(scratch);
     p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.max_chunks * hd;
     cudaError_t e = cudaSuccess;
-#define OVF_CALL(NG) e = launch_aq<NG>(p, st, pdl)
+    // two operands share the cache's where there are rows for them (and registers)
+    const bool two = (int64_t)src.rows * (H / src.KVH) > 4 && hd < 256;
+#define OVF_CALL(NG) e = two ? launch_aq<NG, NG < 8 ? 2 : 1>(p, st, pdl) : launch_aq<NG, 1>(p, st, pdl)
     OVF_Q4_HD(hd, OVF_CALL)
 #undef OVF_CALL
     return cuda_status(e, "attention_q4");
