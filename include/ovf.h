@@ -372,6 +372,11 @@ int64_t ovf_model_weight_bytes(const ovf_model *m);
 #define OVF_KV_F32 0
 #define OVF_KV_Q8 1
 #define OVF_KV_F16 2
+/* The 4-bit cache (ovf_kv_q4_append): 5 bits per element, attended by
+ * ovf_attention_q4.  Decode, batch decode and verify give the same results as
+ * one another, bit for bit; a prompt's batched prefill is within rounding of the
+ * single-token loop.  No prefix snapshots. */
+#define OVF_KV_Q4 3
 
 /* ISlmInferenceEngine.CreateSession (Contracts/ISlmInferenceEngine.cs:9):
  * F32 KV cache. */
@@ -430,18 +435,30 @@ ovf_status ovf_session_set_option(ovf_session *s, int32_t option, int32_t value)
  * max, the greedy acceptance test) or NULL. */
 ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, float *logits_host,
                               int32_t *argmax_out);
+/* The verify forward with sampled acceptance (ovf_verify_drafts): tokens[0] is
+ * the committed token, tokens[1..n) its drafts, drawn from draft_probs [(n - 1) x
+ * vocab] (NULL: certain drafts, such as prompt lookup's).  uniforms: n numbers in
+ * [0, 1), one per draft and one for the next token.  The rows run as in
+ * ovf_session_verify; the session's position becomes that behind the accepted
+ * drafts, and *next_token_out (not decoded yet) is the token drawn there.
+ * temperature 0 or less accepts greedily.  Host pointers.  A row of logits
+ * without a distribution returns OVF_ESTATE, the accepted drafts standing. */
+ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int32_t n, const float *draft_probs,
+                                      const float *uniforms, float temperature, int32_t *accepted_out,
+                                      int32_t *next_token_out);
 /* KeyValueCache.TruncateTo (Runtime/KeyValueCache.cs:246) as
  * CachedLlamaSession.RollbackTo (:318) uses it: the position becomes length
  * (0 <= length <= position); rejected draft rows are dropped. */
 ovf_status ovf_session_truncate(ovf_session *s, int32_t length);
 /* Bytes of one side (keys or values) of a prefix snapshot at the current
- * position: n_layers * n_kv_heads * position * head_dim * element size. */
+ * position: n_layers * n_kv_heads * position * head_dim * element size (0 for a
+ * Q4 cache, which has none). */
 int64_t ovf_session_prefix_bytes(const ovf_session *s);
 /* CachedLlamaSession.SavePrefix (:231) -> KeyValueCache.Snapshot
  * (Runtime/KeyValueCache.cs:264): the live rows packed
  * [layer][kv_head][position][head_dim] into host buffers of
  * ovf_session_prefix_bytes each, in the cache's element type (F32; fp16 for
- * an fp16 cache).  A Q8 cache returns OVF_EUNSUPPORTED, as the reference's
+ * an fp16 cache).  A Q8 or Q4 cache returns OVF_EUNSUPPORTED, as the reference's
  * ThrowIfQuantized does. */
 ovf_status ovf_session_save_prefix(const ovf_session *s, void *keys, void *values, int32_t *length_out);
 /* CachedLlamaSession.RestorePrefix (:242) -> KeyValueCache.RestoreFrom

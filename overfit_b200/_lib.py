@@ -106,6 +106,7 @@ SIGNATURES = {
     "ovf_model_tp_export": (I32, [P, P]),
     "ovf_model_tp_connect": (I32, [P, P]),
     "ovf_session_verify": (I32, [P, P, I32, P, P]),
+    "ovf_session_verify_sampled": (I32, [P, P, I32, P, P, F, P, P]),
     "ovf_session_truncate": (I32, [P, I32]),
     "ovf_session_prefix_bytes": (I64, [P]),
     "ovf_session_save_prefix": (I32, [P, P, P, P]),

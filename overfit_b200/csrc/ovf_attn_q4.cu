@@ -609,6 +609,19 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
     return cuda_status(e, "attention_q4");
 }
 
+ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
+                                    void *scratch, int scratch_rows, cudaStream_t st) {
+    for (int r = 0; r < src.rows; r += scratch_rows) {
+        Q4Source part = src;
+        part.pos0 = src.pos0 + r;
+        part.rows = std::min(scratch_rows, src.rows - r);
+        const size_t at = (size_t)r * H * hd;
+        const ovf_status e = launch_attention_q4(part, H, hd, q + at, out + at, scale, scratch, st, false);
+        if (e) return e;
+    }
+    return OVF_OK;
+}
+
 }  // namespace ovf
 
 extern "C" {

@@ -160,6 +160,14 @@ ovf_status launch_moe_combine_rows(const float *a, const float *slot, const floa
 ovf_status launch_gather_rows(const float *src, const int32_t *rows, int n, int width, float *dst, cudaStream_t st);
 ovf_status launch_scatter_slots(const float *src, const int32_t *rows, const int32_t *slots, int n, int K, int width,
                                 float *dst, cudaStream_t st);
+// ovf_verify.cu: acceptance of drafted tokens and the draw of the next one.
+struct VerifyParams {
+    const float *logits, *probs, *uniforms, *temperatures;
+    const int32_t *drafts, *counts;
+    int32_t *accepted, *token;
+    int max_drafts, vocab;
+};
+ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st);
 ovf_status launch_take_error(int *dev_slot, cudaStream_t st);
 ovf_status launch_exp(const float *x, float *y, int64_t n, cudaStream_t st);
 ovf_status launch_silu_mul(const float *g, const float *u, float *h, int64_t n, cudaStream_t st, bool pdl);

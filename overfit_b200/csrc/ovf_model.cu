@@ -15,6 +15,7 @@
 //   GEMV  rmsnorm | lm head -> logits + argmax     final norm, ProjectLogits, TokenSampler.ArgMax
 // The argmax is fed back on the device, so greedy generation replays the
 // graph with no host round trip.
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
@@ -23,6 +24,7 @@
 #include <vector>
 
 #include "ovf_internal.cuh"
+#include "ovf_q4.cuh"
 
 using namespace ovf;
 
@@ -100,6 +102,11 @@ struct ovf_model {
     int32_t *btok_host = nullptr;  // pinned
     std::atomic<bool> batch_busy{false};  // one ovf_session_decode_batch at a time per model
     MoeRows bmoe;                          // MoE scratch of the batch rows
+    // 4-bit caches of a batch's sessions, and the attention scratch for them
+    Q4Seq *bq4 = nullptr;
+    std::vector<Q4Seq> bq4_host;
+    void *bq4_scratch = nullptr;
+    size_t bq4_scratch_bytes = 0;
     // tensor parallelism (world > 1): this rank's share of heads, FFN rows
     // and vocabulary; the exchange arena (IPC-exported) and the peers'
     int tp_rank = 0, tp_world = 1;
@@ -150,6 +157,11 @@ struct ovf_session {
     // speculative verify: per-row logits and argmax of one verify batch
     float *vlogits = nullptr;
     int32_t *vargmax = nullptr;
+    // 4-bit cache: scratch of its attention (a decoded row; the rows of a batch)
+    void *q4_scratch = nullptr, *q4_rows_scratch = nullptr;
+    // sampled verify: the drafts' probabilities, uniforms | temperature, accepted | next token
+    float *vprobs = nullptr, *vrandom = nullptr;
+    int32_t *vresult = nullptr;
     std::vector<void *> allocs;
 };
 
@@ -228,6 +240,32 @@ ovf_tensor host_vec_slice(const ovf_tensor &t, int64_t i0, int64_t n) {
     v.cols = n;
     return v;
 }
+
+// Bytes of one side of one layer's KV cache of this rank's heads.
+size_t kv_layer_bytes(const ovf_model *m, int kv_dtype, int max_ctx) {
+    const int hd = m->cfg.head_dim;
+    if (kv_dtype == OVF_KV_Q4) return (size_t)ovf_kv_q4_bytes(m->kvh_loc, hd, max_ctx);
+    return (size_t)m->kvh_loc * max_ctx * hd * (kv_dtype == OVF_KV_F32 ? 4 : kv_dtype == OVF_KV_Q8 ? 1 : 2);
+}
+
+// Rows of a 4-bit session's layer at pos0 .. (or at the device step's position).
+Q4Source q4_of(const ovf_session *s, int layer, int rows, int pos0, const int *pos_dev) {
+    Q4Source q{};
+    const size_t lb = kv_layer_bytes(s->m, OVF_KV_Q4, s->max_ctx);
+    q.k = static_cast<uint8_t *>(s->kc) + layer * lb;
+    q.v = static_cast<uint8_t *>(s->vc) + layer * lb;
+    q.positions = pos_dev;
+    q.pos0 = pos0;
+    q.cos = s->rope_cos;
+    q.sin = s->rope_sin;
+    q.split_half = s->m->cfg.rope_split_half;
+    q.max_ctx = s->max_ctx;
+    q.rows = rows;
+    q.n_seq = 1;
+    q.KVH = s->m->kvh_loc;
+    return q;
+}
+constexpr int kQ4ScratchRows = 16;  // rows at a time of a 4-bit session's batches: bounds the scratch of a long context
 
 // Uploads an f32 vector (norm / bias).
 ovf_status upload_vec(ovf_model *m, const ovf_tensor &t, int64_t n, float **out, const char *what) {
@@ -647,9 +685,15 @@ ovf_status enqueue_step(ovf_session *s, bool with_logits) {
             add_prefetch(a.pf, L.gate);
             add_prefetch(a.pf, L.up);
         }
-        a.trace = tslot("attn");
-        a.no_kv_prefetch = env_flag("OVF_ATTN_NOPF") ? 1 : 0;
-        if ((r = launch_attention_exact(a, s->max_ctx, st, true, s->kv_dtype))) return r;
+        if (s->kv_dtype == OVF_KV_Q4) {
+            const Q4Source src = q4_of(s, l, 1, 0, &s->step->cur_pos);
+            if ((r = launch_kv_q4_append(src, hd, s->k, s->v, st, true))) return r;
+            if ((r = launch_attention_q4(src, H, hd, s->q, s->attn, a.scale, s->q4_scratch, st, true))) return r;
+        } else {
+            a.trace = tslot("attn");
+            a.no_kv_prefetch = env_flag("OVF_ATTN_NOPF") ? 1 : 0;
+            if ((r = launch_attention_exact(a, s->max_ctx, st, true, s->kv_dtype))) return r;
+        }
         prof_mark(st, "attn");
         {
             // Wo: per-head Q8_0 (G = hd/32 blocks per head), heads summed in
@@ -887,8 +931,10 @@ ovf_status prefill_alloc(ovf_session *s) {
     A((void **)&s->ptok, (size_t)(s->max_ctx + 1) * 4);
     A((void **)&s->pscale, 16);
     if (!st && c.n_experts > 0) st = moe_rows_alloc(c, kPrefillRows, s->allocs, &s->pmoe);
+    if (s->kv_dtype == OVF_KV_Q4)
+        A(&s->q4_rows_scratch, (size_t)attn_q4_scratch_bytes(1, kQ4ScratchRows, s->m->h_loc, c.head_dim, s->max_ctx));
     const int64_t pfl = attn_rows_scratch_floats(kPrefillRows, s->m->h_loc, s->max_ctx);
-    if (!st && attn_rows_supported(c.head_dim, s->kv_dtype) && pfl * 4 <= ((int64_t)512 << 20))
+    if (!st && s->kv_dtype != OVF_KV_Q4 && attn_rows_supported(c.head_dim, s->kv_dtype) && pfl * 4 <= ((int64_t)512 << 20))
         A((void **)&s->pattn, (size_t)pfl * 4);
     if (!st) s->pf_rows = kPrefillRows;
     return st;
@@ -1055,7 +1101,13 @@ ovf_status enqueue_prefill_batched(ovf_session *s, int n, bool all_rows = false)
             if ((r = quantize_rows_for(ar, L.wv, s->pn, M, D, &fam, st))) return r;
             if ((r = project_rows(ar, L.wv, L.bv, s->pv, M, st))) return r;
             const size_t esz = s->kv_dtype == OVF_KV_F32 ? 4 : s->kv_dtype == OVF_KV_Q8 ? 1 : 2;
-            {
+            if (s->kv_dtype == OVF_KV_Q4) {
+                const Q4Source src = q4_of(s, l, M, base + r0, nullptr);
+                if ((r = launch_kv_q4_append(src, hd, s->pk, s->pv, st, false))) return r;
+                if ((r = launch_attention_q4_rows(src, H, hd, s->pq, s->patt, 1.0f / sqrtf((float)hd), s->q4_rows_scratch,
+                                                  kQ4ScratchRows, st)))
+                    return r;
+            } else {
                 // every row's key and value are appended first, then one launch
                 // attends all rows (each causal at its own position)
                 AttnParams a{};
@@ -1163,18 +1215,75 @@ ovf_status batch_alloc(ovf_model *m) {
     return st;
 }
 
+// The table of n 4-bit sessions' caches on the device, and scratch for their
+// attention.  (A batch call ends behind its stream, so the last one's are idle.)
+ovf_status batch_q4_table(ovf_model *m, ovf_session *const *ss, int n, int max_ctx, cudaStream_t st) {
+    ovf_status r = OVF_OK;
+    if (!m->bq4 && (r = dalloc(m->allocs, (void **)&m->bq4, kBatchMax * sizeof(Q4Seq)))) return r;
+    const size_t need = (size_t)attn_q4_scratch_bytes(n, 1, m->h_loc, m->cfg.head_dim, max_ctx);
+    if (need > m->bq4_scratch_bytes) {
+        if (m->bq4_scratch) {
+            m->allocs.erase(std::find(m->allocs.begin(), m->allocs.end(), m->bq4_scratch));
+            cudaFree(m->bq4_scratch);
+            m->bq4_scratch = nullptr;
+            m->bq4_scratch_bytes = 0;
+        }
+        if ((r = dalloc(m->allocs, &m->bq4_scratch, need))) return r;
+        m->bq4_scratch_bytes = need;
+    }
+    m->bq4_host.resize(n);
+    for (int i = 0; i < n; ++i) {
+        const ovf_session *s = ss[i];
+        m->bq4_host[i] = Q4Seq{static_cast<uint8_t *>(s->kc), static_cast<uint8_t *>(s->vc),
+                               (int64_t)kv_layer_bytes(m, OVF_KV_Q4, s->max_ctx), s->rope_cos, s->rope_sin, s->pos, s->max_ctx};
+    }
+    return cuda_status(cudaMemcpyAsync(m->bq4, m->bq4_host.data(), n * sizeof(Q4Seq), cudaMemcpyHostToDevice, st),
+                       "4-bit cache table");
+}
+
 ovf_status enqueue_batch_decode(ovf_model *m, ovf_session *const *ss, int n, cudaStream_t st) {
     const ovf_model_config &c = m->cfg;
     const int D = c.d_model, H = c.n_heads, KVH = c.n_kv_heads, hd = c.head_dim, QD = H * hd, KD = KVH * hd;
     const RowBufs rb{ActRows{m->baq, m->bas, m->bab}, m->bx, m->ba, m->bn, m->bq, m->bk, m->bv, m->batt,
                      m->bg, m->bu, m->bh};
     ovf_status r;
+    int q4_ctx = 0;  // the longest of their contexts, if all caches are 4-bit
+    for (int i = 0; i < n; ++i) {
+        if (ss[i]->kv_dtype != OVF_KV_Q4) {
+            q4_ctx = 0;
+            break;
+        }
+        q4_ctx = std::max(q4_ctx, ss[i]->max_ctx);
+    }
+    if (q4_ctx && (r = batch_q4_table(m, ss, n, q4_ctx, st))) return r;
     if ((r = launch_embed_rows(m->btok, n, m->embed.type, m->embed.data, m->embed.scales, D, m->bx, st))) return r;
     for (int l = 0; l < c.n_layers; ++l) {
         const DevLayer &L = m->layers[l];
         if ((r = rows_norm_qkv(m, L, rb, n, st))) return r;
-        for (int i = 0; i < n; ++i) {
+        if (q4_ctx) {
+            // every session's row in one launch, over a table of their caches
+            Q4Source src{};
+            src.seqs = m->bq4;
+            src.layer = l;
+            src.split_half = c.rope_split_half;
+            src.max_ctx = q4_ctx;
+            src.rows = 1;
+            src.n_seq = n;
+            src.KVH = KVH;
+            if ((r = launch_kv_q4_append(src, hd, m->bk, m->bv, st, false))) return r;
+            if ((r = launch_attention_q4(src, H, hd, m->bq, m->batt, 1.0f / sqrtf((float)hd), m->bq4_scratch, st, false)))
+                return r;
+        }
+        for (int i = 0; i < (q4_ctx ? 0 : n); ++i) {
             ovf_session *s = ss[i];
+            if (s->kv_dtype == OVF_KV_Q4) {  // (among sessions of other cache types)
+                const Q4Source src = q4_of(s, l, 1, s->pos, nullptr);
+                if ((r = launch_kv_q4_append(src, hd, m->bk + (size_t)i * KD, m->bv + (size_t)i * KD, st, false))) return r;
+                if ((r = launch_attention_q4(src, H, hd, m->bq + (size_t)i * QD, m->batt + (size_t)i * QD,
+                                             1.0f / sqrtf((float)hd), s->q4_scratch, st, false)))
+                    return r;
+                continue;
+            }
             const size_t esz = s->kv_dtype == OVF_KV_F32 ? 4 : s->kv_dtype == OVF_KV_Q8 ? 1 : 2;
             AttnParams a{};
             a.q = m->bq + (size_t)i * QD;
@@ -1539,11 +1648,12 @@ ovf_status ovf_session_create(ovf_model *m, int32_t max_ctx, ovf_session **out) 
 ovf_status ovf_session_create_kv(ovf_model *m, int32_t max_ctx, int32_t kv_dtype, ovf_session **out) {
     OVF_CHECK_ARG(m && out, "ovf_session_create: null argument");
     OVF_CHECK_ARG(max_ctx > 0 && max_ctx <= (1 << 20), "ovf_session_create: bad max_ctx");
-    OVF_CHECK_ARG(kv_dtype == OVF_KV_F32 || kv_dtype == OVF_KV_Q8 || kv_dtype == OVF_KV_F16,
+    const bool q4 = kv_dtype == OVF_KV_Q4;
+    OVF_CHECK_ARG(kv_dtype == OVF_KV_F32 || kv_dtype == OVF_KV_Q8 || kv_dtype == OVF_KV_F16 || q4,
                   "ovf_session_create: unknown KV dtype %d", kv_dtype);
-    OVF_CHECK_ARG(attn_exact_supported(m->cfg.head_dim), "ovf_session_create: head_dim %d unsupported",
-                  m->cfg.head_dim);
-    OVF_CHECK_ARG(max_ctx <= attn_exact_max_seq(m->cfg.head_dim), "ovf_session_create: max_ctx too large");
+    OVF_CHECK_ARG(q4 ? q4_supported(m->cfg.head_dim) : attn_exact_supported(m->cfg.head_dim),
+                  "ovf_session_create: head_dim %d unsupported", m->cfg.head_dim);
+    OVF_CHECK_ARG(q4 || max_ctx <= attn_exact_max_seq(m->cfg.head_dim), "ovf_session_create: max_ctx too large");
     DeviceGuard guard(m->device);
     ovf_session *s = new ovf_session();
     s->m = m;
@@ -1558,9 +1668,10 @@ ovf_status ovf_session_create_kv(ovf_model *m, int32_t max_ctx, int32_t kv_dtype
     auto A = [&](void **p, size_t bytes) {
         if (!st) st = dalloc(s->allocs, p, bytes);
     };
-    const size_t esz = kv_dtype == OVF_KV_F32 ? 4 : kv_dtype == OVF_KV_Q8 ? 1 : 2;
-    A((void **)&s->kc, kv * esz);
-    A((void **)&s->vc, kv * esz);
+    const size_t kv_bytes = (size_t)c.n_layers * kv_layer_bytes(m, kv_dtype, max_ctx);
+    A((void **)&s->kc, kv_bytes);
+    A((void **)&s->vc, kv_bytes);
+    if (q4) A(&s->q4_scratch, (size_t)attn_q4_scratch_bytes(1, 1, m->h_loc, c.head_dim, max_ctx));
     if (kv_dtype == OVF_KV_Q8) {
         A((void **)&s->ks, kv / c.head_dim * 4);
         A((void **)&s->vs, kv / c.head_dim * 4);
@@ -1597,8 +1708,8 @@ ovf_status ovf_session_create_kv(ovf_model *m, int32_t max_ctx, int32_t kv_dtype
     if (!st) st = cuda_status(cudaMemset(s->counters, 0, (size_t)m->kvh_loc * 4), "memset");
     s->prefill_single = m->tp_world > 1;  // the batched prefill is not split over ranks
     if (!st) st = cuda_status(cudaMemset(s->step, 0, sizeof(DevStep)), "memset");
-    if (!st) st = cuda_status(cudaMemset(s->kc, 0, kv * esz), "memset");
-    if (!st) st = cuda_status(cudaMemset(s->vc, 0, kv * esz), "memset");
+    if (!st) st = cuda_status(cudaMemset(s->kc, 0, kv_bytes), "memset");
+    if (!st) st = cuda_status(cudaMemset(s->vc, 0, kv_bytes), "memset");
     if (!st) st = fill_rope_tables(s);
     if (!st) {
         s->pinned_cap = max_ctx + 1;
@@ -1803,8 +1914,9 @@ ovf_status ovf_session_set_option(ovf_session *s, int32_t option, int32_t value)
 // logits equal those a single-token decode of tokens[0..j] would give.
 constexpr int kVerifyMax = 64;
 
-ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, float *logits_host,
-                              int32_t *argmax_out) {
+// The checks and the forward that ovf_session_verify and _verify_sampled share;
+// leaves the rows' logits in vlogits and does not wait for them.
+static ovf_status verify_forward(ovf_session *s, const int32_t *tokens, int32_t n) {
     OVF_CHECK_ARG(s && tokens && n >= 1, "verify: bad arguments");
     OVF_CHECK_ARG(n <= kVerifyMax, "verify: at most %d rows per call, got %d", kVerifyMax, n);
     if (s->m->tp_world > 1) {
@@ -1819,7 +1931,6 @@ ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, 
                   s->max_ctx, s->pos, n);
     for (int i = 0; i < n; ++i)
         OVF_CHECK_ARG(tokens[i] >= 0 && tokens[i] < s->m->cfg.vocab, "token id %d out of range", tokens[i]);
-    DeviceGuard guard(s->m->device);
     OVF_CUDA_TRY(cudaStreamSynchronize(s->stream));
     ovf_status r = prefill_alloc(s);
     if (r) return r;
@@ -1835,11 +1946,67 @@ ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, 
     }
     s->pos += n;
     s->n_logits += 1;
+    return OVF_OK;
+}
+
+ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, float *logits_host,
+                              int32_t *argmax_out) {
+    OVF_CHECK_ARG(s, "verify: bad arguments");
+    DeviceGuard guard(s->m->device);
+    ovf_status r = verify_forward(s, tokens, n);
+    if (r) return r;
     if (logits_host)
         OVF_CUDA_TRY(cudaMemcpyAsync(logits_host, s->vlogits, (size_t)n * s->m->cfg.vocab * 4, cudaMemcpyDeviceToHost,
                                      s->stream));
     if (argmax_out) OVF_CUDA_TRY(cudaMemcpyAsync(argmax_out, s->vargmax, (size_t)n * 4, cudaMemcpyDeviceToHost, s->stream));
     return finish_call(s->stream, s->err_slot);
+}
+
+ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int32_t n, const float *draft_probs,
+                                      const float *uniforms, float temperature, int32_t *accepted_out,
+                                      int32_t *next_token_out) {
+    OVF_CHECK_ARG(s && uniforms && accepted_out && next_token_out, "verify: bad arguments");
+    DeviceGuard guard(s->m->device);
+    const size_t vocab = s->m->cfg.vocab;
+    ovf_status r = OVF_OK;
+    if (!s->vrandom) {
+        if ((r = dalloc(s->allocs, (void **)&s->vresult, 2 * 4))) return r;
+        if ((r = dalloc(s->allocs, (void **)&s->vrandom, (kVerifyMax + 1) * 4))) return r;
+    }
+    if (draft_probs && n > 1 && !s->vprobs &&
+        (r = dalloc(s->allocs, (void **)&s->vprobs, (size_t)(kVerifyMax - 1) * vocab * 4)))
+        return r;
+    const int base = s->pos;
+    if ((r = verify_forward(s, tokens, n))) return r;
+    // from here on the rows are in the cache: a failure leaves the session to be reset
+    const cudaStream_t st = s->stream;
+    float random[kVerifyMax + 1];
+    memcpy(random, uniforms, (size_t)n * 4);
+    random[n] = temperature;
+    int32_t result[2] = {0, 0};
+    auto sample = [&]() -> ovf_status {
+        OVF_CUDA_TRY(cudaMemcpyAsync(s->vrandom, random, (size_t)(n + 1) * 4, cudaMemcpyHostToDevice, st));
+        if (draft_probs && n > 1)
+            OVF_CUDA_TRY(cudaMemcpyAsync(s->vprobs, draft_probs, (size_t)(n - 1) * vocab * 4, cudaMemcpyHostToDevice, st));
+        const VerifyParams p{s->vlogits, draft_probs && n > 1 ? s->vprobs : nullptr, s->vrandom, s->vrandom + n, s->ptok + 1,
+                             nullptr, s->vresult, s->vresult + 1, n - 1, (int)vocab};
+        ovf_status e = launch_verify_drafts(p, 1, st);
+        if (e) return e;
+        OVF_CUDA_TRY(cudaMemcpyAsync(result, s->vresult, sizeof(result), cudaMemcpyDeviceToHost, st));
+        return finish_call(st, s->err_slot);
+    };
+    if ((r = sample())) {
+        s->needs_reset = true;
+        return r;
+    }
+    if ((r = ovf_session_truncate(s, base + 1 + result[0]))) return r;
+    *accepted_out = result[0];
+    *next_token_out = result[1];
+    if (result[1] < 0) {
+        set_error("verify: the logits behind %d accepted drafts are no distribution", result[0]);
+        return OVF_ESTATE;
+    }
+    return OVF_OK;
 }
 
 // KeyValueCache.TruncateTo (Runtime/KeyValueCache.cs:246-258) as
@@ -1862,6 +2029,7 @@ static size_t kv_elem_bytes(const ovf_session *s) {
 
 int64_t ovf_session_prefix_bytes(const ovf_session *s) {
     if (!s) return -1;
+    if (s->kv_dtype == OVF_KV_Q4) return 0;  // no snapshots
     const ovf_model_config &c = s->m->cfg;
     return (int64_t)c.n_layers * c.n_kv_heads * s->pos * c.head_dim * (int64_t)kv_elem_bytes(s);
 }
@@ -1874,8 +2042,8 @@ int64_t ovf_session_prefix_bytes(const ovf_session *s) {
 // ThrowIfQuantized does.
 ovf_status ovf_session_save_prefix(const ovf_session *s, void *keys, void *values, int32_t *length_out) {
     OVF_CHECK_ARG(s && keys && values && length_out, "SavePrefix: null argument");
-    if (s->kv_dtype == OVF_KV_Q8) {
-        set_error("Snapshot is not supported for a quantized (Q8) KV cache");
+    if (s->kv_dtype == OVF_KV_Q8 || s->kv_dtype == OVF_KV_Q4) {
+        set_error("Snapshot is not supported for a quantized (%s) KV cache", s->kv_dtype == OVF_KV_Q8 ? "Q8" : "Q4");
         return OVF_EUNSUPPORTED;
     }
     DeviceGuard guard(s->m->device);
@@ -1897,8 +2065,8 @@ ovf_status ovf_session_save_prefix(const ovf_session *s, void *keys, void *value
 // holds no logits until the next prefill / decode.
 ovf_status ovf_session_restore_prefix(ovf_session *s, const void *keys, const void *values, int32_t length) {
     OVF_CHECK_ARG(s && (length == 0 || (keys && values)), "RestorePrefix: null argument");
-    if (s->kv_dtype == OVF_KV_Q8) {
-        set_error("RestoreFrom is not supported for a quantized (Q8) KV cache");
+    if (s->kv_dtype == OVF_KV_Q8 || s->kv_dtype == OVF_KV_Q4) {
+        set_error("RestoreFrom is not supported for a quantized (%s) KV cache", s->kv_dtype == OVF_KV_Q8 ? "Q8" : "Q4");
         return OVF_EUNSUPPORTED;
     }
     OVF_CHECK_ARG(length >= 0 && length <= s->max_ctx, "Snapshot length %d exceeds cache MaxLength %d", length,

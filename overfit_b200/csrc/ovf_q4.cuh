@@ -88,9 +88,9 @@ struct Q4Seq {
 };
 
 // Where the sequences of a launch are: `seqs` (device memory) for sessions, or
-// caches one behind the other.  positions[s] is what sequence s holds before
-// its rows, counts[s] (or all `rows`) how many of its rows are real; a
-// negative position marks an unused place.
+// caches one behind the other.  positions[s] (pos0 where there are none) is what
+// sequence s holds before its rows, counts[s] (or all `rows`) how many of its
+// rows are real; a negative position marks an unused place.
 struct Q4Source {
     const Q4Seq *seqs;
     int layer;
@@ -98,7 +98,7 @@ struct Q4Source {
     int64_t seq_bytes;
     const int32_t *positions, *counts;
     const float *cos, *sin;  // [max_ctx][hd / 2] or null
-    int split_half, max_ctx, rows, n_seq, KVH;
+    int split_half, max_ctx, rows, n_seq, KVH, pos0;
 };
 
 struct Q4View {
@@ -124,7 +124,7 @@ __device__ __forceinline__ bool q4_view(const Q4Source &p, int s, Q4View *w) {
         w->v = p.v + p.seq_bytes * s;
         w->cos = p.cos;
         w->sin = p.sin;
-        w->pos = p.positions[s];
+        w->pos = p.positions ? p.positions[s] : p.pos0;
     }
     w->tiles = q4_tiles(max_ctx);
     w->count = p.counts ? min(max(p.counts[s], 0), p.rows) : p.rows;
@@ -148,5 +148,9 @@ ovf_status launch_kv_q4_read(const Q4Source &src, int hd, float *k, float *v, cu
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx);
 ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
                                void *scratch, cudaStream_t st, bool pdl);
+// Rows of one sequence at pos0 .., as many at a time as `scratch` was sized for
+// (attn_q4_scratch_bytes of scratch_rows rows): the same results, bit for bit.
+ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
+                                    void *scratch, int scratch_rows, cudaStream_t st);
 
 }  // namespace ovf

@@ -29,13 +29,6 @@
 
 namespace ovf {
 
-struct VerifyParams {
-    const float *logits, *probs, *uniforms, *temperatures;
-    const int32_t *drafts, *counts;
-    int32_t *accepted, *token;
-    int max_drafts, vocab;
-};
-
 static constexpr int kVfThreads = 512, kVfWarps = kVfThreads / 32;
 static constexpr int kVfRows = 1024;        // max_drafts + 1
 static constexpr int kVfCluster = 16;       // at most

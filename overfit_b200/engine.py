@@ -177,7 +177,8 @@ class CudaLlamaInferenceEngine:
     def create_session(self, max_context: int, kv_cache_dtype: str = "f32") -> "CudaLlamaSession":
         """CreateSession(maxContextLength, kvCacheDType): "f32" (the reference's
         default, bit-exact attention), "q8" (the reference's Q8 cache, its
-        exact ComputeSingleHeadQ8 order) or "f16" (no reference counterpart)."""
+        exact ComputeSingleHeadQ8 order), "f16" or "q4" (5 bits per element,
+        ``kernels.KvCacheQ4``); the last two have no reference counterpart."""
         return CudaLlamaSession(self, max_context, kv_cache_dtype)
 
     def decode_batch(self, sessions, tokens, want_logits: bool = True) -> np.ndarray:
@@ -216,7 +217,7 @@ class CudaLlamaSession:
     """ISlmSession over the device-resident decode loop (greedy sampling on
     the device; logits are copied out only when asked for)."""
 
-    KV_DTYPES = {"f32": 0, "q8": 1, "f16": 2}
+    KV_DTYPES = {"f32": 0, "q8": 1, "f16": 2, "q4": 3}
 
     def __init__(self, engine: CudaLlamaInferenceEngine, max_context: int, kv_cache_dtype: str = "f32"):
         self.engine = engine
@@ -306,6 +307,52 @@ class CudaLlamaSession:
                                              am.ctypes.data), "Verify")
         self._have_logits = False
         return (am, lg) if want_logits else am
+
+    def verify_sampled(self, tokens, uniforms, temperature: float, draft_probs=None):
+        """The verify forward with sampled acceptance: tokens[0] is committed, the
+        others are drafts (drawn from the rows of `draft_probs`, or certain).
+        Keeps the accepted drafts' rows and returns (how many were accepted, the
+        token drawn behind them, which is not decoded yet).  `uniforms`: one
+        number in [0, 1) per token."""
+        toks = np.ascontiguousarray(np.asarray(tokens, dtype=np.int32))
+        u = np.ascontiguousarray(np.asarray(uniforms, dtype=np.float32))
+        n = toks.size
+        if u.size != n:
+            raise ValueError("one uniform per token")
+        q = None
+        if draft_probs is not None:
+            q = np.ascontiguousarray(np.asarray(draft_probs, dtype=np.float32))
+            if q.shape != (n - 1, self.engine.cfg["vocab"]):
+                raise ValueError("draft_probs must be [tokens - 1, vocab]")
+        a, t = C.c_int32(), C.c_int32()
+        check(_lib.load().ovf_session_verify_sampled(self._h, toks.ctypes.data, n, None if q is None else q.ctypes.data,
+                                                     u.ctypes.data, float(temperature), C.byref(a), C.byref(t)),
+              "VerifySampled")
+        self._have_logits = False
+        return a.value, t.value
+
+    def generate_speculative_sampled(self, history, rng, temperature: float, max_draft: int = 4, ngram_min: int = 1,
+                                     ngram_max: int = 3) -> list:
+        """GenerateSpeculative for sampled generation: t0 drawn from the current
+        logits, prompt-lookup drafts behind history + [t0], one verify forward
+        that accepts them against the target's distribution, and the token drawn
+        behind them decoded, so that the session holds its logits.  Returns the
+        committed tokens (>= 1), distributed as single sampled steps would be.
+        `rng`: a numpy Generator."""
+        if max_draft <= 0:
+            raise ValueError("maxDraft must be positive")
+        if not temperature > 0:
+            raise ValueError("temperature must be positive (generate_speculative is the greedy form)")
+        z = self.get_last_logits().astype(np.float64) / temperature
+        cum = np.cumsum(np.exp(z - z.max()))
+        t0 = int(np.searchsorted(cum, rng.random() * cum[-1], side="right"))
+        draft = prompt_lookup_draft(list(history) + [t0], max_draft, ngram_min, ngram_max)
+        if not draft or self.current_position + 1 + len(draft) + 1 > self.max_context_length:
+            self.decode(t0)
+            return [t0]
+        accepted, following = self.verify_sampled([t0] + draft, rng.random(1 + len(draft), dtype=np.float32), temperature)
+        self.decode(following)
+        return [t0] + draft[:accepted] + [following]
 
     def rollback_to(self, length: int) -> None:
         """CachedLlamaSession.RollbackTo (:318) -> KeyValueCache.TruncateTo."""
