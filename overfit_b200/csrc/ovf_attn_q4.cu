@@ -25,6 +25,7 @@
 // the call, bit for bit.  CTAs stay resident and take equal runs of the chunks
 // of all sequences, so that unequal lengths cost nothing; a warp's keys of the
 // next chunk load while it weights values, and the values while it scores.
+#include "ovf_attn_q4_rows.cu"
 #include "ovf_q4.cuh"
 
 namespace ovf {
@@ -58,16 +59,8 @@ struct AqParams {
     float *out, *part, *part_ml;  // partial results [row][chunk][hd] and (maximum, sum)
     float scale2;                 // scale * log2(e): exponentials are powers of two
     int max_chunks;
+    int splits;                   // partial results of each row (0: its chunks)
 };
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -83,28 +76,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-// Pair i (codes i and i + 4) of a word as two fp16 numbers 1 + c / 16.
-template <int I>
-__device__ __forceinline__ __half2 q4_pair(uint32_t w) {
-    const uint32_t s = I == 0 ? w << 4 : I == 1 ? w : I == 2 ? w >> 4 : __funnelshift_r(w, w, 8);
-    uint32_t r;
-    asm("lop3.b32 %0, %1, 0x03C003C0, 0x3C003C00, 0xEA;" : "=r"(r) : "r"(s));  // (s & mask) | ones
-    return bits_h2(r);
-}
-
 // hi and lo part of x, as a pair.
 __device__ __forceinline__ uint32_t split1(float x) {
     const __half h = __float2half_rn(x);
     return h2_bits(__halves2half2(h, __float2half_rn(x - __half2float(h))));
-}
-
-// The values of eight codes that share D and M (keys) or have a pair each (values).
-__device__ __forceinline__ void q4_values(uint32_t w, __half2 d0, __half2 m0, __half2 d1, __half2 m1, __half2 d2, __half2 m2,
-                                          __half2 d3, __half2 m3, uint32_t (&v)[4]) {
-    v[0] = h2_bits(__hfma2(d0, q4_pair<0>(w), m0));
-    v[1] = h2_bits(__hfma2(d1, q4_pair<1>(w), m1));
-    v[2] = h2_bits(__hfma2(d2, q4_pair<2>(w), m2));
-    v[3] = h2_bits(__hfma2(d3, q4_pair<3>(w), m3));
 }
 
 // The sequences' chunks as one list: per sequence [kv head][KR query rows][chunk].
@@ -530,7 +505,7 @@ __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const
     const int h = blockIdx.x, r = blockIdx.y, s = blockIdx.z, c0 = threadIdx.x / TC, d = threadIdx.x % TC;
     Q4View w;
     if (!q4_view(p.src, s, &w) || r >= w.count) return;
-    const int chunks = (w.pos + r) / kAqChunk + 1;
+    const int chunks = p.splits ? p.splits : (w.pos + r) / kAqChunk + 1;
     if (chunks == 1) return;
     const size_t row = ((size_t)s * p.src.rows + r) * p.H + h;
     const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
@@ -544,6 +519,7 @@ __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const
 #pragma unroll 4
     for (int c = c0; c < chunks; c += C) {
         const float2 x = ml[c];
+        if (x.x == -INFINITY) continue;  // (a split without an attended position)
         const float4 u = part[(size_t)c * TC];
         const float k = ex2(x.x - top);
         l += x.y * k;
@@ -567,6 +543,15 @@ static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqChunk - 1) / kAqChu
 
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx) {
     return 256 + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
+}
+
+// Scratch of launch_attention_q4_rows for up to `rows` rows, `few` at a time where they are few.
+int64_t attn_q4_rows_scratch_bytes(int rows, int few, int H, int KVH, int hd, int max_ctx, int sms) {
+    int64_t most = attn_q4_scratch_bytes(1, std::min(rows, few), H, hd, max_ctx);
+    for (int r = OVF_Q4_EXACT_ROWS + 1; r <= rows; ++r)
+        if (attn_q4_many_rows(r, hd))
+            most = std::max(most, 256 + (int64_t)4 * r * H * attn_q4_rows_splits(1, r, H, KVH, max_ctx, sms) * (hd + 2));
+    return most;
 }
 
 template <int NG, int NT>
@@ -601,6 +586,19 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
     p.part = static_cast<float *>(scratch);
     p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.max_chunks * hd;
     cudaError_t e = cudaSuccess;
+    if (attn_q4_many_rows(src.rows, hd)) {
+        p.splits = attn_q4_rows_splits(src.n_seq, src.rows, H, src.KVH, src.max_ctx, sm_count(current_device()));
+        p.max_chunks = p.splits;
+        p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.splits * hd;
+        const ArParams a{src, H, q, out, p.part, p.part_ml, p.scale2, p.splits};
+        e = hd == 32 ? launch_ar<1>(a, st) : hd == 64 ? launch_ar<2>(a, st) : launch_ar<4>(a, st);
+        if (e != cudaSuccess || p.splits == 1) return cuda_status(e, "attention_q4");
+        const dim3 grid(H, src.rows, src.n_seq);
+        e = hd == 32   ? launch_pdl(attention_q4_join_kernel<32>, grid, dim3(kAqJoinThreads), 0, st, false, p)
+            : hd == 64 ? launch_pdl(attention_q4_join_kernel<64>, grid, dim3(kAqJoinThreads), 0, st, false, p)
+                       : launch_pdl(attention_q4_join_kernel<128>, grid, dim3(kAqJoinThreads), 0, st, false, p);
+        return cuda_status(e, "attention_q4");
+    }
     // two operands share the cache's where there are rows for them (and registers)
     const bool two = (int64_t)src.rows * (H / src.KVH) > 4 && hd < 256;
 #define OVF_CALL(NG) e = two ? launch_aq<NG, NG < 8 ? 2 : 1>(p, st, pdl) : launch_aq<NG, 1>(p, st, pdl)
@@ -611,6 +609,7 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
 
 ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
                                     void *scratch, int scratch_rows, cudaStream_t st) {
+    if (attn_q4_many_rows(src.rows, hd)) return launch_attention_q4(src, H, hd, q, out, scale, scratch, st, false);
     for (int r = 0; r < src.rows; r += scratch_rows) {
         Q4Source part = src;
         part.pos0 = src.pos0 + r;

@@ -265,7 +265,7 @@ Q4Source q4_of(const ovf_session *s, int layer, int rows, int pos0, const int *p
     q.KVH = s->m->kvh_loc;
     return q;
 }
-constexpr int kQ4ScratchRows = 16;  // rows at a time of a 4-bit session's batches: bounds the scratch of a long context
+constexpr int kQ4ScratchRows = 16;  // rows at a time of a 4-bit session's small batches: bounds the scratch of a long context
 
 // Uploads an f32 vector (norm / bias).
 ovf_status upload_vec(ovf_model *m, const ovf_tensor &t, int64_t n, float **out, const char *what) {
@@ -932,7 +932,8 @@ ovf_status prefill_alloc(ovf_session *s) {
     A((void **)&s->pscale, 16);
     if (!st && c.n_experts > 0) st = moe_rows_alloc(c, kPrefillRows, s->allocs, &s->pmoe);
     if (s->kv_dtype == OVF_KV_Q4)
-        A(&s->q4_rows_scratch, (size_t)attn_q4_scratch_bytes(1, kQ4ScratchRows, s->m->h_loc, c.head_dim, s->max_ctx));
+        A(&s->q4_rows_scratch, (size_t)attn_q4_rows_scratch_bytes(kPrefillRows, kQ4ScratchRows, s->m->h_loc, s->m->kvh_loc,
+                                                                  c.head_dim, s->max_ctx, sm_count(s->m->device)));
     const int64_t pfl = attn_rows_scratch_floats(kPrefillRows, s->m->h_loc, s->max_ctx);
     if (!st && s->kv_dtype != OVF_KV_Q4 && attn_rows_supported(c.head_dim, s->kv_dtype) && pfl * 4 <= ((int64_t)512 << 20))
         A((void **)&s->pattn, (size_t)pfl * 4);

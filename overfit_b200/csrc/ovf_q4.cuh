@@ -79,6 +79,33 @@ __device__ __forceinline__ uint32_t q4_encode(float x, const Q4Params &p) {
     return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+
+// Pair i (codes i and i + 4) of a word as two fp16 numbers 1 + c / 16.
+template <int I>
+__device__ __forceinline__ __half2 q4_pair(uint32_t w) {
+    const uint32_t s = I == 0 ? w << 4 : I == 1 ? w : I == 2 ? w >> 4 : __funnelshift_r(w, w, 8);
+    uint32_t r;
+    asm("lop3.b32 %0, %1, 0x03C003C0, 0x3C003C00, 0xEA;" : "=r"(r) : "r"(s));  // (s & mask) | ones
+    return bits_h2(r);
+}
+
+// The values of eight codes that share D and M (keys) or have a pair each (values).
+__device__ __forceinline__ void q4_values(uint32_t w, __half2 d0, __half2 m0, __half2 d1, __half2 m1, __half2 d2, __half2 m2,
+                                          __half2 d3, __half2 m3, uint32_t (&v)[4]) {
+    v[0] = h2_bits(__hfma2(d0, q4_pair<0>(w), m0));
+    v[1] = h2_bits(__hfma2(d1, q4_pair<1>(w), m1));
+    v[2] = h2_bits(__hfma2(d2, q4_pair<2>(w), m2));
+    v[3] = h2_bits(__hfma2(d3, q4_pair<3>(w), m3));
+}
+
 // The cache of one sequence, for a batch of sessions whose caches are apart.
 struct Q4Seq {
     uint8_t *k, *v;       // layer 0
@@ -148,8 +175,10 @@ ovf_status launch_kv_q4_read(const Q4Source &src, int hd, float *k, float *v, cu
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx);
 ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
                                void *scratch, cudaStream_t st, bool pdl);
-// Rows of one sequence at pos0 .., as many at a time as `scratch` was sized for
-// (attn_q4_scratch_bytes of scratch_rows rows): the same results, bit for bit.
+// Rows of one sequence at pos0 ..; up to OVF_Q4_EXACT_ROWS of them `scratch_rows`
+// at a time (the same results, bit for bit), so that a long context's scratch
+// (attn_q4_rows_scratch_bytes) stays small.
+int64_t attn_q4_rows_scratch_bytes(int rows, int few, int H, int KVH, int hd, int max_ctx, int sms);
 ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
                                     void *scratch, int scratch_rows, cudaStream_t st);
 

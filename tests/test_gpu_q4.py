@@ -268,6 +268,24 @@ def test_queries_of_any_size(K, factor):
         np.testing.assert_allclose(got[0], want, rtol=0, atol=2.0 ** -10 * np.abs(b.kv[0][1]).max())
 
 
+@pytest.mark.parametrize("rows", [3, 80])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(4, 2, 128), (2, 2, 64), (3, 1, 32), (1, 1, 256)])
+def test_maxima_that_keep_rising(K, rows, heads, kv_heads, hd):
+    """Keys that grow along the sequence, so that every tile passes the maximum of the last by far, and then shrink."""
+    b = Batch(K, 1, heads, kv_heads, hd, 1200, [1], seed=rows + hd)
+    n = 1100
+    b.k = b.rng.normal(0, 1, (1, n, kv_heads, hd)).astype(np.float32)
+    b.k *= (0.05 + 3.0 * np.minimum(np.arange(n), 900) / 900).astype(np.float32)[None, :, None, None]
+    b.k[:, 1000:] *= 0.1
+    b.v = b.rng.normal(0, 1, (1, n, kv_heads, hd)).astype(np.float32)
+    K.KvCacheQ4.append(dev(b.k.reshape(1, n, -1)), dev(b.v.reshape(1, n, -1)), b.kc, b.vc, dev([0], torch.int32), kv_heads, hd,
+                       1200, b.dcos, b.dsin)
+    b.kv = [(ref.stored(ref.rotate(b.k[0], b.cos[:n], b.sin[:n], False)), ref.stored(b.v[0]))]
+    q = b.query(rows) * np.float32(6)
+    for pos in (n - rows, 700 - rows, 129):
+        b.check(b.run(q, [pos]), q, [pos])
+
+
 @pytest.mark.parametrize("heads,kv_heads,hd", [(8, 2, 128), (7, 1, 64)])
 def test_a_row_does_not_depend_on_its_company(K, heads, kv_heads, hd):
     """A decode step, the same row in a batch of sequences, and in a verify batch: the same bits."""
