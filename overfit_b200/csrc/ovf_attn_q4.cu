@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
         if (tiles > 0) {
             // scores of row 4 nt + t at positions first + 32 tile + 8 (e / 2) + 4 (e % 2) + i
             float s[NT][2][4];
-            if (!dead && !mbar_wait_sleep_bounded(&bars[0], phase)) dead = true;
+            if (!dead && !mbar_wait_bounded(&bars[0], phase)) dead = true;
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
                 if (tile < tiles) {
@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
 
             // (the maxima stand: every read of the keys is behind this warp)
             if (more) request(next, false);
-            if (!dead && !mbar_wait_sleep_bounded(&bars[1], phase)) dead = true;
+            if (!dead && !mbar_wait_bounded(&bars[1], phase)) dead = true;
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
                 if (tile >= tiles) break;

@@ -21,8 +21,8 @@
 // Warps, linked by mbarriers (each wait is bounded; a role that gives up goes on
 // without waiting, so that every barrier is met and TMEM is freed):
 //   0-7    softmax: a thread per row and half of a tile's columns;
-//   8-15   expansion of K and V, two stages each;
-//   16     TMEM allocation, and the thread that issues the MMAs: S of the next
+//   8-11   expansion of K and V, two stages each;
+//   12     TMEM allocation, and the thread that issues the MMAs: S of the next
 //          tile before O of this one.
 // Per tile the tensor cores need 1024 clocks (two products each way), shared
 // memory about 1500 (K and V are read twice, written once), the schedulers about
@@ -34,7 +34,9 @@ namespace ovf {
 
 static constexpr int kArM = 128;        // query rows of a CTA
 static constexpr int kArN = 128;        // positions of a tile
-static constexpr int kArThreads = 17 * 32;
+static constexpr int kArExpand = 4;      // expanding warps
+static constexpr int kArMma = 8 + kArExpand;
+static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
 static constexpr float kArLift = 6.0f;  // weights times 2^6
 static constexpr float kArSlack = 8.0f; // the maximum is raised when it is passed by 2^8
@@ -65,24 +67,48 @@ struct ArParams {
 };
 
 // D[tmem] (+)= A[tmem] B[shared memory]: kind::f16, fp16 operands, fp32 accumulator, M = 128.
-__device__ __forceinline__ void ar_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+template <bool Accumulate>
+__device__ __forceinline__ void ar_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "r"(a), "l"(b), "r"(idesc), "n"(Accumulate ? 1 : 0)
         : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ constexpr uint32_t ar_idesc(int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kArM >> 4) << 24);
 }
 __device__ __forceinline__ void ar_pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); }
 
+// Two fp32 operations in one instruction (each rounded as the single ones are).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n"
+        " mov.b64 {%0, %1}, z;\n}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 // Two fp32 numbers as pairs of hi and of lo parts.
 __device__ __forceinline__ void ar_split(float x, float y, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
+    const float2 f = __half22float2(h), r = fma2(f, make_float2(-1.0f, -1.0f), make_float2(x, y));
     hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+    lo = h2_bits(__floats2half2_rn(r.x, r.y));
 }
 
 template <int NG>
@@ -114,9 +140,9 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     float *xch = reinterpret_cast<float *>(sm + SM::x_off);  // [parity][half][row]
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 8);
+            mbar_init(&k_full[i], kArExpand);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 8);
+            mbar_init(&v_full[i], kArExpand);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 8);
@@ -124,7 +150,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
         mbar_init(o_done, 1);
         fence_mbar_init();
     }
-    if (warp == 16) {
+    if (warp == kArMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -200,7 +226,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     tc_fence_after();
 
     bool ok = true;
-    auto wait = [&](uint64_t *bar, int parity) { ok = ok && mbar_wait_sleep_bounded(bar, (uint32_t)parity); };
+    auto wait = [&](uint64_t *bar, int parity) { ok = ok && mbar_wait_bounded(bar, (uint32_t)parity); };
     if (warp < 8) {
         // ------------------------------------------------------- softmax
         float m = -INFINITY, l = 0.0f;
@@ -251,20 +277,22 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                 }
             }
             const float base = (m == -INFINITY ? 0.0f : m) - kArLift;
-            float sum = 0.0f;
+            float2 sum = make_float2(0.0f, 0.0f);
+            const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
 #pragma unroll
             for (int c = 0; c < 64; c += 32) {
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float a = ex2(fmaf(x[c + 2 * j], factor, -base)), b = ex2(fmaf(x[c + 2 * j + 1], factor, -base));
-                    sum += a + b;
-                    ar_split(a, b, hi[j], lo[j]);
+                    float2 w = fma2(make_float2(x[c + 2 * j], x[c + 2 * j + 1]), factor2, base2);
+                    w = make_float2(ex2(w.x), ex2(w.y));
+                    sum = add2(sum, w);
+                    ar_split(w.x, w.y, hi[j], lo[j]);
                 }
                 tmem_st16(s_at + c / 2, reinterpret_cast<const float *>(hi));
                 tmem_st16(s_at + 32 + c / 2, reinterpret_cast<const float *>(lo));
             }
-            l += sum;
+            l += sum.x + sum.y;
             tmem_st_wait();
             // O of the last tile is done by now; a phase that nobody waited for could not be told from the next but one
             if (i > 0) wait(o_done, (i - 1) & 1);
@@ -297,13 +325,13 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                         make_float4(o[j] * inv, o[j + 1] * inv, o[j + 2] * inv, o[j + 3] * inv);
             }
         }
-    } else if (warp < 16) {
+    } else if (warp < kArMma) {
         // ----------------------------------------------------- expansion
         const int me = warp - 8, t = lane >> 3, e = lane & 7;
         const int data_end = w.pos + w.count;
-        // K: a unit is 8 positions (a lane a position and the words t of its groups), two units a warp;
+        // K: a unit is 8 positions (a lane a position and the words t of its groups), four units a warp;
         // V: a unit is a group of 32 dimensions of a cache tile (a lane 8 positions of the dimensions 8 n + e)
-        constexpr int KU = 2, VU = NG >= 2 ? NG / 2 : 1;  // units a warp and tile
+        constexpr int KU = kArN / 8 / kArExpand, VU = 4 * NG / kArExpand;  // units a warp and tile
         struct Codes {
             uint32_t w[NG], dm[NG];
         } kc[KU];
@@ -339,7 +367,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             for (int u = 0; u < VU; ++u) {
                 const int unit = me * VU + u, j = unit / NG, g = unit % NG, pos = (t0 + i) * kArN + j * kQ4Tile;
                 vc[u].w = vc[u].d = vc[u].m = make_uint4(0, 0, 0, 0);
-                if (unit < 4 * NG && pos < data_end) {
+                if (pos < data_end) {
                     const uint8_t *tile = w.v + ((size_t)h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
                     vc[u].w = *reinterpret_cast<const uint4 *>(tile + ((g * 8 + e) * 4 + t) * 16);
                     vc[u].d = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + g * 128 + t * 16);
@@ -383,7 +411,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
 #pragma unroll
             for (int u = 0; u < VU; ++u) {
                 const int unit = me * VU + u, j = unit / NG, g = unit % NG;
-                if (unit < 4 * NG) {
+                {
                     const uint32_t words[4] = {vc[u].w.x, vc[u].w.y, vc[u].w.z, vc[u].w.w};
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {  // dimensions 32 g + 8 n + e
@@ -399,21 +427,28 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[st]);
         }
-    } else if (lane == 0) {
+    } else {
         // ---------------------------------------------------------- MMA
+        // (the warp goes through the loop together; one elected lane issues)
+        const uint32_t base = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        const uint32_t kb = smem_u32(sm + SM::k_off), vb = smem_u32(sm + SM::v_off);
         auto scores = [&](int i) {
             const int st = i & 1;
             wait(&k_full[st], (i >> 1) & 1);
             tc_fence_after();
-            const uint32_t kb = smem_u32(sm + SM::k_off + st * SM::kTile), d = tmem + SM::s_col + st * kArN;
+            if (elect_one()) {
+                const uint64_t b = umma_desc(kb + st * SM::kTile, 128, HD / 8 * 128);
+                const uint32_t d = base + SM::s_col + st * kArN;
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const uint64_t b = umma_desc(kb + k * 256, 128, HD / 8 * 128);
-                ar_mma(d, tmem + SM::q_col + 8 * k, b, ar_idesc(kArN), k > 0);
-                ar_mma(d, tmem + SM::q_col + HD / 2 + 8 * k, b, ar_idesc(kArN), 1);
+                for (int k = 0; k < HD / 16; ++k) {  // (a step of 16: 256 bytes, 16 in the descriptor's units)
+                    if (k == 0) ar_mma<false>(d, base + SM::q_col, b, ar_idesc(kArN));
+                    else ar_mma<true>(d, base + SM::q_col + 8 * k, b + 16 * k, ar_idesc(kArN));
+                    ar_mma<true>(d, base + SM::q_col + HD / 2 + 8 * k, b + 16 * k, ar_idesc(kArN));
+                }
+                tc_commit(&k_empty[st]);
+                tc_commit(&s_full[st]);
             }
-            tc_commit(&k_empty[st]);
-            tc_commit(&s_full[st]);
+            __syncwarp();
         };
         scores(0);
         for (int i = 0; i < nt; ++i) {
@@ -423,22 +458,28 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             wait(&v_full[st], (i >> 1) & 1);
             wait(&p_full[st], (i >> 1) & 1);
             tc_fence_after();
-            const uint32_t vb = smem_u32(sm + SM::v_off + st * SM::kTile), pa = tmem + SM::s_col + st * kArN;
+            if (elect_one()) {
+                const uint64_t b = umma_desc(vb + st * SM::kTile, 128, kArN / 8 * 128);
+                const uint32_t pa = base + SM::s_col + st * kArN, d = base + SM::o_col;
+                if (i == 0) ar_mma<false>(d, pa, b, ar_idesc(HD));
+                else ar_mma<true>(d, pa, b, ar_idesc(HD));
+                ar_mma<true>(d, pa + 32, b, ar_idesc(HD));
 #pragma unroll
-            for (int k = 0; k < kArN / 16; ++k) {
-                const uint64_t b = umma_desc(vb + k * 256, 128, kArN / 8 * 128);
-                const uint32_t a = pa + (k >> 2) * 64 + (k & 3) * 8;
-                ar_mma(tmem + SM::o_col, a, b, ar_idesc(HD), i > 0 || k > 0);
-                ar_mma(tmem + SM::o_col, a + 32, b, ar_idesc(HD), 1);
+                for (int k = 1; k < kArN / 16; ++k) {
+                    const uint32_t at = pa + (k >> 2) * 64 + (k & 3) * 8;
+                    ar_mma<true>(d, at, b + 16 * k, ar_idesc(HD));
+                    ar_mma<true>(d, at + 32, b + 16 * k, ar_idesc(HD));
+                }
+                tc_commit(&v_empty[st]);
+                tc_commit(o_done);
             }
-            tc_commit(&v_empty[st]);
-            tc_commit(o_done);
+            __syncwarp();
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == kArMma) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
