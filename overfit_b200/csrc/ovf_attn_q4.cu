@@ -491,22 +491,108 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
     }
 }
 
-// The chunks of a row to its output: weights 2^(m_c - max), sums over the
-// chunks c, c + C, .. by C groups of threads, then over the groups in order.
+// The chunks of a row to its output: weights 2^(m_c - max), sums over the chunks
+// c, c + 8, .. of eight classes in ascending order, then over the classes in
+// order.  Both kernels below form exactly these sums.
+static constexpr int kAqClasses = 8;
 static constexpr int kAqJoinThreads = 256;
+static constexpr int kAqJoinFew = 48;  // chunks up to which a thread takes all classes
 
+// The row of a (row, head) of the call, its number of partial results; false if there is nothing to join.
+__device__ __forceinline__ bool aq_join_of(const AqParams &p, int s, int r, int *chunks) {
+    Q4View w;
+    if (!q4_view(p.src, s, &w) || r >= w.count) return false;
+    *chunks = p.splits ? p.splits : (w.pos + r) / kAqChunk + 1;
+    return *chunks > 1;
+}
+
+// Few chunks: a lane for four dimensions of a row (two fours at head_dim 256); the lanes of a row form its weights
+// together.  (A CTA a row left the 8192 rows of a prefill chunk at 17 us, a thread that reads all maxima by itself a
+// decode step's 32 rows a microsecond longer.)
 template <int HD>
-__global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const AqParams p) {
-    constexpr int TC = HD / 4, C = kAqJoinThreads / TC;
-    __shared__ float4 sv[C][TC];
-    __shared__ float sl[C];
+__global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_few_kernel(const AqParams p) {
+    constexpr int TC = HD / 4, GL = TC < 32 ? TC : 32, E = (kAqJoinFew + GL - 1) / GL, F = TC / GL;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int64_t row = ((int64_t)blockIdx.x * kAqJoinThreads + threadIdx.x) / GL;
+    const int lane = threadIdx.x & 31, l0 = lane % GL, rows = p.src.rows;
+    int chunks = 0;
+    if (row < (int64_t)p.src.n_seq * rows * p.H) {
+        const int s = (int)(row / ((int64_t)rows * p.H)), r = (int)(row / p.H % rows);
+        if (!aq_join_of(p, s, r, &chunks)) chunks = 0;
+    }
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
+    const float4 *part = reinterpret_cast<const float4 *>(p.part) + row * p.max_chunks * TC + l0;
+    float2 y[E];
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        y[j] = j * GL + l0 < chunks ? ml[j * GL + l0] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, y[j].x);
+    }
+#pragma unroll
+    for (int o = GL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[j].x = y[j].x == -INFINITY ? 0.0f : ex2(y[j].x - top);  // (0: a split without an attended position)
+    float4 v[kAqClasses][F];
+    float l[kAqClasses];
+#pragma unroll
+    for (int k = 0; k < kAqClasses; ++k) {
+        l[k] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < F; ++f) v[k][f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    const int most = __reduce_max_sync(0xFFFFFFFFu, chunks);
+#pragma unroll
+    for (int c0 = 0; c0 < kAqJoinFew; c0 += kAqClasses) {
+        if (c0 >= most) break;
+        float4 u[kAqClasses][F];
+        float w[kAqClasses], n[kAqClasses];
+#pragma unroll
+        for (int k = 0; k < kAqClasses; ++k) {
+            const int from = lane - l0 + (c0 + k) % GL;
+            w[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].x, from);
+            n[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].y, from);
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                u[k][f] = c0 + k < chunks && !(w[k] == 0.0f) ? part[(size_t)(c0 + k) * TC + f * GL] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kAqClasses; ++k) {
+            l[k] += n[k] * w[k];
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                v[k][f].x += u[k][f].x * w[k], v[k][f].y += u[k][f].y * w[k];
+                v[k][f].z += u[k][f].z * w[k], v[k][f].w += u[k][f].w * w[k];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 1; k < kAqClasses; ++k) {
+        l[0] += l[k];
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+            v[0][f].x += v[k][f].x, v[0][f].y += v[k][f].y, v[0][f].z += v[k][f].z, v[0][f].w += v[k][f].w;
+    }
+    if (chunks == 0) return;
+    const float inv = 1.0f / l[0];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+        reinterpret_cast<float4 *>(p.out)[row * TC + f * GL + l0] =
+            make_float4(v[0][f].x * inv, v[0][f].y * inv, v[0][f].z * inv, v[0][f].w * inv);
+}
+
+// Many chunks: a CTA a row, a group of threads a class.
+template <int HD>
+__global__ void __launch_bounds__(HD / 4 * kAqClasses) attention_q4_join_kernel(const AqParams p) {
+    constexpr int TC = HD / 4;
+    __shared__ float4 sv[kAqClasses][TC];
+    __shared__ float sl[kAqClasses];
     pdl_wait();
     pdl_launch_dependents();
     const int h = blockIdx.x, r = blockIdx.y, s = blockIdx.z, c0 = threadIdx.x / TC, d = threadIdx.x % TC;
-    Q4View w;
-    if (!q4_view(p.src, s, &w) || r >= w.count) return;
-    const int chunks = p.splits ? p.splits : (w.pos + r) / kAqChunk + 1;
-    if (chunks == 1) return;
+    int chunks;
+    if (!aq_join_of(p, s, r, &chunks)) return;
     const size_t row = ((size_t)s * p.src.rows + r) * p.H + h;
     const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
     const float4 *part = reinterpret_cast<const float4 *>(p.part) + row * p.max_chunks * TC + d;
@@ -516,10 +602,9 @@ __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f;
-#pragma unroll 4
-    for (int c = c0; c < chunks; c += C) {
+#pragma unroll 8
+    for (int c = c0; c < chunks; c += kAqClasses) {
         const float2 x = ml[c];
-        if (x.x == -INFINITY) continue;  // (a split without an attended position)
         const float4 u = part[(size_t)c * TC];
         const float k = ex2(x.x - top);
         l += x.y * k;
@@ -529,7 +614,7 @@ __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const
     if (d == 0) sl[c0] = l;
     __syncthreads();
     if (c0 == 0) {
-        for (int i = 1; i < C; ++i) {
+        for (int i = 1; i < kAqClasses; ++i) {
             const float4 u = sv[i][d];
             v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
             l += sl[i];
@@ -537,6 +622,17 @@ __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_kernel(const
         const float inv = 1.0f / l;
         reinterpret_cast<float4 *>(p.out)[row * TC + d] = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     }
+}
+
+template <int HD>
+static cudaError_t launch_aq_join(const AqParams &p, cudaStream_t st) {
+    if (p.max_chunks <= kAqJoinFew) {
+        const int64_t threads = (int64_t)p.src.n_seq * p.src.rows * p.H * (HD < 128 ? HD / 4 : 32);
+        return launch_pdl(attention_q4_join_few_kernel<HD>, dim3((unsigned)((threads + kAqJoinThreads - 1) / kAqJoinThreads)),
+                          dim3(kAqJoinThreads), 0, st, true, p);
+    }
+    return launch_pdl(attention_q4_join_kernel<HD>, dim3(p.H, p.src.rows, p.src.n_seq), dim3(HD / 4 * kAqClasses), 0, st, true,
+                      p);
 }
 
 static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqChunk - 1) / kAqChunk; }
@@ -570,8 +666,7 @@ static cudaError_t launch_aq(const AqParams &p, cudaStream_t st, bool pdl) {
     const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(dev) * S::kCtas);
     cudaError_t e = launch_pdl(attention_q4_kernel<NG, NT>, dim3(grid), dim3(kAqThreads), S::kTotal, st, pdl, p);
     if (e != cudaSuccess || p.max_chunks == 1) return e;
-    return launch_pdl(attention_q4_join_kernel<NG * 32>, dim3(p.H, p.src.rows, p.src.n_seq), dim3(kAqJoinThreads), 0, st,
-                      true, p);
+    return launch_aq_join<NG * 32>(p, st);
 }
 
 ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
@@ -593,10 +688,7 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
         const ArParams a{src, H, q, out, p.part, p.part_ml, p.scale2, p.splits};
         e = hd == 32 ? launch_ar<1>(a, st) : hd == 64 ? launch_ar<2>(a, st) : launch_ar<4>(a, st);
         if (e != cudaSuccess || p.splits == 1) return cuda_status(e, "attention_q4");
-        const dim3 grid(H, src.rows, src.n_seq);
-        e = hd == 32   ? launch_pdl(attention_q4_join_kernel<32>, grid, dim3(kAqJoinThreads), 0, st, false, p)
-            : hd == 64 ? launch_pdl(attention_q4_join_kernel<64>, grid, dim3(kAqJoinThreads), 0, st, false, p)
-                       : launch_pdl(attention_q4_join_kernel<128>, grid, dim3(kAqJoinThreads), 0, st, false, p);
+        e = hd == 32 ? launch_aq_join<32>(p, st) : hd == 64 ? launch_aq_join<64>(p, st) : launch_aq_join<128>(p, st);
         return cuda_status(e, "attention_q4");
     }
     // two operands share the cache's where there are rows for them (and registers)

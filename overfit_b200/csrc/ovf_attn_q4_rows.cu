@@ -21,8 +21,8 @@
 // Warps, linked by mbarriers (each wait is bounded; a role that gives up goes on
 // without waiting, so that every barrier is met and TMEM is freed):
 //   0-7    softmax: a thread per row and half of a tile's columns;
-//   8-11   expansion of K and V, two stages each;
-//   12     TMEM allocation, and the thread that issues the MMAs: S of the next
+//   8-15   expansion of K and V, two stages each;
+//   16     TMEM allocation, and the thread that issues the MMAs: S of the next
 //          tile before O of this one.
 // Per tile the tensor cores need 1024 clocks (two products each way), shared
 // memory about 1500 (K and V are read twice, written once), the schedulers about
@@ -34,7 +34,7 @@ namespace ovf {
 
 static constexpr int kArM = 128;        // query rows of a CTA
 static constexpr int kArN = 128;        // positions of a tile
-static constexpr int kArExpand = 4;      // expanding warps
+static constexpr int kArExpand = 8;      // expanding warps
 static constexpr int kArMma = 8 + kArExpand;
 static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
@@ -156,22 +156,52 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     }
 
     // The queries, rotated (Rope/RopeKernel.cs:46-93, each step rounded by itself) and times the scale, to shared memory.
+    // (A warp takes four rows at a time, so that their loads are under way together.)
     float *qs = reinterpret_cast<float *>(sm);
-    for (int x = threadIdx.x; x < kArM * (HD / 2); x += kArThreads) {
-        const int i = x / (HD / 2), j = x % (HD / 2), g = mt * kArM + i, r = g / G;
-        const int a = src.split_half ? j : 2 * j, b = src.split_half ? j + HD / 2 : 2 * j + 1;
-        float x0 = 0.0f, x1 = 0.0f;
-        if (r < w.count) {
-            const float *q = p.q + out_row(g) * HD;
-            x0 = q[a], x1 = q[b];
-            if (w.cos) {
-                const float c = w.cos[(size_t)(w.pos + r) * (HD / 2) + j], sn = w.sin[(size_t)(w.pos + r) * (HD / 2) + j];
-                const float y0 = fsub(fmul(x0, c), fmul(x1, sn)), y1 = fadd(fmul(x0, sn), fmul(x1, c));
-                x0 = y0, x1 = y1;
+    constexpr int PL = HD >= 64 ? HD / 64 : 1;  // pairs of a lane
+    for (int i0 = warp * 4; i0 < kArM; i0 += kArThreads / 32 * 4) {
+        float v0[4][PL], v1[4][PL], c[4][PL], sn[4][PL];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int g = mt * kArM + i0 + k, r = g / G;
+            const float *q = p.q + (((size_t)s * src.rows + r) * p.H + h * G + (g - r * G)) * HD;
+#pragma unroll
+            for (int b = 0; b < PL; ++b) {
+                const int j = lane + 32 * b;
+                v0[k][b] = v1[k][b] = c[k][b] = sn[k][b] = 0.0f;
+                if (r < w.count && j < HD / 2) {
+                    if (src.split_half) {
+                        v0[k][b] = q[j];
+                        v1[k][b] = q[j + HD / 2];
+                    } else {
+                        const float2 v = *reinterpret_cast<const float2 *>(q + 2 * j);
+                        v0[k][b] = v.x;
+                        v1[k][b] = v.y;
+                    }
+                    if (w.cos) {
+                        c[k][b] = w.cos[(size_t)(w.pos + r) * (HD / 2) + j];
+                        sn[k][b] = w.sin[(size_t)(w.pos + r) * (HD / 2) + j];
+                    }
+                }
             }
         }
-        qs[i * SM::q_pitch + a] = x0 * p.scale2;
-        qs[i * SM::q_pitch + b] = x1 * p.scale2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int b = 0; b < PL; ++b) {
+                const int j = lane + 32 * b;
+                if (j >= HD / 2) continue;
+                const float x0 = v0[k][b], x1 = v1[k][b], cc = c[k][b], ss = sn[k][b];
+                const float y0 = w.cos ? fsub(fmul(x0, cc), fmul(x1, ss)) : x0;
+                const float y1 = w.cos ? fadd(fmul(x0, ss), fmul(x1, cc)) : x1;
+                float *to = qs + (i0 + k) * SM::q_pitch;
+                if (src.split_half) {
+                    to[j] = y0 * p.scale2;
+                    to[j + HD / 2] = y1 * p.scale2;
+                } else {
+                    *reinterpret_cast<float2 *>(to + 2 * j) = make_float2(y0 * p.scale2, y1 * p.scale2);
+                }
+            }
     }
     tc_fence_before();
     __syncthreads();
@@ -235,18 +265,26 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             const int p0 = (t0 + i) * kArN + half * (kArN / 2);
             wait(&s_full[i & 1], (i >> 1) & 1);
             tc_fence_after();
-            float x[64];
+            // two passes over 32 columns at a time: the registers of 64 would not leave room for 17 warps
+            const bool masked = __any_sync(0xFFFFFFFFu, p0 + kArN / 2 - 1 > limit);
+            float x[32];
+            auto columns = [&](int c0) {
+                tmem_ld16_nowait(s_at + c0, reinterpret_cast<uint32_t *>(x));
+                tmem_ld16_nowait(s_at + c0 + 16, reinterpret_cast<uint32_t *>(x) + 16);
+                tmem_ld_wait();
+                if (masked) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld16_nowait(s_at + 16 * c, reinterpret_cast<uint32_t *>(x) + 16 * c);
-            tmem_ld_wait();
-            if (__any_sync(0xFFFFFFFFu, p0 + kArN / 2 - 1 > limit)) {
-#pragma unroll
-                for (int c = 0; c < 64; ++c)  // columns in the order 0 4 1 5 2 6 3 7 of positions
-                    if (p0 + (c & ~7) + ((c & 7) >> 1) + 4 * (c & 1) > limit) x[c] = -INFINITY;
-            }
+                    for (int c = 0; c < 32; ++c)  // columns in the order 0 4 1 5 2 6 3 7 of positions
+                        if (p0 + c0 + (c & ~7) + ((c & 7) >> 1) + 4 * (c & 1) > limit) x[c] = -INFINITY;
+                }
+            };
+            columns(32);
             float top = x[0];
 #pragma unroll
-            for (int c = 1; c < 64; ++c) top = fmaxf(top, x[c]);
+            for (int c = 1; c < 32; ++c) top = fmaxf(top, x[c]);
+            columns(0);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) top = fmaxf(top, x[c]);
             top *= factor;
             float *mine = xch + (i & 1) * 2 * kArM + half * kArM + row;
             *mine = top;
@@ -279,19 +317,22 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             const float base = (m == -INFINITY ? 0.0f : m) - kArLift;
             float2 sum = make_float2(0.0f, 0.0f);
             const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
-#pragma unroll
-            for (int c = 0; c < 64; c += 32) {
+            // (P of the first 32 columns goes where those scores were, hi parts before lo parts of each half)
+            auto weights = [&](int c0) {
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    float2 w = fma2(make_float2(x[c + 2 * j], x[c + 2 * j + 1]), factor2, base2);
+                    float2 w = fma2(make_float2(x[2 * j], x[2 * j + 1]), factor2, base2);
                     w = make_float2(ex2(w.x), ex2(w.y));
                     sum = add2(sum, w);
                     ar_split(w.x, w.y, hi[j], lo[j]);
                 }
-                tmem_st16(s_at + c / 2, reinterpret_cast<const float *>(hi));
-                tmem_st16(s_at + 32 + c / 2, reinterpret_cast<const float *>(lo));
-            }
+                tmem_st16(s_at + c0, reinterpret_cast<const float *>(hi));
+                tmem_st16(s_at + c0 + 16, reinterpret_cast<const float *>(lo));
+            };
+            weights(0);
+            columns(32);
+            weights(32);
             l += sum.x + sum.y;
             tmem_st_wait();
             // O of the last tile is done by now; a phase that nobody waited for could not be told from the next but one
@@ -329,9 +370,9 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
         // ----------------------------------------------------- expansion
         const int me = warp - 8, t = lane >> 3, e = lane & 7;
         const int data_end = w.pos + w.count;
-        // K: a unit is 8 positions (a lane a position and the words t of its groups), four units a warp;
+        // K: a unit is 8 positions (a lane a position and the words t of its groups), two units a warp;
         // V: a unit is a group of 32 dimensions of a cache tile (a lane 8 positions of the dimensions 8 n + e)
-        constexpr int KU = kArN / 8 / kArExpand, VU = 4 * NG / kArExpand;  // units a warp and tile
+        constexpr int KU = kArN / 8 / kArExpand, VU = 4 * NG > kArExpand ? 4 * NG / kArExpand : 1;  // units a warp and tile
         struct Codes {
             uint32_t w[NG], dm[NG];
         } kc[KU];
@@ -367,7 +408,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             for (int u = 0; u < VU; ++u) {
                 const int unit = me * VU + u, j = unit / NG, g = unit % NG, pos = (t0 + i) * kArN + j * kQ4Tile;
                 vc[u].w = vc[u].d = vc[u].m = make_uint4(0, 0, 0, 0);
-                if (pos < data_end) {
+                if (unit < 4 * NG && pos < data_end) {
                     const uint8_t *tile = w.v + ((size_t)h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
                     vc[u].w = *reinterpret_cast<const uint4 *>(tile + ((g * 8 + e) * 4 + t) * 16);
                     vc[u].d = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + g * 128 + t * 16);
@@ -411,7 +452,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
 #pragma unroll
             for (int u = 0; u < VU; ++u) {
                 const int unit = me * VU + u, j = unit / NG, g = unit % NG;
-                {
+                if (unit < 4 * NG) {
                     const uint32_t words[4] = {vc[u].w.x, vc[u].w.y, vc[u].w.z, vc[u].w.w};
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {  // dimensions 32 g + 8 n + e
@@ -463,12 +504,12 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                 const uint32_t pa = base + SM::s_col + st * kArN, d = base + SM::o_col;
                 if (i == 0) ar_mma<false>(d, pa, b, ar_idesc(HD));
                 else ar_mma<true>(d, pa, b, ar_idesc(HD));
-                ar_mma<true>(d, pa + 32, b, ar_idesc(HD));
+                ar_mma<true>(d, pa + 16, b, ar_idesc(HD));
 #pragma unroll
                 for (int k = 1; k < kArN / 16; ++k) {
-                    const uint32_t at = pa + (k >> 2) * 64 + (k & 3) * 8;
+                    const uint32_t at = pa + (k >> 1) * 32 + (k & 1) * 8;  // 32 positions: 16 columns of hi, 16 of lo parts
                     ar_mma<true>(d, at, b + 16 * k, ar_idesc(HD));
-                    ar_mma<true>(d, at + 32, b + 16 * k, ar_idesc(HD));
+                    ar_mma<true>(d, at + 16, b + 16 * k, ar_idesc(HD));
                 }
                 tc_commit(&v_empty[st]);
                 tc_commit(o_done);
