@@ -29,41 +29,47 @@ __device__ __forceinline__ float redux_max(float x) {
     return y;
 }
 
-// A key word: eight dimensions (32 g + 8 t ..) of one row and head.
-struct Q4KeyWord {
-    int r, h, g, t;
-};
-template <int NG>
-__device__ __forceinline__ Q4KeyWord q4_key_of(int i, int KVH) {
-    Q4KeyWord k;
-    k.t = i & 3;
-    k.g = (i >> 2) % NG;
-    const int v = i / (4 * NG);
-    k.h = v % KVH;
-    k.r = v / KVH;
-    return k;
+// Whether any of eight elements is NaN or beyond the limit, so that they need q4_clean.
+__device__ __forceinline__ bool q4_unclean(const float (&x)[8]) {
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bad |= !(fabsf(x[j]) <= kQ4Limit);
+    return bad;
 }
 
+// The word of eight codes, with the parameters of element j's group from params(j).  A number of 0..15 is rounded to
+// an integer (half to even) by adding 1.5 * 2^23, which leaves it in the low bits; what the addend leaves above is
+// taken off at the end.
+template <class P>
+__device__ __forceinline__ uint32_t q4_word(const float (&x)[8], P params) {
+    uint32_t word = 0, extra = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float3 p = params(j);  // M, D, 16 / D
+        const float c = fminf(fmaxf(fmul(fsub(fsub(x[j], p.x), p.y), p.z), 0.0f), 15.0f);
+        word += __float_as_uint(fadd(c, 12582912.0f)) << (4 * j);
+        extra += 0x4B400000u << (4 * j);
+    }
+    word -= extra;
+    return __funnelshift_l(word, word, 2);
+}
+
+// Keys: a thread takes one word (dimensions 32 g + 8 t ..) of one row of head h.
 template <int NG>
-__device__ __forceinline__ void append_key(const Q4Source &src, const float *k, const Q4View &w, int s) {
+__device__ __forceinline__ void append_key(const Q4Source &src, const float *k, const Q4View &w, int s, int h) {
     constexpr int HD = NG * 32;
-    const int i = blockIdx.x * kKvQ4Threads + threadIdx.x;
-    const Q4KeyWord a = q4_key_of<NG>(i, src.KVH);
-    const bool real = a.r < w.count;
+    const int i = blockIdx.x * kKvQ4Threads + threadIdx.x, r = i / (4 * NG), d = i % (4 * NG) * 8, g = d / 32, t = d / 8 % 4;
+    const bool real = r < w.count;
     if (!__any_sync(0xFFFFFFFFu, real)) return;
-    const int pos = w.pos + (real ? a.r : 0);
-    float x[8];
+    const int pos = w.pos + (real ? r : 0);
+    float x[8] = {};
     if (real) {
-        const float4 *p = reinterpret_cast<const float4 *>(k + ((size_t)s * src.rows * src.KVH * NG * 4 + i) * 8);
+        const float4 *p = reinterpret_cast<const float4 *>(k + (((size_t)s * src.rows + r) * src.KVH + h) * HD + d);
         const float4 u = p[0], v = p[1];
         x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.0f;
     }
     if (w.cos) {
         const float *c = w.cos + (size_t)pos * (HD / 2), *sn = w.sin + (size_t)pos * (HD / 2);
-        const int d = a.g * 32 + a.t * 8;
         if (!src.split_half) {
             const float4 cc = *reinterpret_cast<const float4 *>(c + d / 2), ss = *reinterpret_cast<const float4 *>(sn + d / 2);
             const float cv[4] = {cc.x, cc.y, cc.z, cc.w}, sv[4] = {ss.x, ss.y, ss.z, ss.w};
@@ -75,146 +81,174 @@ __device__ __forceinline__ void append_key(const Q4Source &src, const float *k, 
             }
         } else {
             const int at = d % (HD / 2);
+            float cv[8], sv[8];
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                *reinterpret_cast<float4 *>(cv + j) = *reinterpret_cast<const float4 *>(c + at + j);
+                *reinterpret_cast<float4 *>(sv + j) = *reinterpret_cast<const float4 *>(sn + at + j);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float other = __shfl_xor_sync(0xFFFFFFFFu, x[j], NG * 2);  // half a head further
-                const float cc = c[at + j], ss = sn[at + j];
-                x[j] = d < HD / 2 ? fsub(fmul(x[j], cc), fmul(other, ss)) : fadd(fmul(other, ss), fmul(x[j], cc));
+                x[j] = d < HD / 2 ? fsub(fmul(x[j], cv[j]), fmul(other, sv[j])) : fadd(fmul(other, sv[j]), fmul(x[j], cv[j]));
             }
         }
     }
-    float lo, hi;
+    if (q4_unclean(x)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = q4_clean(x[j]);
-        lo = j ? fminf(lo, x[j]) : x[j];
-        hi = j ? fmaxf(hi, x[j]) : x[j];
+        for (int j = 0; j < 8; ++j) x[j] = q4_clean(x[j]);
     }
+    float lo = x[0], hi = x[0];
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
+    for (int j = 1; j < 8; ++j) lo = fminf(lo, x[j]), hi = fmaxf(hi, x[j]);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {  // the lanes of a group
         lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     }
     const Q4Params q = q4_params(lo, hi);
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) word |= q4_encode(x[j], q) << (4 * j);
+    const uint32_t word = q4_word(x, [&](int) { return make_float3(q.m, q.d, q.inv); });
     if (!real) return;
-    uint8_t *tile = w.k + ((size_t)a.h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
-    reinterpret_cast<uint32_t *>(tile)[q4_key_word(NG, pos & 31, a.t, a.g)] = __funnelshift_l(word, word, 2);
-    if (a.t == 0)
-        *reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(tile + q4_code_bytes(HD)) +
-                                     q4_key_param(NG, pos & 31, a.g)) = __halves2half2(q.D, q.M);
+    uint8_t *tile = w.k + ((size_t)h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
+    reinterpret_cast<uint32_t *>(tile)[q4_key_word(NG, pos & 31, t, g)] = word;
+    if (t == 0)
+        *reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(tile + q4_code_bytes(HD)) + q4_key_param(NG, pos & 31, g)) =
+            __halves2half2(q.D, q.M);
 }
 
-// A group of a block of eight positions: rows r0 .. r0 + 7, of which [0, count) are real.
+// Values: a warp takes group g of the block b of eight positions of head h: rows r0 .. r0 + 7, of which [j0, j1) are real.
 struct Q4ValueBlock {
-    int b, h, g, r0;
+    int b, g, r0, j0, j1;
 };
 template <int NG>
-__device__ __forceinline__ bool q4_value_of(int i, const Q4View &w, int KVH, Q4ValueBlock *v) {
+__device__ __forceinline__ bool q4_value_of(const Q4View &w, Q4ValueBlock *v) {
+    const int i = blockIdx.x * (kKvQ4Threads / 32) + (threadIdx.x >> 5);
     v->g = i % NG;
-    v->h = i / NG % KVH;
-    v->b = (w.pos >> 3) + i / (NG * KVH);
+    v->b = (w.pos >> 3) + i / NG;
     v->r0 = v->b * 8 - w.pos;
+    v->j0 = max(0, -v->r0);
+    v->j1 = min(8, w.count - v->r0);
     return v->r0 < w.count;
 }
 
 template <int NG>
-__device__ __forceinline__ void append_value(const Q4Source &src, const float *v, const Q4View &w, int s) {
+__device__ __forceinline__ void append_value(const Q4Source &src, const float *v, const Q4View &w, int s, int h) {
     constexpr int HD = NG * 32;
+    __shared__ float4 params[kKvQ4Threads / 32][8];  // M, D, 16 / D of each position
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Q4ValueBlock a;
-    if (!q4_value_of<NG>(blockIdx.x * (kKvQ4Threads / 32) + warp, w, src.KVH, &a)) return;
-    const int j0 = max(0, -a.r0), j1 = min(8, w.count - a.r0), t = a.b & 3;
-    uint8_t *tile = w.v + ((size_t)a.h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
+    if (!q4_value_of<NG>(w, &a)) return;
+    const int t = a.b & 3;
+    const bool whole = a.j0 == 0 && a.j1 == 8;
+    uint8_t *tile = w.v + ((size_t)h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
     uint32_t *word = reinterpret_cast<uint32_t *>(tile) + q4_value_word(a.g, lane & 7, t, lane >> 3);
-    __half *params = reinterpret_cast<__half *>(tile + q4_code_bytes(HD));
-    const float *x0 = v + (((size_t)s * src.rows + a.r0) * src.KVH + a.h) * HD + a.g * 32 + lane;
-    float x[8], lo = 0.0f, hi = 0.0f;
+    const float *x0 = v + (((long long)s * src.rows + a.r0) * src.KVH + h) * HD + a.g * 32 + lane;
+    const size_t step = (size_t)src.KVH * HD;
+    float x[8];
+    if (whole) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j >= j0 && j < j1 ? x0[(long long)j * src.KVH * HD] : 0.0f;
+        for (int j = 0; j < 8; ++j) x[j] = x0[j * step];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = j >= a.j0 && j < a.j1 ? x0[j * step] : 0.0f;
+    }
     uint32_t old = 0;
-    if (j0 > 0 || j1 < 8) old = *word;
-    // lane j forms the parameters of position j
+    if (!whole) old = *word;
+    if (q4_unclean(x)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = q4_clean(x[j]);
+    }
+    __syncwarp();
+    float lo = 0.0f, hi = 0.0f;  // of position `lane`
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        x[j] = q4_clean(x[j]);
-        const float l = redux_min(x[j]), h = redux_max(x[j]);
-        if (lane == j) lo = l, hi = h;
+        const float l = redux_min(x[j]), m = redux_max(x[j]);
+        if (lane == j) lo = l, hi = m;
     }
-    const Q4Params q = q4_params(lo, hi);
-    if (lane >= j0 && lane < j1) {
-        const int at = q4_value_param(a.g, t, lane);
-        params[at] = q.D;
-        params[at + 32] = q.M;
+    if (lane < 8) {
+        const Q4Params q = q4_params(lo, hi);
+        params[warp][lane] = make_float4(q.m, q.d, q.inv, 0.0f);
+        if (lane >= a.j0 && lane < a.j1) {
+            __half *to = reinterpret_cast<__half *>(tile + q4_code_bytes(HD)) + q4_value_param(a.g, t, lane);
+            to[0] = q.D;
+            to[32] = q.M;
+        }
     }
-    uint32_t codes = __funnelshift_r(old, old, 2);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        Q4Params p;
-        p.m = __shfl_sync(0xFFFFFFFFu, q.m, j);
-        p.d = __shfl_sync(0xFFFFFFFFu, q.d, j);
-        p.inv = __shfl_sync(0xFFFFFFFFu, q.inv, j);
-        if (j >= j0 && j < j1) codes = (codes & ~(15u << (4 * j))) | q4_encode(x[j], p) << (4 * j);
+    __syncwarp();
+    uint32_t codes = q4_word(x, [&](int j) {
+        const float4 q = params[warp][j];
+        return make_float3(q.x, q.y, q.z);
+    });
+    if (!whole) {
+        // the codes of the block's other positions stay: nibbles j0 .. j1 - 1 are ours
+        uint32_t ours = (a.j1 == 8 ? 0xFFFFFFFFu : (1u << (4 * a.j1)) - 1u) & ~((1u << (4 * a.j0)) - 1u);
+        ours = __funnelshift_l(ours, ours, 2);
+        codes = (codes & ours) | (old & ~ours);
     }
-    *word = __funnelshift_l(codes, codes, 2);
+    *word = codes;
 }
 
+// blockIdx.y: KV head and side
 template <int NG>
 __global__ void __launch_bounds__(kKvQ4Threads) kv_q4_append_kernel(const Q4Source src, const float *k, const float *v) {
     Q4View w;
     pdl_wait();
     pdl_launch_dependents();
     if (!q4_view(src, blockIdx.z, &w)) return;
-    if (blockIdx.y) append_value<NG>(src, v, w, blockIdx.z);
-    else append_key<NG>(src, k, w, blockIdx.z);
+    if (blockIdx.y & 1) append_value<NG>(src, v, w, blockIdx.z, blockIdx.y >> 1);
+    else append_key<NG>(src, k, w, blockIdx.z, blockIdx.y >> 1);
 }
 
 template <int NG>
 __global__ void __launch_bounds__(kKvQ4Threads) kv_q4_read_kernel(const Q4Source src, float *k, float *v) {
     constexpr int HD = NG * 32;
-    const int s = blockIdx.z;
+    const int s = blockIdx.z, h = blockIdx.y >> 1;
     Q4View w;
     if (!q4_view(src, s, &w)) return;
-    if (blockIdx.y == 0) {
-        const int i = blockIdx.x * kKvQ4Threads + threadIdx.x;
-        const Q4KeyWord a = q4_key_of<NG>(i, src.KVH);
-        if (a.r >= w.count) return;
-        const int p = (w.pos + a.r) & 31;
-        const uint8_t *tile = w.k + ((size_t)a.h * w.tiles + (w.pos + a.r) / kQ4Tile) * q4_tile_bytes(HD);
-        const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[q4_key_word(NG, p, a.t, a.g)];
+    uint32_t x[4];  // pairs (i, i + 4)
+    if (!(blockIdx.y & 1)) {
+        const int i = blockIdx.x * kKvQ4Threads + threadIdx.x, r = i / (4 * NG), d = i % (4 * NG) * 8;
+        if (r >= w.count) return;
+        const int p = (w.pos + r) & 31;
+        const uint8_t *tile = w.k + ((size_t)h * w.tiles + (w.pos + r) / kQ4Tile) * q4_tile_bytes(HD);
+        const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[q4_key_word(NG, p, d / 8 % 4, d / 32)];
         const __half2 dm = *reinterpret_cast<const __half2 *>(reinterpret_cast<const __half *>(tile + q4_code_bytes(HD)) +
-                                                              q4_key_param(NG, p, a.g));
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = q4_value(q4_code(word, j), __low2half(dm), __high2half(dm));
-        float4 *y = reinterpret_cast<float4 *>(k + ((size_t)s * src.rows * src.KVH * NG * 4 + i) * 8);
-        y[0] = make_float4(x[0], x[1], x[2], x[3]);
-        y[1] = make_float4(x[4], x[5], x[6], x[7]);
+                                                              q4_key_param(NG, p, d / 32));
+        const __half2 D = __low2half2(dm), M = __high2half2(dm);
+        q4_values(word, D, M, D, M, D, M, D, M, x);
+        const float2 a = __half22float2(bits_h2(x[0])), b = __half22float2(bits_h2(x[1])), c = __half22float2(bits_h2(x[2])),
+                     e = __half22float2(bits_h2(x[3]));
+        float4 *y = reinterpret_cast<float4 *>(k + (((size_t)s * src.rows + r) * src.KVH + h) * HD + d);
+        y[0] = make_float4(a.x, b.x, c.x, e.x);
+        y[1] = make_float4(a.y, b.y, c.y, e.y);
         return;
     }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
     Q4ValueBlock a;
-    if (!q4_value_of<NG>(blockIdx.x * (kKvQ4Threads / 32) + warp, w, src.KVH, &a)) return;
+    if (!q4_value_of<NG>(w, &a)) return;
     const int t = a.b & 3;
-    const uint8_t *tile = w.v + ((size_t)a.h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
+    const uint8_t *tile = w.v + ((size_t)h * w.tiles + a.b / 4) * q4_tile_bytes(HD);
     const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[q4_value_word(a.g, lane & 7, t, lane >> 3)];
-    const __half *params = reinterpret_cast<const __half *>(tile + q4_code_bytes(HD));
-    float *y = v + (((size_t)s * src.rows + a.r0) * src.KVH + a.h) * HD + a.g * 32 + lane;
+    const uint4 d = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + a.g * 128 + t * 16);
+    const uint4 m = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + a.g * 128 + 64 + t * 16);
+    q4_values(word, bits_h2(d.x), bits_h2(m.x), bits_h2(d.y), bits_h2(m.y), bits_h2(d.z), bits_h2(m.z), bits_h2(d.w),
+              bits_h2(m.w), x);
+    float *y = v + (((long long)s * src.rows + a.r0) * src.KVH + h) * HD + a.g * 32 + lane;
+    const size_t step = (size_t)src.KVH * HD;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int at = q4_value_param(a.g, t, j);
-        if (a.r0 + j >= 0 && a.r0 + j < w.count) y[(long long)j * src.KVH * HD] = q4_value(q4_code(word, j), params[at], params[at + 32]);
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = __half22float2(bits_h2(x[j]));
+        if (j >= a.j0 && j < a.j1) y[j * step] = f.x;
+        if (j + 4 >= a.j0 && j + 4 < a.j1) y[(j + 4) * step] = f.y;
     }
 }
 
 bool q4_supported(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
 static dim3 kv_q4_grid(const Q4Source &src, int hd) {
-    const int64_t keys = (int64_t)src.rows * src.KVH * (hd / 8);  // words
-    const int64_t values = (int64_t)((src.rows + 14) / 8) * src.KVH * (hd / 32) * 32;  // rows may start anywhere in a block
-    return dim3((unsigned)((std::max(keys, values) + kKvQ4Threads - 1) / kKvQ4Threads), 2, src.n_seq);
+    const int64_t keys = (int64_t)src.rows * (hd / 8);                       // words of a head
+    const int64_t values = (int64_t)((src.rows + 14) / 8) * (hd / 32) * 32;  // rows may start anywhere in a block
+    return dim3((unsigned)((std::max(keys, values) + kKvQ4Threads - 1) / kKvQ4Threads), src.KVH * 2, src.n_seq);
 }
 
 #define OVF_Q4_HD(hd, CALL)              \

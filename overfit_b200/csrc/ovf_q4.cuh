@@ -47,17 +47,10 @@ __device__ __forceinline__ int q4_value_word(int g, int e, int t, int n) { retur
 // Half index of a value's D at position 8 t + i; M is 32 halves further.
 __device__ __forceinline__ int q4_value_param(int g, int t, int i) { return g * 64 + t * 8 + 2 * (i & 3) + (i >> 2); }
 
-__device__ __forceinline__ int q4_shift(int i) { return (4 * i + 2) & 31; }
-__device__ __forceinline__ uint32_t q4_code(uint32_t word, int i) {
-    return __funnelshift_r(word, word, q4_shift(i)) & 15u;
-}
-__device__ __forceinline__ float q4_value(uint32_t c, __half D, __half M) {
-    return __half2float(__hfma(D, __ushort_as_half((unsigned short)(0x3C00u | (c << 6))), M));
-}
-
-// The code of x in a group of smallest and largest element lo and hi, and the
-// group's D and M.  Each step is rounded by itself (no contraction), so the
-// codes are the same wherever the definition is computed in fp32.
+// D and M of a group of smallest and largest element lo and hi.  Each step is
+// rounded by itself (no contraction), so that they, and the codes
+// clamp(rint(((x - M) - D) * inv), 0, 15), are the same wherever the definition
+// is computed in fp32.
 struct Q4Params {
     __half D, M;
     float d, m, inv;
@@ -74,11 +67,6 @@ __device__ __forceinline__ Q4Params q4_params(float lo, float hi) {
     p.inv = p.d > 0.0f ? fdiv(16.0f, p.d) : 0.0f;
     return p;
 }
-__device__ __forceinline__ uint32_t q4_encode(float x, const Q4Params &p) {
-    const float c = rintf(fmul(fsub(fsub(x, p.m), p.d), p.inv));
-    return (uint32_t)fminf(fmaxf(c, 0.0f), 15.0f);
-}
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
