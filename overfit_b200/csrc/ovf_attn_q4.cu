@@ -17,14 +17,16 @@
 // times hi and lo, a decode step of 4 heads a KV head left half of it empty: 1037
 // instructions a tile of 32 positions and warp, now about half.)
 //
-// Work is cut into chunks of 256 positions, 64 (two tiles) a warp: scores, their
-// maximum, weights, weighted values, with no rescaling.  A CTA's four warps'
-// results (maximum, sum, weighted values) are joined in shared memory, and a
-// second kernel joins the chunks of a row.  Chunks, tiles and the order of every
-// sum go by position alone, so a row's result does not depend on what else is in
-// the call, bit for bit.  CTAs stay resident and take equal runs of the chunks
-// of all sequences, so that unequal lengths cost nothing; a warp's keys of the
-// next chunk load while it weights values, and the values while it scores.
+// Work is cut into chunks of 256 positions (512 in caches of more than 4096,
+// where joining less outweighs a shorter chunk's latency).  A CTA's four warps
+// take 64 (two tiles) of each 256 at a time: scores, their maximum, weights,
+// weighted values; a second 256 rescales once.  The four results (maximum, sum,
+// weighted values) are joined in shared memory, and a second kernel joins the
+// chunks of a row.  Chunks, tiles and the order of every sum go by position (and
+// the cache's capacity) alone, so a row's result does not depend on what else is
+// in the call, bit for bit.  CTAs stay resident and take equal runs of the chunks
+// of all sequences, so that unequal lengths cost nothing; a warp's next keys load
+// while it weights values, and its next values while it scores.
 #include "ovf_attn_q4_rows.cu"
 #include "ovf_q4.cuh"
 
@@ -32,9 +34,10 @@ namespace ovf {
 
 static constexpr int kAqWarps = 4;
 static constexpr int kAqThreads = kAqWarps * 32;
-static constexpr int kAqChunk = 256;               // positions of a chunk: kAqWarps warps x 2 tiles
+static constexpr int kAqLeaf = 256;                // positions that the warps take at a time, two tiles each
+static constexpr int kAqWideTiles = 128;           // caches of more tiles have chunks of two leaves
 static constexpr float kAqLift = 14.0f;            // weights are held times 2^14: lo parts stay normal fp16 numbers
-static_assert(kAqChunk == kAqWarps * 2 * kQ4Tile, "two tiles a warp");
+static_assert(kAqLeaf == kAqWarps * 2 * kQ4Tile, "two tiles a warp");
 
 // A call's shape in the template: NG groups of 32 dimensions, NT operands of 4
 // query rows that share the cache's operand.
@@ -49,7 +52,7 @@ struct AqShape {
     static constexpr int kRing = kAqWarps * 2 * kSide;
     static constexpr int kMerge = kAqWarps * kRows * kPad * 4;
     static constexpr int kTotal = kRing + kMerge + kAqWarps * kRows * 8 + kAqWarps * 2 * 8;
-    static constexpr int kCtas = NG == 8 ? 2 : NT == 2 ? 3 : 4;  // per SM
+    static constexpr int kCtas = NG == 8 ? 2 : NT == 2 ? (NG == 4 ? 2 : 3) : 4;  // per SM (registers)
 };
 
 struct AqParams {
@@ -64,7 +67,7 @@ struct AqParams {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -82,23 +85,36 @@ __device__ __forceinline__ uint32_t split1(float x) {
     return h2_bits(__halves2half2(h, __float2half_rn(x - __half2float(h))));
 }
 
-// The sequences' chunks as one list: per sequence [kv head][KR query rows][chunk].
+// Positions of a chunk of a sequence.
+__device__ __forceinline__ int aq_span(const Q4View &w) { return w.tiles > kAqWideTiles ? 2 * kAqLeaf : kAqLeaf; }
+
+// The sequences' chunks as one list: per sequence [kv head][KR query rows][chunk].  An item of it:
 struct AqItem {
-    Q4View w;
-    int s, left;               // items of this sequence behind this one
-    int chunks, groups, chunk, mt, h;  // chunks and groups of KR rows of the sequence; this item's
+    const uint8_t *k, *v;  // caches of its head
+    const float *cos, *sin;
+    int64_t head;          // bytes from one head to the next
+    int s, pos, count;
+    int left;              // items of this sequence behind this one
+    int span, chunks, groups, chunk, mt, h;
+    int last;              // last position that any of its rows attends
 };
 
 template <int KR>
 __device__ __forceinline__ int aq_count(const Q4Source &src, int s, int G) {
     Q4View w;
     if (s >= src.n_seq || !q4_view(src, s, &w)) return 0;
-    return src.KVH * ((w.count * G + KR - 1) / KR) * ((w.pos + w.count + kAqChunk - 1) / kAqChunk);
+    const int span = aq_span(w);
+    return src.KVH * ((w.count * G + KR - 1) / KR) * ((w.pos + w.count + span - 1) / span);
+}
+
+template <int KR>
+__device__ __forceinline__ void aq_last(AqItem *it, int G) {
+    it->last = it->pos + min(it->count - 1, (it->mt * KR + KR - 1) / G);
 }
 
 // Item `target` of the list that starts with sequence `from`; false if it has fewer.
 template <int KR>
-__device__ __forceinline__ bool aq_locate(const Q4Source &src, int G, int from, long long target, AqItem *it) {
+__device__ __forceinline__ bool aq_locate(const Q4Source &src, int G, int tile_bytes, int from, long long target, AqItem *it) {
     const int lane = threadIdx.x & 31;
     for (int s0 = from; s0 < src.n_seq; s0 += 32) {
         const int n = aq_count<KR>(src, s0 + lane, G);
@@ -116,44 +132,61 @@ __device__ __forceinline__ bool aq_locate(const Q4Source &src, int G, int from, 
         const int l = __ffs(there) - 1;
         const int local = (int)(target - __shfl_sync(0xFFFFFFFFu, sum - n, l));
         const int items = __shfl_sync(0xFFFFFFFFu, n, l);
+        Q4View w;
         it->s = s0 + l;
-        q4_view(src, it->s, &it->w);
-        it->chunks = (it->w.pos + it->w.count + kAqChunk - 1) / kAqChunk;
-        it->groups = (it->w.count * G + KR - 1) / KR;
+        q4_view(src, it->s, &w);
+        it->pos = w.pos;
+        it->count = w.count;
+        it->cos = w.cos;
+        it->sin = w.sin;
+        it->head = (int64_t)w.tiles * tile_bytes;
+        it->span = aq_span(w);
+        it->chunks = (w.pos + w.count + it->span - 1) / it->span;
+        it->groups = (w.count * G + KR - 1) / KR;
         it->left = items - 1 - local;
         it->chunk = local % it->chunks;
         it->mt = local / it->chunks % it->groups;
         it->h = local / it->chunks / it->groups;
+        it->k = w.k + it->head * it->h;
+        it->v = w.v + it->head * it->h;
+        aq_last<KR>(it, G);
         return true;
     }
     return false;
 }
 
 template <int KR>
-__device__ __forceinline__ bool aq_next(const Q4Source &src, int G, AqItem *it) {
-    if (it->left == 0) return aq_locate<KR>(src, G, it->s + 1, 0, it);
+__device__ __forceinline__ void aq_next(const Q4Source &src, int G, int tile_bytes, AqItem *it) {
+    if (it->left == 0) {
+        aq_locate<KR>(src, G, tile_bytes, it->s + 1, 0, it);
+        return;
+    }
     --it->left;
     if (++it->chunk == it->chunks) {
         it->chunk = 0;
         if (++it->mt == it->groups) {
             it->mt = 0;
             ++it->h;
+            it->k += it->head;
+            it->v += it->head;
         }
+        aq_last<KR>(it, G);
     }
-    return true;
 }
 
-// Positions of the item that any of its rows attends: [256 chunk, end).
-template <int KR>
-__device__ __forceinline__ int aq_end(const AqItem &it, int G) {
-    const int last_row = min(it.w.count - 1, (it.mt * KR + KR - 1) / G);
-    return min((it.chunk + 1) * kAqChunk, it.w.pos + last_row + 1);
+// A warp's part of leaf `leaf` of an item: its first position, and its tiles that hold attended ones.
+__device__ __forceinline__ int aq_first(const AqItem &it, int leaf, int warp) {
+    return it.chunk * it.span + leaf * kAqLeaf + warp * 2 * kQ4Tile;
+}
+__device__ __forceinline__ int aq_tiles(const AqItem &it, int first) {
+    return min(2, (it.last - first + kQ4Tile) >> 5);  // (0 or less: none)
 }
 
 template <int NG, int NT>
 __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_q4_kernel(const AqParams p) {
     using S = AqShape<NG, NT>;
     constexpr int HD = NG * 32, KR = S::kRows, TB = S::kTile, MD = S::MD, PAD = S::kPad;
+    constexpr int RL = MD / 4, NP = KR * RL / kAqThreads > 0 ? KR * RL / kAqThreads : 1;  // the join: lanes a row, rows a thread
     extern __shared__ __align__(128) uint8_t smem[];
     const Q4Source &src = p.src;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = lane >> 2, t = lane & 3, G = p.H / src.KVH;
@@ -178,25 +211,25 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
     const long long lo = total * blockIdx.x / gridDim.x;
     int left = (int)(total * (blockIdx.x + 1) / gridDim.x - lo);
     AqItem it, next;
-    if (left <= 0 || !aq_locate<KR>(src, G, 0, lo, &it)) return;
+    if (left <= 0 || !aq_locate<KR>(src, G, TB, 0, lo, &it)) return;
 
-    // One side of this warp's part of an item: its tiles that hold attended positions, or none (false).
+    // Requests one side of this warp's part of a leaf, if it has one.
     const uint64_t policy = l2_evict_first_policy();
-    auto request = [&](const AqItem &i, bool side) {
-        const int p0 = i.chunk * kAqChunk + warp * 2 * kQ4Tile, tiles = min(2, (aq_end<KR>(i, G) - p0 + kQ4Tile - 1) / kQ4Tile);
-        if (tiles <= 0) return;
-        if (lane == 0) {
-            const size_t at = ((size_t)i.h * i.w.tiles + p0 / kQ4Tile) * TB;
+    auto request = [&](const AqItem &i, int leaf, bool side) {
+        const int first = aq_first(i, leaf, warp), tiles = aq_tiles(i, first);
+        if (tiles > 0 && lane == 0) {
             mbar_arrive_expect_tx(&bars[side], tiles * TB);
-            bulk_g2s(side ? values : keys, (side ? i.w.v : i.w.k) + at, tiles * TB, &bars[side], policy);
+            bulk_g2s(side ? values : keys, (side ? i.v : i.k) + (size_t)(first / kQ4Tile) * TB, tiles * TB, &bars[side], policy);
         }
     };
-    request(it, false);
-    request(it, true);
+    request(it, 0, false);
+    request(it, 0, true);
 
     uint32_t q[NT][NG][4];  // query operand: pairs (0, 4) (1, 5) (2, 6) (3, 7) of this lane's dimensions
     float factor[NT];       // a score from its sum of products, of row 4 nt + t
     int limit[NT];          // last position that the row attends
+    int row_last[NP];       // the join's rows of this thread: last position (-1: none),
+    int64_t row_out[NP];    // place among the call's (row, head)s
     int have_h = -1, have_mt = -1, have_s = -1, phase = 0;
     bool dead = false;
 
@@ -207,7 +240,7 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
             for (int nt = 0; nt < NT; ++nt) {
                 // column e of the operand: row e / 2, its hi (even) or lo part
                 const int i = it.mt * KR + nt * 4 + (e >> 1), r = i / G;
-                const bool real = r < it.w.count;
+                const bool real = r < it.count;
                 float x[NG][8];
                 if (real) {
                     const float4 *src4 = reinterpret_cast<const float4 *>(
@@ -224,9 +257,9 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[g][k] = 0.0f;
                 }
-                if (it.w.cos) {  // Rope/RopeKernel.cs:46-93, each step rounded by itself
-                    const int pos = real ? it.w.pos + r : 0;
-                    const float *c = it.w.cos + (size_t)pos * (HD / 2), *sn = it.w.sin + (size_t)pos * (HD / 2);
+                if (it.cos) {  // Rope/RopeKernel.cs:46-93, each step rounded by itself
+                    const int pos = real ? it.pos + r : 0;
+                    const float *c = it.cos + (size_t)pos * (HD / 2), *sn = it.sin + (size_t)pos * (HD / 2);
                     if (!src.split_half) {
 #pragma unroll
                         for (int g = 0; g < NG; ++g)
@@ -278,15 +311,20 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
                 // of row 4 nt + t, whose operand the lanes of column 2 t formed
                 factor[nt] = p.scale2 * __int_as_float((__shfl_sync(0xFFFFFFFFu, ex, 8 * t) - 14) << 23);
                 const int row = (it.mt * KR + nt * 4 + t) / G;
-                limit[nt] = row < it.w.count ? it.w.pos + row : 0x7FFFFFFF;  // (a row that is none: zeros, which nothing reads)
+                limit[nt] = row < it.count ? it.pos + row : 0x7FFFFFFF;  // (a row that is none: zeros, which nothing reads)
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int i = it.mt * KR + (threadIdx.x + n * kAqThreads) / RL, r = i / G;
+                row_last[n] = r < it.count ? it.pos + r : -1;
+                row_out[n] = ((int64_t)it.s * src.rows + r) * p.H + it.h * G + (i - r * G);
             }
         }
         const bool more = left > 1;
         next = it;
-        if (more) aq_next<KR>(src, G, &next);
+        if (more) aq_next<KR>(src, G, TB, &next);
 
-        const int first = it.chunk * kAqChunk + warp * 2 * kQ4Tile, end = aq_end<KR>(it, G), data_end = it.w.pos + it.w.count;
-        const int tiles = min(2, (end - first + kQ4Tile - 1) / kQ4Tile);
+        const int leaves = it.span / kAqLeaf, data_end = it.pos + it.count;
         float m[NT], l[NT], o[NT][NG * 2][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -296,7 +334,19 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[nt][d][k] = 0.0f;
         }
-        if (tiles > 0) {
+        for (int leaf = 0; leaf < leaves; ++leaf) {
+            const int first = aq_first(it, leaf, warp), tiles = aq_tiles(it, first);
+            // the leaf behind this one
+            const bool same = leaf + 1 < leaves;
+            auto request_next = [&](bool side) {
+                if (same) request(it, leaf + 1, side);
+                else if (more) request(next, 0, side);
+            };
+            if (tiles <= 0) {
+                request_next(false);
+                request_next(true);
+                continue;
+            }
             // scores of row 4 nt + t at positions first + 32 tile + 8 (e / 2) + 4 (e % 2) + i
             float s[NT][2][4];
             if (!dead && !mbar_wait_bounded(&bars[0], phase)) dead = true;
@@ -363,15 +413,23 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
                         for (int i = 0; i < 4; ++i)
                             if (at + tile * kQ4Tile + i > limit[nt]) s[nt][tile][i] = -INFINITY;
                 }
-                float top = -INFINITY;
+                float top = m[nt];
 #pragma unroll
                 for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[nt][tile][i]);
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+                const float zero = top == -INFINITY ? 0.0f : top, base = zero - kAqLift;  // (nothing attended: weights of 0)
+                if (leaf > 0) {
+                    const float keep = ex2(m[nt] - zero);
+                    l[nt] *= keep;
+#pragma unroll
+                    for (int d = 0; d < NG * 2; ++d)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[nt][d][k] *= keep;
+                }
                 m[nt] = top;
-                const float base = (top == -INFINITY ? 0.0f : top) - kAqLift;  // (nothing attended: weights of 0)
 #pragma unroll
                 for (int tile = 0; tile < 2; ++tile)
 #pragma unroll
@@ -383,7 +441,7 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
             }
 
             // (the maxima stand: every read of the keys is behind this warp)
-            if (more) request(next, false);
+            request_next(false);
             if (!dead && !mbar_wait_bounded(&bars[1], phase)) dead = true;
 #pragma unroll
             for (int tile = 0; tile < 2; ++tile) {
@@ -424,9 +482,9 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
                     }
                 }
             }
+            // (the last product has been issued, so its operands have arrived: every read of the values is behind this warp)
+            request_next(true);
             phase ^= 1;
-        } else if (more) {
-            request(next, false);
         }
 
         // the four warps' results to one
@@ -456,13 +514,11 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
                     to[0] = (c[0] + c[1]) * share[nt];
                     to[8] = (c[2] + c[3]) * share[nt];
                 }
-            // (the last sums are written: every read of the values is behind this warp)
-            if (more && d0 + MD == HD) request(next, true);
             __syncthreads();
-            for (int x = threadIdx.x; x < KR * MD / 4; x += kAqThreads) {
-                const int row = x / (MD / 4), d = x % (MD / 4) * 4, i = it.mt * KR + row, r = i / G;
-                const int row_last = it.w.pos + r;
-                if (r >= it.w.count || row_last < it.chunk * kAqChunk) continue;  // no row, or one that ends before
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int row = (threadIdx.x + n * kAqThreads) / RL, d = threadIdx.x % RL * 4;
+                if (row >= KR || row_last[n] < it.chunk * it.span) continue;  // no row, or one that ends before
                 float mm = -INFINITY, sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < kAqWarps; ++w) mm = fmaxf(mm, merge_ml[w * KR + row].x);
@@ -474,13 +530,12 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
                     const float4 u = *reinterpret_cast<const float4 *>(&merge[(w * KR + row) * PAD + d]);
                     v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
                 }
-                const size_t orow = ((size_t)it.s * src.rows + r) * p.H + it.h * G + i % G;
-                if (row_last < kAqChunk) {  // the row's only chunk
+                if (row_last[n] < it.span) {  // the row's only chunk
                     const float inv = 1.0f / sum;
-                    *reinterpret_cast<float4 *>(p.out + orow * HD + d0 + d) =
+                    *reinterpret_cast<float4 *>(p.out + row_out[n] * HD + d0 + d) =
                         make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                 } else {
-                    const size_t pc = orow * p.max_chunks + it.chunk;
+                    const int64_t pc = row_out[n] * p.max_chunks + it.chunk;
                     *reinterpret_cast<float4 *>(p.part + pc * HD + d0 + d) = v;
                     if (d0 == 0 && d == 0) *reinterpret_cast<float2 *>(p.part_ml + pc * 2) = make_float2(mm, sum);
                 }
@@ -502,7 +557,7 @@ static constexpr int kAqJoinFew = 48;  // chunks up to which a thread takes all 
 __device__ __forceinline__ bool aq_join_of(const AqParams &p, int s, int r, int *chunks) {
     Q4View w;
     if (!q4_view(p.src, s, &w) || r >= w.count) return false;
-    *chunks = p.splits ? p.splits : (w.pos + r) / kAqChunk + 1;
+    *chunks = p.splits ? p.splits : (w.pos + r) / aq_span(w) + 1;
     return *chunks > 1;
 }
 
@@ -635,7 +690,7 @@ static cudaError_t launch_aq_join(const AqParams &p, cudaStream_t st) {
                       p);
 }
 
-static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqChunk - 1) / kAqChunk; }
+static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqLeaf - 1) / kAqLeaf; }
 
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx) {
     return 256 + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
