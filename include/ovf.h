@@ -261,9 +261,11 @@ ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_
  * result on the cached values.  Up to OVF_Q4_EXACT_ROWS rows, a row's output
  * does not depend on the other rows and sequences of the call, bit for bit.
  * k_new / v_new (or NULL): rows that are appended first, as ovf_kv_q4_append
- * does.  scratch: ovf_attention_q4_scratch_bytes, 16-byte aligned, for one
- * call at a time (calls that may overlap, graphs included, need their own). */
+ * does.  scratch: ovf_attention_q4_scratch_bytes, 16-byte aligned, the first
+ * OVF_Q4_SCRATCH_ZEROS bytes zero (a call leaves them zero), for one call at a
+ * time (calls that may overlap, graphs included, need their own). */
 #define OVF_Q4_EXACT_ROWS 64
+#define OVF_Q4_SCRATCH_ZEROS 256
 int64_t ovf_attention_q4_scratch_bytes(int32_t n_seq, int32_t rows, int32_t n_heads, int32_t n_kv_heads,
                                        int32_t head_dim, int32_t max_ctx);
 ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_new, void *k_cache, void *v_cache,

@@ -35,6 +35,8 @@ namespace ovf {
 static constexpr int kAqWarps = 4;
 static constexpr int kAqThreads = kAqWarps * 32;
 static constexpr int kAqLeaf = 256;                // positions that the warps take at a time, two tiles each
+static constexpr int kAqCounters = 64;             // ints at the start of the scratch, zero between calls
+static_assert(4 * kAqCounters == OVF_Q4_SCRATCH_ZEROS, "what a call finds zero and leaves zero");
 static constexpr int kAqWideTiles = 128;           // caches of more tiles have chunks of two leaves
 static constexpr float kAqLift = 14.0f;            // weights are held times 2^14: lo parts stay normal fp16 numbers
 static_assert(kAqLeaf == kAqWarps * 2 * kQ4Tile, "two tiles a warp");
@@ -63,6 +65,8 @@ struct AqParams {
     float scale2;                 // scale * log2(e): exponentials are powers of two
     int max_chunks;
     int splits;                   // partial results of each row (0: its chunks)
+    int groups;                   // groups of rows that the counters have room for, per KV head
+    int *done;                    // chunks finished of each (sequence, KV head, group of rows)
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -174,6 +178,94 @@ __device__ __forceinline__ void aq_next(const Q4Source &src, int G, int tile_byt
     }
 }
 
+// The chunks of a row to its output: weights 2^(m_c - max), sums over the chunks
+// c, c + 8, .. of eight classes in ascending order, then over the classes in
+// order.  Every kernel that joins forms exactly these sums.
+static constexpr int kAqClasses = 8;
+static constexpr int kAqJoinThreads = 256;
+static constexpr int kAqJoinFew = 48;  // chunks up to which a thread takes all classes
+
+// The row of a (row, head) of the call, its number of partial results; false if there is nothing to join.
+__device__ __forceinline__ bool aq_join_of(const AqParams &p, int s, int r, int *chunks) {
+    Q4View w;
+    if (!q4_view(p.src, s, &w) || r >= w.count) return false;
+    *chunks = p.splits ? p.splits : (w.pos + r) / aq_span(w) + 1;
+    return *chunks > 1;
+}
+
+// A row by a group of GL lanes, a lane four dimensions (two fours at head_dim 256); the lanes form the weights
+// together.  (A CTA a row left the 8192 rows of a prefill chunk at 17 us, a thread that reads all maxima by itself a
+// decode step's 32 rows a microsecond longer.)  Groups without a row pass chunks = 0.
+template <int HD>
+struct AqJoin {
+    static constexpr int TC = HD / 4, GL = TC < 32 ? TC : 32, E = (kAqJoinFew + GL - 1) / GL, F = TC / GL;
+};
+template <int HD>
+__device__ __forceinline__ void aq_join_few(const AqParams &p, int64_t row, int chunks) {
+    constexpr int TC = AqJoin<HD>::TC, GL = AqJoin<HD>::GL, E = AqJoin<HD>::E, F = AqJoin<HD>::F;
+    const int lane = threadIdx.x & 31, l0 = lane % GL;
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
+    const float4 *part = reinterpret_cast<const float4 *>(p.part) + row * p.max_chunks * TC + l0;
+    float2 y[E];
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        y[j] = j * GL + l0 < chunks ? __ldcg(ml + j * GL + l0) : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, y[j].x);
+    }
+#pragma unroll
+    for (int o = GL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+#pragma unroll
+    for (int j = 0; j < E; ++j) y[j].x = y[j].x == -INFINITY ? 0.0f : ex2(y[j].x - top);  // (0: a split without an attended position)
+    float4 v[kAqClasses][F];
+    float l[kAqClasses];
+#pragma unroll
+    for (int k = 0; k < kAqClasses; ++k) {
+        l[k] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < F; ++f) v[k][f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    const int most = __reduce_max_sync(0xFFFFFFFFu, chunks);
+#pragma unroll
+    for (int c0 = 0; c0 < kAqJoinFew; c0 += kAqClasses) {
+        if (c0 >= most) break;
+        float4 u[kAqClasses][F];
+        float w[kAqClasses], n[kAqClasses];
+#pragma unroll
+        for (int k = 0; k < kAqClasses; ++k) {
+            const int from = lane - l0 + (c0 + k) % GL;
+            w[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].x, from);
+            n[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].y, from);
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                u[k][f] = c0 + k < chunks && !(w[k] == 0.0f) ? __ldcg(part + (size_t)(c0 + k) * TC + f * GL)
+                                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < kAqClasses; ++k) {
+            l[k] += n[k] * w[k];
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                v[k][f].x += u[k][f].x * w[k], v[k][f].y += u[k][f].y * w[k];
+                v[k][f].z += u[k][f].z * w[k], v[k][f].w += u[k][f].w * w[k];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 1; k < kAqClasses; ++k) {
+        l[0] += l[k];
+#pragma unroll
+        for (int f = 0; f < F; ++f)
+            v[0][f].x += v[k][f].x, v[0][f].y += v[k][f].y, v[0][f].z += v[k][f].z, v[0][f].w += v[k][f].w;
+    }
+    if (chunks == 0) return;
+    const float inv = 1.0f / l[0];
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+        reinterpret_cast<float4 *>(p.out)[row * TC + f * GL + l0] =
+            make_float4(v[0][f].x * inv, v[0][f].y * inv, v[0][f].z * inv, v[0][f].w * inv);
+}
+
 // A warp's part of leaf `leaf` of an item: its first position, and its tiles that hold attended ones.
 __device__ __forceinline__ int aq_first(const AqItem &it, int leaf, int warp) {
     return it.chunk * it.span + leaf * kAqLeaf + warp * 2 * kQ4Tile;
@@ -182,8 +274,8 @@ __device__ __forceinline__ int aq_tiles(const AqItem &it, int first) {
     return min(2, (it.last - first + kQ4Tile) >> 5);  // (0 or less: none)
 }
 
-template <int NG, int NT>
-__global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_q4_kernel(const AqParams p) {
+template <int NG, int NT, bool Fused>
+__global__ void __launch_bounds__(kAqThreads, Fused ? 2 : AqShape<NG, NT>::kCtas) attention_q4_kernel(const AqParams p) {
     using S = AqShape<NG, NT>;
     constexpr int HD = NG * 32, KR = S::kRows, TB = S::kTile, MD = S::MD, PAD = S::kPad;
     constexpr int RL = MD / 4, NP = KR * RL / kAqThreads > 0 ? KR * RL / kAqThreads : 1;  // the join: lanes a row, rows a thread
@@ -194,6 +286,7 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
     float *merge = reinterpret_cast<float *>(smem + S::kRing);                             // [warp][row][PAD]
     float2 *merge_ml = reinterpret_cast<float2 *>(merge + kAqWarps * KR * PAD);            // [warp][row]
     uint64_t *bars = reinterpret_cast<uint64_t *>(merge_ml + kAqWarps * KR) + warp * 2;    // keys, values
+    __shared__ int last_one;
     if (lane < 2) mbar_init(&bars[lane], 1);
     fence_mbar_init();
     __syncwarp();
@@ -542,99 +635,43 @@ __global__ void __launch_bounds__(kAqThreads, AqShape<NG, NT>::kCtas) attention_
             }
             __syncthreads();
         }
+        if (Fused && it.chunks > 1) {
+            // the CTA that finishes the last chunk of these rows joins them
+            __threadfence();
+            __syncthreads();
+            int *done = p.done + (it.s * src.KVH + it.h) * p.groups + it.mt;
+            if (threadIdx.x == 0) last_one = atomicAdd(done, 1) == it.chunks - 1;
+            __syncthreads();
+            if (last_one) {
+                if (threadIdx.x == 0) *done = 0;  // as it was found
+                __threadfence();
+                constexpr int GL = AqJoin<HD>::GL;
+#pragma unroll 1
+                for (int g = threadIdx.x / GL; g < (KR * GL + 31) / 32 * 32 / GL; g += kAqThreads / GL) {
+                    const int i = it.mt * KR + g, r = i / G;
+                    const int chunks = g < KR && r < it.count ? (it.pos + r) / it.span + 1 : 0;
+                    aq_join_few<HD>(p, ((int64_t)it.s * src.rows + r) * p.H + it.h * G + (i - r * G), chunks > 1 ? chunks : 0);
+                }
+            }
+        }
         it = next;
     }
 }
 
-// The chunks of a row to its output: weights 2^(m_c - max), sums over the chunks
-// c, c + 8, .. of eight classes in ascending order, then over the classes in
-// order.  Both kernels below form exactly these sums.
-static constexpr int kAqClasses = 8;
-static constexpr int kAqJoinThreads = 256;
-static constexpr int kAqJoinFew = 48;  // chunks up to which a thread takes all classes
-
-// The row of a (row, head) of the call, its number of partial results; false if there is nothing to join.
-__device__ __forceinline__ bool aq_join_of(const AqParams &p, int s, int r, int *chunks) {
-    Q4View w;
-    if (!q4_view(p.src, s, &w) || r >= w.count) return false;
-    *chunks = p.splits ? p.splits : (w.pos + r) / aq_span(w) + 1;
-    return *chunks > 1;
-}
-
-// Few chunks: a lane for four dimensions of a row (two fours at head_dim 256); the lanes of a row form its weights
-// together.  (A CTA a row left the 8192 rows of a prefill chunk at 17 us, a thread that reads all maxima by itself a
-// decode step's 32 rows a microsecond longer.)
+// Few chunks: the rows of a call, a group of lanes each.
 template <int HD>
 __global__ void __launch_bounds__(kAqJoinThreads) attention_q4_join_few_kernel(const AqParams p) {
-    constexpr int TC = HD / 4, GL = TC < 32 ? TC : 32, E = (kAqJoinFew + GL - 1) / GL, F = TC / GL;
+    constexpr int GL = AqJoin<HD>::GL;
     pdl_wait();
     pdl_launch_dependents();
     const int64_t row = ((int64_t)blockIdx.x * kAqJoinThreads + threadIdx.x) / GL;
-    const int lane = threadIdx.x & 31, l0 = lane % GL, rows = p.src.rows;
+    const int rows = p.src.rows;
     int chunks = 0;
     if (row < (int64_t)p.src.n_seq * rows * p.H) {
         const int s = (int)(row / ((int64_t)rows * p.H)), r = (int)(row / p.H % rows);
         if (!aq_join_of(p, s, r, &chunks)) chunks = 0;
     }
-    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
-    const float4 *part = reinterpret_cast<const float4 *>(p.part) + row * p.max_chunks * TC + l0;
-    float2 y[E];
-    float top = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-        y[j] = j * GL + l0 < chunks ? ml[j * GL + l0] : make_float2(-INFINITY, 0.0f);
-        top = fmaxf(top, y[j].x);
-    }
-#pragma unroll
-    for (int o = GL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-#pragma unroll
-    for (int j = 0; j < E; ++j) y[j].x = y[j].x == -INFINITY ? 0.0f : ex2(y[j].x - top);  // (0: a split without an attended position)
-    float4 v[kAqClasses][F];
-    float l[kAqClasses];
-#pragma unroll
-    for (int k = 0; k < kAqClasses; ++k) {
-        l[k] = 0.0f;
-#pragma unroll
-        for (int f = 0; f < F; ++f) v[k][f] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    const int most = __reduce_max_sync(0xFFFFFFFFu, chunks);
-#pragma unroll
-    for (int c0 = 0; c0 < kAqJoinFew; c0 += kAqClasses) {
-        if (c0 >= most) break;
-        float4 u[kAqClasses][F];
-        float w[kAqClasses], n[kAqClasses];
-#pragma unroll
-        for (int k = 0; k < kAqClasses; ++k) {
-            const int from = lane - l0 + (c0 + k) % GL;
-            w[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].x, from);
-            n[k] = __shfl_sync(0xFFFFFFFFu, y[(c0 + k) / GL].y, from);
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-                u[k][f] = c0 + k < chunks && !(w[k] == 0.0f) ? part[(size_t)(c0 + k) * TC + f * GL] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-#pragma unroll
-        for (int k = 0; k < kAqClasses; ++k) {
-            l[k] += n[k] * w[k];
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                v[k][f].x += u[k][f].x * w[k], v[k][f].y += u[k][f].y * w[k];
-                v[k][f].z += u[k][f].z * w[k], v[k][f].w += u[k][f].w * w[k];
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 1; k < kAqClasses; ++k) {
-        l[0] += l[k];
-#pragma unroll
-        for (int f = 0; f < F; ++f)
-            v[0][f].x += v[k][f].x, v[0][f].y += v[k][f].y, v[0][f].z += v[k][f].z, v[0][f].w += v[k][f].w;
-    }
-    if (chunks == 0) return;
-    const float inv = 1.0f / l[0];
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-        reinterpret_cast<float4 *>(p.out)[row * TC + f * GL + l0] =
-            make_float4(v[0][f].x * inv, v[0][f].y * inv, v[0][f].z * inv, v[0][f].w * inv);
+    aq_join_few<HD>(p, row, chunks);
 }
 
 // Many chunks: a CTA a row, a group of threads a class.
@@ -693,7 +730,7 @@ static cudaError_t launch_aq_join(const AqParams &p, cudaStream_t st) {
 static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqLeaf - 1) / kAqLeaf; }
 
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx) {
-    return 256 + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
+    return 4 * kAqCounters + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
 }
 
 // Scratch of launch_attention_q4_rows for up to `rows` rows, `few` at a time where they are few.
@@ -701,25 +738,35 @@ int64_t attn_q4_rows_scratch_bytes(int rows, int few, int H, int KVH, int hd, in
     int64_t most = attn_q4_scratch_bytes(1, std::min(rows, few), H, hd, max_ctx);
     for (int r = OVF_Q4_EXACT_ROWS + 1; r <= rows; ++r)
         if (attn_q4_many_rows(r, hd))
-            most = std::max(most, 256 + (int64_t)4 * r * H * attn_q4_rows_splits(1, r, H, KVH, max_ctx, sms) * (hd + 2));
+            most = std::max(most, 4 * kAqCounters + (int64_t)4 * r * H * attn_q4_rows_splits(1, r, H, KVH, max_ctx, sms) * (hd + 2));
     return most;
 }
 
 template <int NG, int NT>
-static cudaError_t launch_aq(const AqParams &p, cudaStream_t st, bool pdl) {
+static cudaError_t launch_aq(AqParams p, cudaStream_t st, bool pdl) {
     using S = AqShape<NG, NT>;
     static PerDeviceOnce once;
     const int dev = current_device();
     if (once.pending(dev)) {
-        const cudaError_t e = cudaFuncSetAttribute(attention_q4_kernel<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   S::kTotal);
+        cudaError_t e = cudaFuncSetAttribute(attention_q4_kernel<NG, NT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             S::kTotal);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attention_q4_kernel<NG, NT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
         if (e != cudaSuccess) return e;
         once.mark(dev);
     }
     const int64_t rows = (int64_t)p.src.rows * (p.H / p.src.KVH);
     const int64_t most = (int64_t)p.src.n_seq * p.src.KVH * ((rows + S::kRows - 1) / S::kRows) * p.max_chunks;
-    const int grid = (int)std::min<int64_t>(most, (int64_t)sm_count(dev) * S::kCtas);
-    cudaError_t e = launch_pdl(attention_q4_kernel<NG, NT>, dim3(grid), dim3(kAqThreads), S::kTotal, st, pdl, p);
+    // One launch where the counters have room for every group of rows and a row has few chunks: calls so small that
+    // launching takes the host longer than they take the device (one decoded token of 32 heads over 8 at 2048
+    // positions, called from Python: 13.7 us with a second kernel, 11.5 us without; on the device they are alike).
+    p.groups = (int)((rows + S::kRows - 1) / S::kRows);
+    const bool fused = p.max_chunks > 1 && p.max_chunks <= kAqJoinFew &&
+                       (int64_t)p.src.n_seq * p.src.KVH * p.groups <= kAqCounters;
+    const int64_t room = (int64_t)sm_count(dev) * (fused ? 2 : S::kCtas);
+    const dim3 grid((unsigned)std::min(most, room));
+    if (fused) return launch_pdl(attention_q4_kernel<NG, NT, true>, grid, dim3(kAqThreads), S::kTotal, st, pdl, p);
+    const cudaError_t e = launch_pdl(attention_q4_kernel<NG, NT, false>, grid, dim3(kAqThreads), S::kTotal, st, pdl, p);
     if (e != cudaSuccess || p.max_chunks == 1) return e;
     return launch_aq_join<NG * 32>(p, st);
 }
@@ -733,7 +780,8 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
     p.out = out;
     p.scale2 = scale * 1.44269504088896340736f;
     p.max_chunks = aq_max_chunks(src.max_ctx);
-    p.part = static_cast<float *>(scratch);
+    p.done = static_cast<int *>(scratch);
+    p.part = static_cast<float *>(scratch) + kAqCounters;
     p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.max_chunks * hd;
     cudaError_t e = cudaSuccess;
     if (attn_q4_many_rows(src.rows, hd)) {

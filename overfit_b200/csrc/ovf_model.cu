@@ -934,6 +934,8 @@ ovf_status prefill_alloc(ovf_session *s) {
     if (s->kv_dtype == OVF_KV_Q4)
         A(&s->q4_rows_scratch, (size_t)attn_q4_rows_scratch_bytes(kPrefillRows, kQ4ScratchRows, s->m->h_loc, s->m->kvh_loc,
                                                                   c.head_dim, s->max_ctx, sm_count(s->m->device)));
+    if (!st && s->q4_rows_scratch)
+        st = cuda_status(cudaMemsetAsync(s->q4_rows_scratch, 0, OVF_Q4_SCRATCH_ZEROS, s->stream), "memset");
     const int64_t pfl = attn_rows_scratch_floats(kPrefillRows, s->m->h_loc, s->max_ctx);
     if (!st && s->kv_dtype != OVF_KV_Q4 && attn_rows_supported(c.head_dim, s->kv_dtype) && pfl * 4 <= ((int64_t)512 << 20))
         A((void **)&s->pattn, (size_t)pfl * 4);
@@ -1230,6 +1232,7 @@ ovf_status batch_q4_table(ovf_model *m, ovf_session *const *ss, int n, int max_c
             m->bq4_scratch_bytes = 0;
         }
         if ((r = dalloc(m->allocs, &m->bq4_scratch, need))) return r;
+        OVF_CUDA_TRY(cudaMemsetAsync(m->bq4_scratch, 0, OVF_Q4_SCRATCH_ZEROS, st));
         m->bq4_scratch_bytes = need;
     }
     m->bq4_host.resize(n);
@@ -1709,6 +1712,7 @@ ovf_status ovf_session_create_kv(ovf_model *m, int32_t max_ctx, int32_t kv_dtype
     if (!st) st = cuda_status(cudaMemset(s->counters, 0, (size_t)m->kvh_loc * 4), "memset");
     s->prefill_single = m->tp_world > 1;  // the batched prefill is not split over ranks
     if (!st) st = cuda_status(cudaMemset(s->step, 0, sizeof(DevStep)), "memset");
+    if (!st && q4) st = cuda_status(cudaMemset(s->q4_scratch, 0, OVF_Q4_SCRATCH_ZEROS), "memset");
     if (!st) st = cuda_status(cudaMemset(s->kc, 0, kv_bytes), "memset");
     if (!st) st = cuda_status(cudaMemset(s->vc, 0, kv_bytes), "memset");
     if (!st) st = fill_rope_tables(s);

@@ -489,7 +489,8 @@ class CachedAttentionKernel:
         4-bit caches (``KvCacheQ4``): row r of sequence s is at positions[s] + r
         and attends everything up to itself.  ``k_new`` / ``v_new`` [n_seq, rows,
         n_kv_heads * head_dim] are appended first.  ``scratch``: uint8 of
-        ``q4_scratch_bytes``, for one call at a time."""
+        ``q4_scratch_bytes``, the first 256 zero (a call leaves them so), for one
+        call at a time."""
         n_seq, rows, spans = KvCacheQ4.spans(k_cache, v_cache, positions, query, "query", n_kv_heads, head_dim, max_ctx,
                                              rope_cos, rope_sin, row_counts, n_heads)
         if output is None or scratch is None or (k_new is None) != (v_new is None):

@@ -86,9 +86,11 @@ class Batch:
         if scratch is None:
             scratch = torch.full((A.q4_scratch_bytes(n, rows, self.heads, self.kv_heads, self.hd, self.ctx),), 0xFF,
                                  dtype=torch.uint8, device="cuda")
+            scratch[:256] = 0
         A.compute_q4(dev(q.reshape(n, rows, -1)), kc, vc, out, dev(positions, torch.int32), self.heads, self.kv_heads, self.hd,
                      self.ctx, self.scale, scratch, self.dcos, self.dsin, self.split_half,
                      row_counts=None if counts is None else dev(counts, torch.int32))
+        assert not scratch[:256].any()
         return host(out).reshape(q.shape)
 
     def check(self, got, q, positions, counts=None):
