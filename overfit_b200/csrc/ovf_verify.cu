@@ -38,7 +38,8 @@ static constexpr int kVfStep = 128;         // elements that a warp takes at onc
 static constexpr int kVfSlots = kVfRows / (kVfMinCluster * kVfWarps) + 2;
 
 // e^x in 64 bits for x of -700 to 700, off by less than 2^-44: x = n ln 2 / 64 + r, the series of e^r to r^4
-// (|r| < 0.0055), and 2^(n / 64) from `tab`: entry i holds the bits of 2^(i / 64) less i << 46.  NaN stays NaN.
+// (|r| < 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64)
+// less i << 46 (the lanes of half a warp have a copy each, for indices are as good as random).  NaN stays NaN.
 // A branch for other x would double its time (3.8 clocks a warp and SM): its callers raise smaller logits to
 // a floor of weight e^-690 instead, in 32 bits.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
@@ -50,7 +51,7 @@ __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab
     y = fma(y, r, 1.0);
     y = fma(y, r, 1.0);
     const int k = __double2loint(kd);
-    return y * __longlong_as_double((long long)(tab[k & 63] + ((unsigned long long)(long long)k << 46)));
+    return y * __longlong_as_double((long long)(tab[(k & 63) * 16] + ((unsigned long long)(long long)k << 46)));
 }
 // The same for any x up to 0 (0 below e^-690).
 __device__ __forceinline__ double vf_exp0(double x, const unsigned long long *tab) {
@@ -122,7 +123,7 @@ struct VfShared {
     double part[kVfWarps];               // the drawing: sums of this CTA's warps' parts
     double all[kVfCluster * kVfWarps];   // of all parts
     double step[kVfWarps];               // of the steps of the part that holds the token
-    unsigned long long tab[64];
+    unsigned long long tab[64 * 16];
     int token, last;
 };
 
@@ -163,7 +164,9 @@ __device__ __forceinline__ VfFour vf_weights(const VfRow &r, const VfLoad &l, in
     return f;
 }
 
-__global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const VerifyParams p) {
+// Steps: loads of a lane that are under way together.
+template <int Steps, int Ctas>
+__global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const VerifyParams p) {
     extern __shared__ __align__(16) unsigned char vf_smem[];
     VfShared &sh = *reinterpret_cast<VfShared *>(vf_smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = p.vocab;
@@ -179,7 +182,8 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
     const float *logits = p.logits + (size_t)s * (p.max_drafts + 1) * V;
     const double inv = 1.0 / (double)T;
     const float last_u = u[p.max_drafts];
-    if (tid < 64) sh.tab[tid] = vf_tab(tid);
+    for (int i = tid; i < 64 * 16; i += kVfThreads) sh.tab[i] = vf_tab(i / 16);
+    const unsigned long long *tab = sh.tab + (lane & 15);
     for (int j = tid; j < n; j += kVfThreads) sh.draft[j] = p.drafts[(size_t)s * p.max_drafts + j];
 
     __syncthreads();
@@ -199,20 +203,20 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         double sum = 0.0;
         bool bad = false;
         const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        float4 v[2];
+        float4 v[Steps];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY) : none;
-        for (; st < stop; st += 2, at += 2 * kVfStep) {
-            float4 w[2];
+        for (int i = 0; i < Steps; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY) : none;
+        for (; st < stop; st += Steps, at += Steps * kVfStep) {
+            float e[4 * Steps];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                w[i] = v[i];  // the next two are under way meanwhile
-                v[i] = st + 2 + i < stop ? vf_load4(x, V, at + (2 + i) * kVfStep, -INFINITY) : none;
+            for (int i = 0; i < Steps; ++i) {
+                e[4 * i] = v[i].x, e[4 * i + 1] = v[i].y, e[4 * i + 2] = v[i].z, e[4 * i + 3] = v[i].w;
+                // the next ones are under way meanwhile
+                v[i] = st + Steps + i < stop ? vf_load4(x, V, at + (Steps + i) * kVfStep, -INFINITY) : none;
             }
-            const float e[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
             if (greedy) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 4 * Steps; ++i) {
                     bad |= e[i] != e[i];
                     const int here = at + (i >> 2) * kVfStep + (i & 3);
                     if (e[i] > m || (e[i] == m && here < place)) m = e[i], place = here;
@@ -220,17 +224,17 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             } else {
                 float top = m;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, e[i]);
+                for (int i = 0; i < 4 * Steps; ++i) top = fmaxf(top, e[i]);
                 if (top > m) {
-                    sum *= vf_exp0(((double)m - (double)top) * inv, sh.tab);
+                    sum *= vf_exp0(((double)m - (double)top) * inv, tab);
                     m = top;
                 }
                 const double md = (double)m;
                 const float floor = vf_floor(m, T);
                 double part[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const double y = vf_exp(((double)vf_raise(e[i], floor) - md) * inv, sh.tab);
+                for (int i = 0; i < 4 * Steps; ++i) {
+                    const double y = vf_exp(((double)vf_raise(e[i], floor) - md) * inv, tab);
                     part[i & 3] = i < 4 ? y : part[i & 3] + y;
                 }
                 sum += (part[0] + part[1]) + (part[2] + part[3]);
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             place = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)place : 0x7FFFFFFFu);
             if (__any_sync(0xFFFFFFFFu, bad)) sum = __longlong_as_double(0x7ff8000000000000ll);
         } else {
-            sum = warp_sum(sum * vf_exp0(((double)m - (double)top) * inv, sh.tab));
+            sum = warp_sum(sum * vf_exp0(((double)m - (double)top) * inv, tab));
         }
         if (lane == 0) {
             sh.m[warp][j - first_row] = top;
@@ -274,15 +278,15 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             const int at2 = cluster_read(&sh.at[w % kVfWarps][slot], from);
             const float top = fmaxf(m, m2);
             sum = greedy ? sum + sum2
-                         : sum * vf_exp0(((double)m - (double)top) * inv, sh.tab) +
-                               sum2 * vf_exp0(((double)m2 - (double)top) * inv, sh.tab);
+                         : sum * vf_exp0(((double)m - (double)top) * inv, tab) +
+                               sum2 * vf_exp0(((double)m2 - (double)top) * inv, tab);
             if (m2 > m || (m2 == m && at2 < at)) at = at2;
             m = top;
         }
         float top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        if (!greedy) sum *= vf_exp0(((double)m - (double)top) * inv, sh.tab);
+        if (!greedy) sum *= vf_exp0(((double)m - (double)top) * inv, tab);
         sum = warp_sum(sum);
         at = (int)__reduce_min_sync(0xFFFFFFFFu, m == top ? (unsigned)at : 0x7FFFFFFFu);
         if (lane) continue;
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         } else if (greedy) {
             if (j < n && d == at) state = VF_ACCEPT;
         } else if (d >= 0 && d < V) {
-            const double e = vf_exp0(((double)draft_x - (double)top) * inv, sh.tab);
+            const double e = vf_exp0(((double)draft_x - (double)top) * inv, tab);
             if ((double)draft_u * (double)draft_q * sum < e) state = VF_ACCEPT;
         }
         sh.row_sum[j] = sum;
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
         double drafted = 0.0;  // the weight of a certain draft, which is taken away
         if (k < n && !p.probs && sh.draft[k] >= 0 && sh.draft[k] < V) {
             row.out = sh.draft[k];
-            drafted = vf_exp0(((double)row.x[row.out] - row.m) * inv, sh.tab);
+            drafted = vf_exp0(((double)row.x[row.out] - row.m) * inv, tab);
         }
         // The row's parts and their weights.  Without a distribution to take away they are the runs above and their
         // sums (less a draft's, unless little were left: a difference of nearly equal sums would be inexact); else
@@ -350,7 +354,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
                 const VfLoad now = a;
                 a = b;
                 vf_load(row, i + 2, &b);
-                const VfFour f = vf_weights(row, now, i, sh.tab);
+                const VfFour f = vf_weights(row, now, i, tab);
                 mine += (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
             }
             mine = warp_sum(mine);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
                 } else {
                     const int slot = k - (int)(w * run / steps);
                     const double m2 = (double)cluster_read(&sh.m[w % kVfWarps][slot], from);
-                    y = cluster_read(&sh.sum[w % kVfWarps][slot], from) * vf_exp0((m2 - row.m) * inv, sh.tab);
+                    y = cluster_read(&sh.sum[w % kVfWarps][slot], from) * vf_exp0((m2 - row.m) * inv, tab);
                     if (row.out >= 0 && (unsigned)((row.out + row.shift) / kVfStep + k * steps) / run == (unsigned)w) {
                         y -= drafted;
                         if (y < 1e-12 * sh.row_sum[k]) y = 0.0;  // rounding, if the part had nothing else
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
             for (int i = p0; i < p1 && found < 0; i += kVfWarps) {
                 VfLoad l;
                 vf_load(row, min(i + warp, p1), &l);
-                VfFour f = vf_weights(row, l, i + warp, sh.tab);
+                VfFour f = vf_weights(row, l, i + warp, tab);
                 if (i + warp >= p1) f.w[0] = f.w[1] = f.w[2] = f.w[3] = 0.0;
                 const double four = (f.w[0] + f.w[1]) + (f.w[2] + f.w[3]);
                 double incl = four;
@@ -481,18 +485,18 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_drafts_kernel(const Veri
     cluster_barrier();  // nobody reads another CTA's memory any more
 }
 
-ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st) {
+template <int Steps, int Ctas>
+static cudaError_t launch_vf(const VerifyParams &p, int n_seq, int cluster, cudaStream_t st) {
     static PerDeviceOnce once;
     const int dev = current_device();
+    const auto kernel = verify_drafts_kernel<Steps, Ctas>;
     if (once.pending(dev)) {
-        cudaError_t e = cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(verify_drafts_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)sizeof(VfShared));
-        if (e != cudaSuccess) return cuda_status(e, "verify_drafts");
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(VfShared));
+        if (e != cudaSuccess) return e;
         once.mark(dev);
     }
-    const int cluster = n_seq * kVfCluster <= sm_count(dev) ? kVfCluster : kVfMinCluster;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_seq * cluster);
     cfg.blockDim = dim3(kVfThreads);
@@ -504,7 +508,14 @@ ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t s
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, verify_drafts_kernel, p), "verify_drafts");
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st) {
+    // where every CTA of 16-CTA clusters has an SM for itself, more loads a lane; else clusters of 8, two CTAs an SM
+    const bool few = n_seq * kVfCluster <= sm_count(current_device());
+    const cudaError_t e = few ? launch_vf<4, 1>(p, n_seq, kVfCluster, st) : launch_vf<2, 2>(p, n_seq, kVfMinCluster, st);
+    return cuda_status(e, "verify_drafts");
 }
 
 }  // namespace ovf
