@@ -143,7 +143,16 @@ struct VfLoad {
     float x[4], q[4];
 };
 __device__ __forceinline__ void vf_load(const VfRow &r, int i, VfLoad *l) {
-    const int at = 4 * (32 * i + (threadIdx.x & 31)) - r.shift;
+    const int at = 4 * (32 * i + (threadIdx.x & 31)) - r.shift, a0 = 128 * i - r.shift;
+    if (a0 >= 0 && a0 + kVfStep <= r.V) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(r.x + at));
+        l->x[0] = v.x, l->x[1] = v.y, l->x[2] = v.z, l->x[3] = v.w;
+        if (r.q) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) l->q[b] = __ldg(r.q + at + b);
+        }
+        return;
+    }
     const float4 v = vf_load4(r.x, r.V, at, -INFINITY);
     l->x[0] = v.x, l->x[1] = v.y, l->x[2] = v.z, l->x[3] = v.w;
     if (r.q) {
@@ -204,16 +213,26 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
         bool bad = false;
         const float4 none = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         float4 v[Steps];
+        auto load = [&](unsigned from, int place0) {
+            // (a branch of the whole warp: one per load would keep them from being under way together)
+            const int a0 = place0 - 4 * lane;
+            if (a0 >= 0 && a0 + Steps * kVfStep <= V && from + Steps <= stop) {
 #pragma unroll
-        for (int i = 0; i < Steps; ++i) v[i] = st + i < stop ? vf_load4(x, V, at + i * kVfStep, -INFINITY) : none;
+                for (int i = 0; i < Steps; ++i) v[i] = __ldg(reinterpret_cast<const float4 *>(x + place0 + i * kVfStep));
+            } else {
+#pragma unroll
+                for (int i = 0; i < Steps; ++i) v[i] = from + i < stop ? vf_load4(x, V, place0 + i * kVfStep, -INFINITY) : none;
+            }
+        };
+        load(st, at);
         for (; st < stop; st += Steps, at += Steps * kVfStep) {
+            float4 w[Steps];
+#pragma unroll
+            for (int i = 0; i < Steps; ++i) w[i] = v[i];
+            if (st + Steps < stop) load(st + Steps, at + Steps * kVfStep);  // under way meanwhile
             float e[4 * Steps];
 #pragma unroll
-            for (int i = 0; i < Steps; ++i) {
-                e[4 * i] = v[i].x, e[4 * i + 1] = v[i].y, e[4 * i + 2] = v[i].z, e[4 * i + 3] = v[i].w;
-                // the next ones are under way meanwhile
-                v[i] = st + Steps + i < stop ? vf_load4(x, V, at + (Steps + i) * kVfStep, -INFINITY) : none;
-            }
+            for (int i = 0; i < Steps; ++i) e[4 * i] = w[i].x, e[4 * i + 1] = w[i].y, e[4 * i + 2] = w[i].z, e[4 * i + 3] = w[i].w;
             if (greedy) {
 #pragma unroll
                 for (int i = 0; i < 4 * Steps; ++i) {
