@@ -32,10 +32,9 @@ namespace ovf {
 static constexpr int kVfThreads = 512, kVfWarps = kVfThreads / 32;
 static constexpr int kVfRows = 1024;        // max_drafts + 1
 static constexpr int kVfCluster = 16;       // at most
-static constexpr int kVfMinCluster = 8;
 static constexpr int kVfStep = 128;         // elements that a warp takes at once
 // rows that a warp's run meets: the run is ceil(rows * steps / warps) steps of `steps` a row
-static constexpr int kVfSlots = kVfRows / (kVfMinCluster * kVfWarps) + 2;
+static constexpr int kVfSlots = kVfRows / kVfWarps + 2;  // (a cluster of one CTA)
 
 // e^x in 64 bits for x of -700 to 700, off by less than 2^-44: x = n ln 2 / 64 + r, the series of e^r to r^4
 // (|r| < 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64)
@@ -531,9 +530,14 @@ static cudaError_t launch_vf(const VerifyParams &p, int n_seq, int cluster, cuda
 }
 
 ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st) {
-    // where every CTA of 16-CTA clusters has an SM for itself, more loads a lane; else clusters of 8, two CTAs an SM
-    const bool few = n_seq * kVfCluster <= sm_count(current_device());
-    const cudaError_t e = few ? launch_vf<4, 1>(p, n_seq, kVfCluster, st) : launch_vf<2, 2>(p, n_seq, kVfMinCluster, st);
+    // Where every CTA of 16-CTA clusters has an SM for itself, those, with more loads a lane; else the largest clusters
+    // of which all sequences' run at once, two CTAs an SM (42 sequences of 4 x 25276 logits: 34.5 us in clusters of 8,
+    // of which only 37 fit, 25.7 in clusters of 4; 32 of 8 x 151936: 77.0 in clusters of 8, 85.7 in clusters of 4).
+    const int sms = sm_count(current_device());
+    int cluster = 8;
+    while (cluster > 1 && n_seq * cluster > 2 * sms) cluster /= 2;
+    const cudaError_t e = n_seq * kVfCluster <= sms ? launch_vf<4, 1>(p, n_seq, kVfCluster, st)
+                                                    : launch_vf<2, 2>(p, n_seq, cluster, st);
     return cuda_status(e, "verify_drafts");
 }
 
