@@ -379,17 +379,31 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
         struct VCodes {
             uint4 w, d, m;
         } vc[VU];
+        // this lane's places in the head's cache, from the tile that is loaded next on; a tile inside the data (all but
+        // the last) needs no checks
+        const uint8_t *kp[KU], *vp[VU];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int pos = (me * KU + u) * 8 + (e >> 1) + 4 * (e & 1);
+            kp[u] = w.k + ((size_t)h * w.tiles + (size_t)t0 * (kArN / kQ4Tile) + pos / kQ4Tile) * q4_tile_bytes(HD) +
+                    q4_key_word(NG, pos & 31, t, 0) * 4;
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int unit = me * VU + u;
+            vp[u] = w.v + ((size_t)h * w.tiles + (size_t)t0 * (kArN / kQ4Tile) + unit / NG) * q4_tile_bytes(HD);
+        }
+        constexpr int kStep = kArN / kQ4Tile * q4_tile_bytes(HD);
         auto load_keys = [&](int i) {
+            const bool inside = (t0 + i + 1) * kArN <= data_end;
 #pragma unroll
             for (int u = 0; u < KU; ++u) {
-                const int p8 = (t0 + i) * kArN + (me * KU + u) * 8, pos = p8 + (e >> 1) + 4 * (e & 1);
-                if (p8 < data_end) {
-                    const uint8_t *tile = w.k + ((size_t)h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
-                    const uint32_t *wp = reinterpret_cast<const uint32_t *>(tile) + q4_key_word(NG, pos & 31, t, 0);
-                    const uint32_t *dp = reinterpret_cast<const uint32_t *>(tile + q4_code_bytes(HD)) + (pos & 31) * NG;
+                const int row = ((me * KU + u) * 8 + (e >> 1) + 4 * (e & 1)) & 31;  // of its cache tile
+                const uint8_t *wp = kp[u], *dp = kp[u] + q4_code_bytes(HD) + row * NG * 4 - q4_key_word(NG, row, t, 0) * 4;
+                if (inside || (t0 + i) * kArN + (me * KU + u) * 8 < data_end) {
                     if (NG == 1) {
-                        kc[u].w[0] = *wp;
-                        kc[u].dm[0] = *dp;
+                        kc[u].w[0] = *reinterpret_cast<const uint32_t *>(wp);
+                        kc[u].dm[0] = *reinterpret_cast<const uint32_t *>(dp);
                     } else if (NG == 2) {
                         *reinterpret_cast<uint2 *>(kc[u].w) = *reinterpret_cast<const uint2 *>(wp);
                         *reinterpret_cast<uint2 *>(kc[u].dm) = *reinterpret_cast<const uint2 *>(dp);
@@ -401,21 +415,21 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
 #pragma unroll
                     for (int g = 0; g < NG; ++g) kc[u].w[g] = kc[u].dm[g] = 0;
                 }
+                kp[u] += kStep;
             }
         };
         auto load_values = [&](int i) {
+            const bool inside = (t0 + i + 1) * kArN <= data_end;
 #pragma unroll
             for (int u = 0; u < VU; ++u) {
                 const int unit = me * VU + u, j = unit / NG, g = unit % NG, pos = (t0 + i) * kArN + j * kQ4Tile;
-                vc[u].w = vc[u].d = vc[u].m = make_uint4(0, 0, 0, 0);
-                if (unit < 4 * NG && pos < data_end) {
-                    const uint8_t *tile = w.v + ((size_t)h * w.tiles + pos / kQ4Tile) * q4_tile_bytes(HD);
-                    vc[u].w = *reinterpret_cast<const uint4 *>(tile + ((g * 8 + e) * 4 + t) * 16);
-                    vc[u].d = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + g * 128 + t * 16);
-                    vc[u].m = *reinterpret_cast<const uint4 *>(tile + q4_code_bytes(HD) + g * 128 + 64 + t * 16);
-                    const int have = data_end - (pos + 8 * t);  // of these 8 positions
-                    if (have < 8) {
+                if (unit < 4 * NG && (inside || pos < data_end)) {
+                    vc[u].w = *reinterpret_cast<const uint4 *>(vp[u] + ((g * 8 + e) * 4 + t) * 16);
+                    vc[u].d = *reinterpret_cast<const uint4 *>(vp[u] + q4_code_bytes(HD) + g * 128 + t * 16);
+                    vc[u].m = *reinterpret_cast<const uint4 *>(vp[u] + q4_code_bytes(HD) + g * 128 + 64 + t * 16);
+                    if (!inside) {
                         // what lies behind the data may be anything: its weights are 0, and its values must be numbers
+                        const int have = data_end - (pos + 8 * t);  // of these 8 positions
                         uint32_t *d = &vc[u].d.x, *m = &vc[u].m.x;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -424,7 +438,10 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                             m[k] &= keep;
                         }
                     }
+                } else {
+                    vc[u].w = vc[u].d = vc[u].m = make_uint4(0, 0, 0, 0);
                 }
+                vp[u] += kStep;
             }
         };
         load_keys(0);
