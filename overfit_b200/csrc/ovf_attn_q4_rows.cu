@@ -265,26 +265,28 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             const int p0 = (t0 + i) * kArN + half * (kArN / 2);
             wait(&s_full[i & 1], (i >> 1) & 1);
             tc_fence_after();
-            // two passes over 32 columns at a time: the registers of 64 would not leave room for 17 warps
+            // two passes over the columns, a few at a time: the registers of 64 would not leave room for 17 warps
             const bool masked = __any_sync(0xFFFFFFFFu, p0 + kArN / 2 - 1 > limit);
-            float x[32];
-            auto columns = [&](int c0) {
-                tmem_ld16_nowait(s_at + c0, reinterpret_cast<uint32_t *>(x));
-                tmem_ld16_nowait(s_at + c0 + 16, reinterpret_cast<uint32_t *>(x) + 16);
-                tmem_ld_wait();
+            float x[2][16];
+            auto hide = [&](int c0, float *y) {
                 if (masked) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)  // columns in the order 0 4 1 5 2 6 3 7 of positions
-                        if (p0 + c0 + (c & ~7) + ((c & 7) >> 1) + 4 * (c & 1) > limit) x[c] = -INFINITY;
+                    for (int c = 0; c < 16; ++c)  // columns in the order 0 4 1 5 2 6 3 7 of positions
+                        if (p0 + c0 + (c & ~7) + ((c & 7) >> 1) + 4 * (c & 1) > limit) y[c] = -INFINITY;
                 }
             };
-            columns(32);
-            float top = x[0];
+            auto load = [&](int c0, float *y) { tmem_ld16_nowait(s_at + c0, reinterpret_cast<uint32_t *>(y)); };
+            float top = -INFINITY;
 #pragma unroll
-            for (int c = 1; c < 32; ++c) top = fmaxf(top, x[c]);
-            columns(0);
+            for (int c0 = 32; c0 >= 0; c0 -= 32) {
+                load(c0, x[0]);
+                load(c0 + 16, x[1]);
+                tmem_ld_wait();
+                hide(c0, x[0]);
+                hide(c0 + 16, x[1]);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) top = fmaxf(top, x[c]);
+                for (int c = 0; c < 16; ++c) top = fmaxf(top, fmaxf(x[0][c], x[1][c]));
+            }
             top *= factor;
             float *mine = xch + (i & 1) * 2 * kArM + half * kArM + row;
             *mine = top;
@@ -317,22 +319,28 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             const float base = (m == -INFINITY ? 0.0f : m) - kArLift;
             float2 sum = make_float2(0.0f, 0.0f);
             const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
-            // (P of the first 32 columns goes where those scores were, hi parts before lo parts of each half)
-            auto weights = [&](int c0) {
-                uint32_t hi[16], lo[16];
+            // (P of 16 columns goes where those scores were: 8 columns of hi, 8 of lo parts)
+            auto weights = [&](int c0, const float *y) {
+                uint32_t p16[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float2 w = fma2(make_float2(x[2 * j], x[2 * j + 1]), factor2, base2);
+                for (int j = 0; j < 8; ++j) {
+                    float2 w = fma2(make_float2(y[2 * j], y[2 * j + 1]), factor2, base2);
                     w = make_float2(ex2(w.x), ex2(w.y));
                     sum = add2(sum, w);
-                    ar_split(w.x, w.y, hi[j], lo[j]);
+                    ar_split(w.x, w.y, p16[j], p16[8 + j]);
                 }
-                tmem_st16(s_at + c0, reinterpret_cast<const float *>(hi));
-                tmem_st16(s_at + c0 + 16, reinterpret_cast<const float *>(lo));
+                tmem_st16(s_at + c0, reinterpret_cast<const float *>(p16));
             };
-            weights(0);
-            columns(32);
-            weights(32);
+            // (the first 32 columns are still there)
+            weights(0, x[0]);
+            load(32, x[0]);
+            weights(16, x[1]);
+            load(48, x[1]);
+            tmem_ld_wait();
+            hide(32, x[0]);
+            hide(48, x[1]);
+            weights(32, x[0]);
+            weights(48, x[1]);
             l += sum.x + sum.y;
             tmem_st_wait();
             // O of the last tile is done by now; a phase that nobody waited for could not be told from the next but one
@@ -521,12 +529,12 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                 const uint32_t pa = base + SM::s_col + st * kArN, d = base + SM::o_col;
                 if (i == 0) ar_mma<false>(d, pa, b, ar_idesc(HD));
                 else ar_mma<true>(d, pa, b, ar_idesc(HD));
-                ar_mma<true>(d, pa + 16, b, ar_idesc(HD));
+                ar_mma<true>(d, pa + 8, b, ar_idesc(HD));
 #pragma unroll
                 for (int k = 1; k < kArN / 16; ++k) {
-                    const uint32_t at = pa + (k >> 1) * 32 + (k & 1) * 8;  // 32 positions: 16 columns of hi, 16 of lo parts
+                    const uint32_t at = pa + k * 16;  // 16 positions: 8 columns of hi, 8 of lo parts
                     ar_mma<true>(d, at, b + 16 * k, ar_idesc(HD));
-                    ar_mma<true>(d, at + 16, b + 16 * k, ar_idesc(HD));
+                    ar_mma<true>(d, at + 8, b + 16 * k, ar_idesc(HD));
                 }
                 tc_commit(&v_empty[st]);
                 tc_commit(o_done);
