@@ -9,6 +9,13 @@
 // operand enters as two fp16 numbers (hi + lo, 22 bits), here as two products into
 // one accumulator, and the cached values are fp16 numbers by definition.
 //
+// The tensor cores cut an accumulator's lower bits off at each addition, toward zero,
+// so that a long sum falls short (measured: 3e-7 of O per 128 positions, 1.9e-5 at
+// 8192), where fp32's rounding would average out.  An accumulator in TMEM therefore
+// sums kArWindow tiles at most; the windows are added in fp32 in shared memory.  Four
+// tiles: 1.5e-6 off at any length; eight: 2.7e-6, and 4 % faster.  S takes its small lo
+// products first.
+//
 // The maximum that P refers to is raised only when a row's scores pass it by more
 // than 2^8; until then P is at most 2^(6 + 8 + 1), inside fp16, and O needs no
 // rescaling.  Weights are held times 2^6.
@@ -38,6 +45,7 @@ static constexpr int kArExpand = 8;      // expanding warps
 static constexpr int kArMma = 8 + kArExpand;
 static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
+static constexpr int kArWindow = 4;      // tiles that one accumulator in TMEM sums (a power of 2)
 static constexpr float kArLift = 6.0f;  // weights times 2^6
 static constexpr float kArSlack = 8.0f; // the maximum is raised when it is passed by 2^8
 
@@ -50,7 +58,8 @@ struct ArSmem {
     static constexpr int q_pitch = HD + 4;                       // rows of Q on its way to TMEM (in K's and V's place)
     static constexpr int q_bytes = kArM * q_pitch * 4;
     static constexpr int main_bytes = 2 * kArStages * kTile > q_bytes ? 2 * kArStages * kTile : q_bytes;
-    static constexpr int x_off = main_bytes;                     // [2][2][128] floats: halves' maxima, sums
+    static constexpr int acc_off = main_bytes;                   // [half][dimension / 4][row] float4: O of earlier windows
+    static constexpr int x_off = acc_off + kArM * HD * 4;        // [2][2][128] floats: halves' maxima, sums
     static constexpr int bar_off = x_off + 2 * 2 * kArM * 4;
     static constexpr int total = bar_off + 256 + 128;
     // TMEM columns
@@ -259,8 +268,10 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     auto wait = [&](uint64_t *bar, int parity) { ok = ok && mbar_wait_bounded(bar, (uint32_t)parity); };
     if (warp < 8) {
         // ------------------------------------------------------- softmax
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f, m_acc = -INFINITY;  // m_acc: what O of the earlier windows refers to
+        float4 *acc = reinterpret_cast<float4 *>(sm + SM::acc_off) + half * (HD / 8) * kArM + row;
         for (int i = 0; i < nt; ++i) {
+            const bool fresh = (i & (kArWindow - 1)) == 0;  // O begins anew with this tile
             const uint32_t s_at = lane_addr + SM::s_col + (i & 1) * kArN + half * (kArN / 2);
             const int p0 = (t0 + i) * kArN + half * (kArN / 2);
             wait(&s_full[i & 1], (i >> 1) & 1);
@@ -292,8 +303,10 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             *mine = top;
             ar_pair_sync(warp & 3);
             top = fmaxf(top, xch[(i & 1) * 2 * kArM + (half ^ 1) * kArM + row]);
-            if (i == 0) {
-                m = top;
+            const float m_before = m;
+            if (fresh) {
+                if (top > m + kArSlack || m == -INFINITY) m = top;
+                l *= m_before == m ? 1.0f : ex2(m_before - m);
             } else {
                 const bool raise = top > m + kArSlack || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, raise)) {
@@ -345,6 +358,27 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             tmem_st_wait();
             // O of the last tile is done by now; a phase that nobody waited for could not be told from the next but one
             if (i > 0) wait(o_done, (i - 1) & 1);
+            if (fresh && i > 0) {
+                tc_fence_after();
+                const float k = m_before == -INFINITY ? 0.0f : ex2(m_before - m), ka = m_acc == -INFINITY ? 0.0f : ex2(m_acc - m);
+                constexpr int W = HD >= 64 ? 32 : 16;  // columns at a time
+#pragma unroll
+                for (int c = 0; c < HD / 2; c += W) {
+                    float o[W];
+#pragma unroll
+                    for (int j = 0; j < W; j += 16)
+                        tmem_ld16_nowait(lane_addr + SM::o_col + half * (HD / 2) + c + j, reinterpret_cast<uint32_t *>(o + j));
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < W; j += 4) {
+                        float4 *at = acc + (c + j) / 4 * kArM, a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (i > kArWindow) a = *at;
+                        *at = make_float4(fmaf(a.x, ka, o[j] * k), fmaf(a.y, ka, o[j + 1] * k), fmaf(a.z, ka, o[j + 2] * k),
+                                          fmaf(a.w, ka, o[j + 3] * k));
+                    }
+                }
+                m_acc = m;
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[i & 1]);
@@ -362,11 +396,22 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
         float *dst = p.splits == 1 ? p.out + orow * HD : p.part + (orow * p.splits + split) * HD;
         if (real && half == 0 && p.splits > 1)
             *reinterpret_cast<float2 *>(p.part_ml + (orow * p.splits + split) * 2) = make_float2(m, l);
+        const float ka = m_acc == -INFINITY ? 0.0f : ex2(m_acc - m);
 #pragma unroll
         for (int c = 0; c < HD / 2; c += 16) {
             float o[16];
             tmem_ld16_nowait(lane_addr + SM::o_col + half * (HD / 2) + c, reinterpret_cast<uint32_t *>(o));
             tmem_ld_wait();
+            if (nt > kArWindow) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 a = acc[(c / 4 + j) * kArM];
+                    o[4 * j] = fmaf(a.x, ka, o[4 * j]);
+                    o[4 * j + 1] = fmaf(a.y, ka, o[4 * j + 1]);
+                    o[4 * j + 2] = fmaf(a.z, ka, o[4 * j + 2]);
+                    o[4 * j + 3] = fmaf(a.w, ka, o[4 * j + 3]);
+                }
+            }
             if (real) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4)
@@ -507,10 +552,11 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                 const uint32_t d = base + SM::s_col + st * kArN;
 #pragma unroll
                 for (int k = 0; k < HD / 16; ++k) {  // (a step of 16: 256 bytes, 16 in the descriptor's units)
-                    if (k == 0) ar_mma<false>(d, base + SM::q_col, b, ar_idesc(kArN));
-                    else ar_mma<true>(d, base + SM::q_col + 8 * k, b + 16 * k, ar_idesc(kArN));
-                    ar_mma<true>(d, base + SM::q_col + HD / 2 + 8 * k, b + 16 * k, ar_idesc(kArN));
+                    if (k == 0) ar_mma<false>(d, base + SM::q_col + HD / 2, b, ar_idesc(kArN));
+                    else ar_mma<true>(d, base + SM::q_col + HD / 2 + 8 * k, b + 16 * k, ar_idesc(kArN));
                 }
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) ar_mma<true>(d, base + SM::q_col + 8 * k, b + 16 * k, ar_idesc(kArN));
                 tc_commit(&k_empty[st]);
                 tc_commit(&s_full[st]);
             }
@@ -527,7 +573,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             if (elect_one()) {
                 const uint64_t b = umma_desc(vb + st * SM::kTile, 128, kArN / 8 * 128);
                 const uint32_t pa = base + SM::s_col + st * kArN, d = base + SM::o_col;
-                if (i == 0) ar_mma<false>(d, pa, b, ar_idesc(HD));
+                if ((i & (kArWindow - 1)) == 0) ar_mma<false>(d, pa, b, ar_idesc(HD));
                 else ar_mma<true>(d, pa, b, ar_idesc(HD));
                 ar_mma<true>(d, pa + 8, b, ar_idesc(HD));
 #pragma unroll

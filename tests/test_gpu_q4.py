@@ -228,6 +228,44 @@ def test_long_sequence(K):
     b.check(b.run(q, [19997]), q, [19997])
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd", [(6, 2, 64), (2, 1, 256)])
+def test_long_sequences_of_several_rows(K, heads, kv_heads, hd):
+    """More chunks than one group of lanes joins, for every (sequence, row, head)."""
+    b = Batch(K, 3, heads, kv_heads, hd, 13000, [12990, 77, 12999], seed=31)
+    q = b.query(3)
+    at, counts = [12987, 74, 12998], [3, 2, 1]
+    b.check(b.run(q, at, counts), q, at, counts)
+
+
+@pytest.mark.parametrize("hd", [32, 128])
+def test_long_sums_of_many_rows(K, hd):
+    """Sums over 16384 positions by one CTA.  Values of 1 to 2, so that errors of one sign add up: the tensor cores cut an
+    accumulator by less than 2^-23 of itself at each of at most 64 additions, the sums of these follow fp32 rounding; a
+    score's error is bounded as in Batch.check."""
+    heads, rows, ctx = 8, 1200, 16384
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k = torch.randn(1, ctx, hd, generator=g, device="cuda")
+    v = 1 + torch.rand(1, ctx, hd, generator=g, device="cuda")
+    q = torch.randn(1, rows, heads * hd, generator=g, device="cuda") * 0.1
+    kc, vc = (torch.zeros(K.KvCacheQ4.bytes(1, hd, ctx), dtype=torch.uint8, device="cuda") for _ in "kv")
+    zero = dev([0], torch.int32)
+    K.KvCacheQ4.append(k, v, kc, vc, zero, 1, hd, ctx)
+    K.KvCacheQ4.read(kc, vc, zero, 1, hd, ctx, k, v)
+    A = K.CachedAttentionKernel
+    scratch = torch.zeros(A.q4_scratch_bytes(1, rows, heads, 1, hd, ctx), dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(q)
+    A.compute_q4(q, kc, vc, out, dev([ctx - rows], torch.int32), heads, 1, hd, ctx, hd ** -0.5, scratch)
+    k, v = k[0].double(), v[0].double()
+    most, off = 0.0, torch.arange(ctx, device="cuda")
+    for r in range(0, rows, 100):
+        x = q[0, r:r + 100].view(-1, heads, hd).double() * hd ** -0.5
+        most = max(most, (x.abs() @ k.abs().T).max().item())
+        hidden = off[None] > ctx - rows + r + torch.arange(x.shape[0], device="cuda")[:, None]
+        want = (x @ k.T).masked_fill(hidden[:, None], -torch.inf).softmax(-1) @ v
+        tol = 2 * (64 * 2.0 ** -23 + 2 * (most * 2.0 ** -21 + 2.0 ** -20))
+        torch.testing.assert_close(out[0, r:r + 100].view_as(want).double(), want, rtol=0, atol=tol)
+
+
 @pytest.mark.parametrize("rows", [1, 5, 100])
 def test_bytes_behind_a_sequence_do_not_matter(K, rows):
     """Stale bytes behind the last position (all ones: codes 15, D and M NaN) change no bit."""
@@ -373,6 +411,37 @@ def test_streams_and_graphs(K):
         A.compute_q4(q, b.kc, b.vc, out2, pos, heads, kvh, hd, ctx, b.scale, scratch, b.dcos, b.dsin)
     side.synchronize()
     np.testing.assert_array_equal(host(out2), host(out))
+
+
+def test_graphs_that_overlap(K):
+    """Two captured steps (append and attention) with caches and scratch of their own, replayed on two streams at once,
+    again and again."""
+    heads, kvh, hd, ctx, rows = 8, 2, 64, 1200, 2
+    A = K.CachedAttentionKernel
+    steps = []
+    for seed in (37, 41):
+        b = Batch(K, 2, heads, kvh, hd, ctx, [1100, 600], seed=seed)
+        q, k, v = (torch.randn(2, rows, h * hd, device="cuda") for h in (heads, kvh, kvh))
+        pos = dev([1100, 600], torch.int32)
+        scratch = torch.zeros(A.q4_scratch_bytes(2, rows, heads, kvh, hd, ctx), dtype=torch.uint8, device="cuda")
+        kc, vc, want, out = b.kc.clone(), b.vc.clone(), torch.zeros_like(q), torch.zeros_like(q)
+        A.compute_q4(q, kc, vc, want, pos, heads, kvh, hd, ctx, b.scale, scratch, b.dcos, b.dsin, k_new=k, v_new=v)
+        steps.append((b, q, k, v, pos, scratch, out, want, kc, vc, torch.cuda.Stream(), torch.cuda.CUDAGraph()))
+    torch.cuda.synchronize()
+    for b, q, k, v, pos, scratch, out, want, kc, vc, stream, graph in steps:
+        with torch.cuda.graph(graph, stream=stream):
+            A.compute_q4(q, b.kc, b.vc, out, pos, heads, kvh, hd, ctx, b.scale, scratch, b.dcos, b.dsin, k_new=k, v_new=v)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for step in steps:
+            with torch.cuda.stream(step[-2]):
+                step[-1].replay()
+    torch.cuda.synchronize()
+    for b, q, k, v, pos, scratch, out, want, kc, vc, stream, graph in steps:
+        np.testing.assert_array_equal(host(out), host(want))
+        np.testing.assert_array_equal(host(b.kc), host(kc))
+        np.testing.assert_array_equal(host(b.vc), host(vc))
+        assert not scratch[:256].any()
 
 
 # ------------------------------------------------------------------ drafts
