@@ -237,7 +237,7 @@ ovf_status ovf_attention_decode_noalloc(const float *q, const void *k_cache, con
  * real; the others are not read, and their places in an output are left as
  * they are.  A sequence whose rows do not fit max_ctx is left out and sets the
  * error word (ovf_device_error code 4).  Rows are [n_seq][rows][heads *
- * head_dim] fp32, 16-byte aligned; at most 2^22 rows times heads in a call.
+ * head_dim] fp32, 16-byte aligned; rows times heads at most 2^22.
  * Buffers of a call must not overlap; calls on the same cache are ordered by the
  * caller (one stream, or events).
  *
@@ -263,7 +263,8 @@ ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_
  * k_new / v_new (or NULL): rows that are appended first, as ovf_kv_q4_append
  * does.  scratch: ovf_attention_q4_scratch_bytes, 16-byte aligned, the first
  * OVF_Q4_SCRATCH_ZEROS bytes zero (a call leaves them zero), for one call at a
- * time (calls that may overlap, graphs included, need their own). */
+ * time (calls that may overlap, graphs included, need their own).  At most
+ * 2^31 - 1 query rows, heads and blocks of 256 positions multiplied. */
 #define OVF_Q4_EXACT_ROWS 64
 #define OVF_Q4_SCRATCH_ZEROS 256
 int64_t ovf_attention_q4_scratch_bytes(int32_t n_seq, int32_t rows, int32_t n_heads, int32_t n_kv_heads,

@@ -682,10 +682,11 @@ __global__ void __launch_bounds__(HD / 4 * kAqClasses) attention_q4_join_kernel(
     __shared__ float sl[kAqClasses];
     pdl_wait();
     pdl_launch_dependents();
-    const int h = blockIdx.x, r = blockIdx.y, s = blockIdx.z, c0 = threadIdx.x / TC, d = threadIdx.x % TC;
+    const int rows = p.src.rows, c0 = threadIdx.x / TC, d = threadIdx.x % TC;
+    const size_t row = blockIdx.x;
+    const int s = (int)(row / ((size_t)rows * p.H)), r = (int)(row / p.H % rows);
     int chunks;
     if (!aq_join_of(p, s, r, &chunks)) return;
-    const size_t row = ((size_t)s * p.src.rows + r) * p.H + h;
     const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml) + row * p.max_chunks;
     const float4 *part = reinterpret_cast<const float4 *>(p.part) + row * p.max_chunks * TC + d;
     float top = -INFINITY;
@@ -723,8 +724,8 @@ static cudaError_t launch_aq_join(const AqParams &p, cudaStream_t st) {
         return launch_pdl(attention_q4_join_few_kernel<HD>, dim3((unsigned)((threads + kAqJoinThreads - 1) / kAqJoinThreads)),
                           dim3(kAqJoinThreads), 0, st, true, p);
     }
-    return launch_pdl(attention_q4_join_kernel<HD>, dim3(p.H, p.src.rows, p.src.n_seq), dim3(HD / 4 * kAqClasses), 0, st, true,
-                      p);
+    return launch_pdl(attention_q4_join_kernel<HD>, dim3((unsigned)((int64_t)p.src.n_seq * p.src.rows * p.H)),
+                      dim3(HD / 4 * kAqClasses), 0, st, true, p);
 }
 
 static int aq_max_chunks(int max_ctx) { return (max_ctx + kAqLeaf - 1) / kAqLeaf; }
@@ -845,6 +846,10 @@ ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_n
     if (n_seq == 0 || rows == 0) return OVF_OK;
     OVF_CHECK_ARG((int64_t)rows * n_heads <= (1 << 22), "attention_q4: %d rows of %d heads in one call (at most 2^22 in all)",
                   rows, n_heads);
+    // (as many partial results as an int counts: more need hundreds of GB of scratch)
+    OVF_CHECK_ARG((int64_t)n_seq * rows * n_heads <= INT32_MAX / aq_max_chunks(max_ctx),
+                  "attention_q4: %d sequences of %d rows of %d heads over %d positions are too many for one call", n_seq, rows,
+                  n_heads, max_ctx);
     const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (k_new) {
         OVF_CHECK_ARG(k_cache != v_cache, "attention_q4: keys and values need caches of their own");

@@ -60,7 +60,8 @@ def test_attention_refusals(lib):
     for bad in (dict(q=None), dict(out=None), dict(scratch=None), dict(kc=None), dict(pos=None), dict(h=0), dict(h=30),
                 dict(h=-8), dict(kvh=0), dict(hd=80), dict(rows=65), dict(ctx=0), dict(out=P), dict(q=C.c_void_p(4)),
                 dict(scratch=C.c_void_p(8)), dict(out=C.c_void_p(20)), dict(cos=P), dict(kn=P), dict(vn=P),
-                dict(kn=P, vn=P, vc=P), dict(n=-1)):
+                dict(kn=P, vn=P, vc=P), dict(n=-1), dict(n=70000), dict(h=65536 * 8), dict(rows=1 << 18, ctx=1 << 18),
+                dict(n=65535, rows=1 << 10, ctx=1 << 10), dict(n=2, rows=1 << 18, h=8, hd=256, ctx=1 << 20)):
         assert call(**bad) == _lib.OVF_EINVAL, bad
     assert call(n=0) == _lib.OVF_OK and call(rows=0) == _lib.OVF_OK
     assert b"" != lib.ovf_last_error()
