@@ -265,7 +265,7 @@ ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_
  * OVF_Q4_SCRATCH_ZEROS bytes zero (a call leaves them zero), for one call at a
  * time (calls that may overlap, graphs included, need their own).  At most
  * 2^31 - 1 query rows, heads and blocks of 256 positions multiplied. */
-#define OVF_Q4_EXACT_ROWS 64
+#define OVF_Q4_EXACT_ROWS 16
 #define OVF_Q4_SCRATCH_ZEROS 256
 int64_t ovf_attention_q4_scratch_bytes(int32_t n_seq, int32_t rows, int32_t n_heads, int32_t n_kv_heads,
                                        int32_t head_dim, int32_t max_ctx);

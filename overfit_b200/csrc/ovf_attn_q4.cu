@@ -734,12 +734,13 @@ int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx) {
     return 4 * kAqCounters + (int64_t)4 * n_seq * rows * H * aq_max_chunks(max_ctx) * (hd + 2);
 }
 
-// Scratch of launch_attention_q4_rows for up to `rows` rows, `few` at a time where they are few.
+// Scratch of launch_attention_q4_rows for up to `rows` rows, `few` at a time where they go to attention_q4_kernel.
 int64_t attn_q4_rows_scratch_bytes(int rows, int few, int H, int KVH, int hd, int max_ctx, int sms) {
     int64_t most = attn_q4_scratch_bytes(1, std::min(rows, few), H, hd, max_ctx);
-    for (int r = OVF_Q4_EXACT_ROWS + 1; r <= rows; ++r)
-        if (attn_q4_many_rows(r, hd))
-            most = std::max(most, 4 * kAqCounters + (int64_t)4 * r * H * attn_q4_rows_splits(1, r, H, KVH, max_ctx, sms) * (hd + 2));
+    for (int r = OVF_Q4_EXACT_ROWS + 1; r <= rows && hd <= 128; ++r)
+        most = std::max(most, attn_q4_many_rows(1, r, H, KVH, hd, max_ctx, sms)
+                                  ? 4 * kAqCounters + (int64_t)4 * r * H * attn_q4_rows_splits(1, r, H, KVH, max_ctx, sms) * (hd + 2)
+                                  : attn_q4_scratch_bytes(1, r, H, hd, max_ctx));
     return most;
 }
 
@@ -785,8 +786,9 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
     p.part = static_cast<float *>(scratch) + kAqCounters;
     p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.max_chunks * hd;
     cudaError_t e = cudaSuccess;
-    if (attn_q4_many_rows(src.rows, hd)) {
-        p.splits = attn_q4_rows_splits(src.n_seq, src.rows, H, src.KVH, src.max_ctx, sm_count(current_device()));
+    const int sms = sm_count(current_device());
+    if (attn_q4_many_rows(src.n_seq, src.rows, H, src.KVH, hd, src.max_ctx, sms)) {
+        p.splits = attn_q4_rows_splits(src.n_seq, src.rows, H, src.KVH, src.max_ctx, sms);
         p.max_chunks = p.splits;
         p.part_ml = p.part + (size_t)src.n_seq * src.rows * H * p.splits * hd;
         const ArParams a{src, H, q, out, p.part, p.part_ml, p.scale2, p.splits};
@@ -804,8 +806,8 @@ ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *
 }
 
 ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
-                                    void *scratch, int scratch_rows, cudaStream_t st) {
-    if (attn_q4_many_rows(src.rows, hd)) return launch_attention_q4(src, H, hd, q, out, scale, scratch, st, false);
+                                    void *scratch, int scratch_rows, bool exact, cudaStream_t st) {
+    if (!exact && hd <= 128) return launch_attention_q4(src, H, hd, q, out, scale, scratch, st, false);
     for (int r = 0; r < src.rows; r += scratch_rows) {
         Q4Source part = src;
         part.pos0 = src.pos0 + r;

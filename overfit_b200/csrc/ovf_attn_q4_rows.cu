@@ -45,7 +45,7 @@ static constexpr int kArExpand = 8;      // expanding warps
 static constexpr int kArMma = 8 + kArExpand;
 static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
-static constexpr int kArWindow = 4;      // tiles that one accumulator in TMEM sums (a power of 2)
+static constexpr int kArWindow = 2;      // tiles that one accumulator in TMEM sums (a power of 2)
 static constexpr float kArLift = 6.0f;  // weights times 2^6
 static constexpr float kArSlack = 8.0f; // the maximum is raised when it is passed by 2^8
 
@@ -597,9 +597,15 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     }
 }
 
-// Whether rows of this shape are for attention_q4_rows_kernel (more than
-// OVF_Q4_EXACT_ROWS of them; its accumulators fill TMEM at head_dim 128).
-bool attn_q4_many_rows(int rows, int hd) { return rows > OVF_Q4_EXACT_ROWS && hd <= 128; }
+// Whether a call is for attention_q4_rows_kernel: more than OVF_Q4_EXACT_ROWS rows (its accumulators fill TMEM at
+// head_dim 128), and more chunks of 8 query rows than attention_q4_kernel has CTAs under way, 2 a SM.  That kernel's
+// time goes with their number; this one needs 13 us for the first.  (17, 32 and 64 rows of 32 heads over 8, 128 wide,
+// in 4 sequences of 4096 positions: 84, 144 and 280 us there, 30, 34 and 54 us here; 17 rows of 14 heads over 2, 64
+// wide, in one of 2048, 240 chunks: 10.8 and 14.2 us; 32 rows, 448 chunks: 16.0 and 14.6 us.)
+bool attn_q4_many_rows(int n_seq, int rows, int H, int KVH, int hd, int max_ctx, int sms) {
+    const int64_t chunks = ((int64_t)rows * (H / KVH) + 7) / 8 * ((max_ctx + 255) / 256);
+    return rows > OVF_Q4_EXACT_ROWS && hd <= 128 && chunks * KVH * n_seq > 2 * sms;
+}
 
 // Splits of a row's tiles: as many as give each SM a CTA, no more than there are places for partial results.
 int attn_q4_rows_splits(int n_seq, int rows, int H, int KVH, int max_ctx, int sms) {

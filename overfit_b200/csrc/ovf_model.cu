@@ -265,7 +265,8 @@ Q4Source q4_of(const ovf_session *s, int layer, int rows, int pos0, const int *p
     q.KVH = s->m->kvh_loc;
     return q;
 }
-constexpr int kQ4ScratchRows = 16;  // rows at a time of a 4-bit session's small batches: bounds the scratch of a long context
+// rows at a time of a 4-bit session's verify: each gets a decode step's results, and a long context's scratch stays small
+constexpr int kQ4ScratchRows = OVF_Q4_EXACT_ROWS;
 
 // Uploads an f32 vector (norm / bias).
 ovf_status upload_vec(ovf_model *m, const ovf_tensor &t, int64_t n, float **out, const char *what) {
@@ -1108,7 +1109,7 @@ ovf_status enqueue_prefill_batched(ovf_session *s, int n, bool all_rows = false)
                 const Q4Source src = q4_of(s, l, M, base + r0, nullptr);
                 if ((r = launch_kv_q4_append(src, hd, s->pk, s->pv, st, false))) return r;
                 if ((r = launch_attention_q4_rows(src, H, hd, s->pq, s->patt, 1.0f / sqrtf((float)hd), s->q4_rows_scratch,
-                                                  kQ4ScratchRows, st)))
+                                                  kQ4ScratchRows, all_rows, st)))
                     return r;
             } else {
                 // every row's key and value are appended first, then one launch

@@ -163,11 +163,12 @@ ovf_status launch_kv_q4_read(const Q4Source &src, int hd, float *k, float *v, cu
 int64_t attn_q4_scratch_bytes(int n_seq, int rows, int H, int hd, int max_ctx);
 ovf_status launch_attention_q4(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
                                void *scratch, cudaStream_t st, bool pdl);
-// Rows of one sequence at pos0 ..; up to OVF_Q4_EXACT_ROWS of them `scratch_rows`
-// at a time (the same results, bit for bit), so that a long context's scratch
-// (attn_q4_rows_scratch_bytes) stays small.
+// Rows of one sequence at pos0 ..; `exact`, or at head_dim 256, `scratch_rows`
+// (OVF_Q4_EXACT_ROWS at most) at a time, so that they get the results of single
+// rows, bit for bit, and a long context's scratch (attn_q4_rows_scratch_bytes)
+// stays small.
 int64_t attn_q4_rows_scratch_bytes(int rows, int few, int H, int KVH, int hd, int max_ctx, int sms);
 ovf_status launch_attention_q4_rows(const Q4Source &src, int H, int hd, const float *q, float *out, float scale,
-                                    void *scratch, int scratch_rows, cudaStream_t st);
+                                    void *scratch, int scratch_rows, bool exact, cudaStream_t st);
 
 }  // namespace ovf
