@@ -18,10 +18,10 @@
 // large came out 1.9e-6 off, now 3.9e-7 (an fp32 softmax: 5.5e-7).  The shorter chains
 // take a token of 32 heads at 2048 positions from 9.9 to 9.5 us, the additions 64
 // sessions of 8192 from 93 to 96.
-// Queries are scaled by a power of two into fp16's range,
-// weights by 2^14, both exactly.  (With the query as the 16-row operand, 8 rows
-// times hi and lo, a decode step of 4 heads a KV head left half of it empty: 1037
-// instructions a tile of 32 positions and warp, now about half.)
+// Queries are scaled by a power of two into fp16's range, weights by 2^14, both
+// exactly.  (With the query as the 16-row operand, 8 rows times hi and lo, a decode
+// step of 4 heads a KV head left half of it empty: 1037 instructions a tile of 32
+// positions and warp, now about half.)
 //
 // Work is cut into chunks of 256 positions (512 in caches of more than 4096,
 // where joining less outweighs a shorter chunk's latency).  A CTA's four warps
@@ -33,6 +33,9 @@
 // in the call, bit for bit.  CTAs stay resident and take equal runs of the chunks
 // of all sequences, so that unequal lengths cost nothing; a warp's next keys load
 // while it weights values, and its next values while it scores.
+// Measured, 32 heads over 8, 128 wide: one token at 2048 positions 9.5 us (latency);
+// 64 sessions of up to 8192, 96 us, 3.94 TB/s (60 % of the copy rate), bound by
+// instructions (2.4 of 4 a clock; half of the integer pipe takes codes apart).
 #include "ovf_attn_q4_rows.cu"
 #include "ovf_q4.cuh"
 

@@ -12,9 +12,10 @@
 // The tensor cores cut an accumulator's lower bits off at each addition, toward zero,
 // so that a long sum falls short (measured: 3e-7 of O per 128 positions, 1.9e-5 at
 // 8192), where fp32's rounding would average out.  An accumulator in TMEM therefore
-// sums kArWindow tiles at most; the windows are added in fp32 in shared memory.  Four
-// tiles: 1.5e-6 off at any length; eight: 2.7e-6, and 4 % faster.  S takes its small lo
-// products first.
+// sums kArWindow tiles at most; the windows are added in fp32 in shared memory.  Two tiles:
+// 1.2e-6 off at 8192 positions (a plain fp32 softmax 2.1e-6), four: 1.7e-6 and 7 %
+// faster; at 1024 positions 0.95e-6 and 1.4e-6 (fp32 1.1e-6), so two.  S takes its
+// small lo products first.
 //
 // The maximum that P refers to is raised only when a row's scores pass it by more
 // than 2^8; until then P is at most 2^(6 + 8 + 1), inside fp16, and O needs no
@@ -31,9 +32,11 @@
 //   8-15   expansion of K and V, two stages each;
 //   16     TMEM allocation, and the thread that issues the MMAs: S of the next
 //          tile before O of this one.
-// Per tile the tensor cores need 1024 clocks (two products each way), shared
-// memory about 1500 (K and V are read twice, written once), the schedulers about
-// 1400 each (7 instructions per score, 15 per eight codes): the design's bound.
+// Per tile at head_dim 128 the tensor cores need 2048 clocks (32 MMAs of 64: two
+// products each way), shared memory about 2000 (K and V read twice and written once,
+// O of a window every other tile), the schedulers about 1400 each (7 instructions per
+// score, 15 per eight codes); 3600 are measured, about half of the tensor cores' time.
+// Single operands would halve their part at the price of an fp16 softmax's precision.
 // No cluster, no multicast; tensor operands are this GPU's own.
 #include "ovf_q4.cuh"
 

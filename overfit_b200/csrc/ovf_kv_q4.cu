@@ -9,7 +9,9 @@
 // block that the rows fill in part keeps the codes of its other positions.  No
 // two warps write the same word.
 // Bound by memory: 4 bytes read and 0.625 written per element (reading back: the
-// other way round).
+// other way round).  Measured, both calls, 8 KV heads of 128: 3.7 us for one row,
+// 4.7 for 256, 65 for eight prompts of 2048 (3.6 TB/s, 55 % of the copy rate: the
+// quantising and packing instructions, half an SM's issue slots, come first).
 #include <algorithm>
 
 #include "ovf_q4.cuh"

@@ -16,13 +16,17 @@
 // a token.  The device does 64 such products a clock and SM, so an exponential of
 // ten of them (a table and a short series) keeps pace with memory.
 //
-// A cluster of 8 or 16 CTAs takes a sequence.  Its warps cut all rows, one behind
+// A cluster of up to 16 CTAs takes a sequence (all 16 while all sequences' fit the
+// SMs at once).  Its warps cut all rows, one behind
 // the other, into equal runs of steps (128 elements), so that a warp meets one or
 // two rows and reduces as often; the partial sums meet in distributed shared
 // memory, and every CTA forms the same decisions.  Where the drawn row's weights
 // are its exponentials, the partial sums serve the drawing too; where a draft's
-// distribution is taken away, the row is passed once more.  For a batch the
-// logits' bytes and the exponentials bound it alike; for one sequence latency does.
+// distribution is taken away, the row is passed once more.
+// Measured: 4 drafts of one sequence over 128256 tokens, 15.0 us (five chained
+// phases: a maximum pass, sums, decisions, search); 32 sequences of 7 drafts over
+// 151936, 77 us, 2.27 TB/s (35 % of the copy rate): the exponentials alone take 16 us
+// of all SMs, the rest is the waits of each phase's loads, with 32 warps an SM.
 #include <float.h>
 
 #include "ovf_internal.cuh"
