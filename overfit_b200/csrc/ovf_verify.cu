@@ -25,7 +25,7 @@
 // distribution is taken away, the row is passed once more.
 // Measured: 4 drafts of one sequence over 128256 tokens, 15.0 us (five chained
 // phases: a maximum pass, sums, decisions, search); 32 sequences of 7 drafts over
-// 151936, 77 us, 2.27 TB/s (35 % of the copy rate): the exponentials alone take 16 us
+// 151936, 78 us, 2.24 TB/s (34 % of the copy rate): the exponentials alone take 16 us
 // of all SMs, the rest is the waits of each phase's loads, with 32 warps an SM.
 #include <float.h>
 
@@ -60,7 +60,19 @@ __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab
 __device__ __forceinline__ double vf_exp0(double x, const unsigned long long *tab) {
     return x < -690.0 ? 0.0 : vf_exp(x, tab);
 }
-__device__ __forceinline__ float vf_floor(float m, float T) { return fmaxf(m - 690.0f * T, -FLT_MAX); }
+// The temperature for a row of largest logit m: at least 2^-31 of |m|.  (The next float is 2^-25 |m| below m or more, so
+// that all that is smaller has a weight below e^-64 at that temperature and at any lower one, which no sum of 2^24 in
+// 64 bits holds; and the floor lies a few floats below m, not on it.)
+__device__ __forceinline__ float vf_temperature(float m, float T) { return fmaxf(T, fabsf(m) * 0x1p-31f); }
+// Logits up to this have no weight: rounded up, so that its own weight stays in vf_exp's range.
+__device__ __forceinline__ float vf_floor(float m, float T) {
+    return fmaxf(__fsub_ru(m, __fmul_rd(690.0f, vf_temperature(m, T))), -FLT_MAX);
+}
+// 1 / the row's temperature, from 1 / T.
+__device__ __forceinline__ double vf_inverse(float m, float T, double inv) {
+    const float t = vf_temperature(m, T);
+    return t == T ? inv : 1.0 / (double)t;
+}
 __device__ __forceinline__ float vf_raise(float x, float floor) {  // the larger; NaN stays NaN
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(floor));
@@ -188,8 +200,8 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
     const int s = blockIdx.x / size, warps = size * kVfWarps, me = rank * kVfWarps + warp;
     const int n = p.counts ? min(p.counts[s], p.max_drafts) : p.max_drafts;
     if (n < 0) return;  // an unused place (all CTAs of the cluster leave)
-    const float T = p.temperatures[s];
-    const bool greedy = !(T > 0.0f);
+    const bool greedy = !(p.temperatures[s] > 0.0f);
+    const float T = fminf(p.temperatures[s], 1e30f);  // (impossible tokens stay impossible)
     const float *u = p.uniforms + (size_t)s * (p.max_drafts + 1);
     const float *logits = p.logits + (size_t)s * (p.max_drafts + 1) * V;
     const double inv = 1.0 / (double)T;
@@ -210,7 +222,8 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
         const unsigned stop = min(run1, (unsigned)(j + 1) * steps);
         const float *x = logits + (size_t)j * V;
         int at = 4 * (32 * (int)(st - j * steps) + lane) - vf_shift(x);
-        float m = -FLT_MAX;
+        float m = -FLT_MAX, floor = -FLT_MAX;
+        double scale = inv;  // 1 / temperature, for that m
         int place = 0x7FFFFFFF;
         double sum = 0.0;
         bool bad = false;
@@ -250,13 +263,14 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
                 if (top > m) {
                     sum *= vf_exp0(((double)m - (double)top) * inv, tab);
                     m = top;
+                    floor = vf_floor(m, T);
+                    scale = vf_inverse(m, T, inv);
                 }
                 const double md = (double)m;
-                const float floor = vf_floor(m, T);
                 double part[4];
 #pragma unroll
                 for (int i = 0; i < 4 * Steps; ++i) {
-                    const double y = vf_exp(((double)vf_raise(e[i], floor) - md) * inv, tab);
+                    const double y = vf_exp(((double)vf_raise(e[i], floor) - md) * scale, tab);
                     part[i & 3] = i < 4 ? y : part[i & 3] + y;
                 }
                 sum += (part[0] + part[1]) + (part[2] + part[3]);
@@ -345,7 +359,7 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
         row.x = logits + (size_t)k * V;
         row.q = nullptr;
         row.m = (double)sh.row_m[k];
-        row.inv = inv;
+        row.inv = vf_inverse(sh.row_m[k], T, inv);
         row.scale = 1.0;
         row.floor = vf_floor(sh.row_m[k], T);
         row.V = V;

@@ -345,7 +345,7 @@ class CudaLlamaSession:
             raise ValueError("temperature must be positive (generate_speculative is the greedy form)")
         z = self.get_last_logits().astype(np.float64) / temperature
         cum = np.cumsum(np.exp(z - z.max()))
-        t0 = int(np.searchsorted(cum, rng.random() * cum[-1], side="right"))
+        t0 = min(int(np.searchsorted(cum, rng.random() * cum[-1], side="right")), cum.size - 1)
         draft = prompt_lookup_draft(list(history) + [t0], max_draft, ngram_min, ngram_max)
         if not draft or self.current_position + 1 + len(draft) + 1 > self.max_context_length:
             self.decode(t0)

@@ -513,6 +513,34 @@ def test_verify_unusual_rows(K):
     assert run_verify(K, logits, d, u, T, None, counts)[1][1] == -1
 
 
+@pytest.mark.parametrize("with_probs", [False, True])
+def test_verify_of_extreme_temperatures(K, with_probs):
+    """From temperatures at which neighbouring floats are worlds apart (the largest logits, which tie, share everything)
+    to ones at which all tokens are alike; logits of several magnitudes and both signs, some impossible."""
+    rng = np.random.default_rng(11)
+    T = np.array([1e-38, 1e-20, 1e-10, 1e-9, 3e-9, 1e-8, 3e-8, 1e-7, 3e-7, 1e-6, 1e-5, 1e-3, 1e3, 1e10, 1e30], np.float32)
+    n, m, vocab = 4 * T.size, 2, 700
+    T = np.tile(T, 4)
+    logits, q, d, u = drafted(rng, n, m, vocab)
+    logits[:15] += 20
+    logits[15:30] *= 300
+    logits[30:45] -= 150
+    for s in range(n):
+        for j in range(m + 1):
+            order = np.argsort(logits[s, j])
+            top = logits[s, j, order[-1]]
+            logits[s, j, order[-4:-1]] = top
+            for i, k in enumerate(order[-8:-4]):  # the next floats below
+                logits[s, j, k] = np.nextafter(logits[s, j, order[-4 - i]], np.float32(-np.inf))
+            logits[s, j, order[:5]] = -np.inf
+            logits[s, j, order[5:9]] = -np.finfo(np.float32).max
+            if j < m and rng.random() < 0.7:
+                d[s, j] = order[-1 - rng.integers(0, 3)]
+    a, t = run_verify(K, logits, d, u, T, q if with_probs else None)
+    want = [ref.verify(logits[s], d[s], u[s], T[s], q[s] if with_probs else None, m) for s in range(n)]
+    np.testing.assert_array_equal(np.stack([a, t], 1), want)
+
+
 def test_verify_at_its_borders(K):
     """u q against p where they are equal but for the last bits, and a cumulative sum that meets its target."""
     vocab, T = 4, 1.0
