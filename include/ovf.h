@@ -291,7 +291,8 @@ ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_n
  * row's first maximum, and the next token is that maximum), more than 1e30 is
  * 1e30.  Logits of -infinity or of the lowest float are impossible tokens; a
  * row that has no others, or a NaN or +infinity, accepts nothing and gives
- * token -1.  A draft outside the vocabulary is rejected.  draft_counts [n_seq] or NULL (max_drafts each): negative marks an
+ * token -1.  A draft outside the vocabulary is rejected.  draft_counts [n_seq]
+ * or NULL (max_drafts each): negative marks an
  * unused place, whose results are left as they are.
  * accepted [n_seq]: drafts accepted; next_token [n_seq].  max_drafts 0 samples
  * plainly.  Probabilities and sums are formed in 64 bits. */
