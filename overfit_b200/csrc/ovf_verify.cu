@@ -16,8 +16,8 @@
 // a token.  The device does 64 such products a clock and SM, so an exponential of
 // ten of them (a table and a short series) keeps pace with memory.
 //
-// A cluster of up to 16 CTAs takes a sequence (all 16 while all sequences' fit the
-// SMs at once).  Its warps cut all rows, one behind
+// A cluster of up to 16 CTAs takes a sequence, as many as let all sequences' run at
+// once.  Its warps cut all rows, one behind
 // the other, into equal runs of steps (128 elements), so that a warp meets one or
 // two rows and reduces as often; the partial sums meet in distributed shared
 // memory, and every CTA forms the same decisions.  Where the drawn row's weights
@@ -522,40 +522,63 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
 }
 
 template <int Steps, int Ctas>
-static cudaError_t launch_vf(const VerifyParams &p, int n_seq, int cluster, cudaStream_t st) {
+static void vf_config(int n_seq, int cluster, cudaStream_t st, cudaLaunchAttribute *attr, cudaLaunchConfig_t *cfg) {
+    *cfg = {};
+    cfg->gridDim = dim3(n_seq * cluster);
+    cfg->blockDim = dim3(kVfThreads);
+    cfg->dynamicSmemBytes = sizeof(VfShared);
+    cfg->stream = st;
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = cluster;
+    attr->val.clusterDim.y = attr->val.clusterDim.z = 1;
+    cfg->attrs = attr;
+    cfg->numAttrs = 1;
+}
+
+// Prepares the kernel on this device, and gives how many of its clusters of 1 to kVfCluster CTAs run there at once.
+template <int Steps, int Ctas>
+static cudaError_t vf_prepare(const int **fit) {
     static PerDeviceOnce once;
-    const int dev = current_device();
+    static int fits[65][kVfCluster + 1];  // (the last for a device that PerDeviceOnce does not keep)
+    const int dev = current_device(), at = dev >= 0 && dev < 64 ? dev : 64;
     const auto kernel = verify_drafts_kernel<Steps, Ctas>;
     if (once.pending(dev)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(VfShared));
+        for (int c = 1; c <= kVfCluster && e == cudaSuccess; ++c) {
+            cudaLaunchAttribute attr[1];
+            cudaLaunchConfig_t cfg;
+            vf_config<Steps, Ctas>(1, c, nullptr, attr, &cfg);
+            e = cudaOccupancyMaxActiveClusters(&fits[at][c], kernel, &cfg);
+        }
         if (e != cudaSuccess) return e;
         once.mark(dev);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(n_seq * cluster);
-    cfg.blockDim = dim3(kVfThreads);
-    cfg.dynamicSmemBytes = sizeof(VfShared);
-    cfg.stream = st;
+    *fit = fits[at];
+    return cudaSuccess;
+}
+
+template <int Steps, int Ctas>
+static cudaError_t launch_vf(const VerifyParams &p, int n_seq, int cluster, cudaStream_t st) {
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    cudaLaunchConfig_t cfg;
+    vf_config<Steps, Ctas>(n_seq, cluster, st, attr, &cfg);
+    return cudaLaunchKernelEx(&cfg, verify_drafts_kernel<Steps, Ctas>, p);
 }
 
 ovf_status launch_verify_drafts(const VerifyParams &p, int n_seq, cudaStream_t st) {
-    // Where every CTA of 16-CTA clusters has an SM for itself, those, with more loads a lane; else the largest clusters
-    // of which all sequences' run at once, two CTAs an SM (42 sequences of 4 x 25276 logits: 34.5 us in clusters of 8,
-    // of which only 37 fit, 25.7 in clusters of 4; 32 of 8 x 151936: 77.0 in clusters of 8, 85.7 in clusters of 4).
-    const int sms = sm_count(current_device());
-    int cluster = 8;
-    while (cluster > 1 && n_seq * cluster > 2 * sms) cluster /= 2;
-    const cudaError_t e = n_seq * kVfCluster <= sms ? launch_vf<4, 1>(p, n_seq, kVfCluster, st)
-                                                    : launch_vf<2, 2>(p, n_seq, cluster, st);
+    const int *alone, *shared;
+    cudaError_t e = vf_prepare<4, 1>(&alone);
+    if (e == cudaSuccess) e = vf_prepare<2, 2>(&shared);
+    if (e != cudaSuccess) return cuda_status(e, "verify_drafts");
+    // Clusters of 16 with an SM a CTA and more loads a lane, if all sequences' run at once; else the largest of which all
+    // do, two CTAs an SM.  (A cluster stays within a group of SMs, so that fewer run than the SMs have room for; the
+    // largest power of two for which these would do took 29.5 us for 8 sequences of 5 x 128256 logits, now 22.8, and
+    // 45.0 for 36 of 8 x 50000, now 35.0.)
+    int cluster = kVfCluster;
+    while (cluster > 1 && shared[cluster] < n_seq) --cluster;
+    e = alone[kVfCluster] >= n_seq ? launch_vf<4, 1>(p, n_seq, kVfCluster, st) : launch_vf<2, 2>(p, n_seq, cluster, st);
     return cuda_status(e, "verify_drafts");
 }
 
