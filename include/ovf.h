@@ -52,7 +52,12 @@ typedef int32_t ovf_status;
 /* ---------------------------------------------------------------- misc */
 const char *ovf_last_error(void);
 int32_t ovf_version(void);
-/* Reads and clears the device-side error word that bounded waits set. */
+/* Reads and clears what kernels reported on the device: 1 to 3, a bounded wait
+ * gave up (a session call that ends takes these itself and returns
+ * OVF_ETIMEDOUT); 4, a position or row count that the caller of a kernel-level
+ * entry point has in device memory does not fit its cache (session calls leave
+ * this one alone).  Where both stand, the first call gives the wait's code and the
+ * next one 4. */
 ovf_status ovf_device_error(int32_t device, int32_t *code_out);
 
 /* ---------------------------------------------------- activation quantizers */
@@ -235,8 +240,8 @@ ovf_status ovf_attention_decode_noalloc(const float *q, const void *k_cache, con
  * negative marks an unused place, for which nothing is read or written.
  * row_counts (device, n_seq, or NULL for all): how many of its `rows` are
  * real; the others are not read, and their places in an output are left as
- * they are.  A sequence whose rows do not fit max_ctx is left out and sets the
- * error word (ovf_device_error code 4).  Rows are [n_seq][rows][heads *
+ * they are.  A sequence whose rows do not fit max_ctx is left out and reported
+ * by ovf_device_error (code 4).  Rows are [n_seq][rows][heads *
  * head_dim] fp32, 16-byte aligned; rows times heads at most 2^22.
  * Buffers of a call must not overlap; calls on the same cache are ordered by the
  * caller (one stream, or events).

@@ -42,8 +42,14 @@ ovf_status ovf_device_error(int32_t device, int32_t *code_out) {
     OVF_CUDA_TRY(cudaGetDevice(&prev));
     OVF_CUDA_TRY(cudaSetDevice(device));
     int code = 0, zero = 0;
+    // the library's own error first; a caller's is given by the next call then
     cudaError_t e = cudaMemcpyFromSymbol(&code, g_dev_error, sizeof(int));
-    if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int));
+    if (e == cudaSuccess && code != 0) {
+        e = cudaMemcpyToSymbol(g_dev_error, &zero, sizeof(int));
+    } else if (e == cudaSuccess) {
+        e = cudaMemcpyFromSymbol(&code, g_caller_error, sizeof(int));
+        if (e == cudaSuccess && code != 0) e = cudaMemcpyToSymbol(g_caller_error, &zero, sizeof(int));
+    }
     cudaSetDevice(prev);
     if (e != cudaSuccess) return cuda_status(e, "ovf_device_error");
     *code_out = code;

@@ -53,8 +53,11 @@ ovf_status cuda_status(cudaError_t e, const char *what);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Device-side error word (per device, per library instance).  Kernels set it
-// when a bounded wait gives up; the host reads it with ovf_device_error.
+// Device-side error words (per device, per library instance).  Kernels set
+// g_dev_error when a bounded wait gives up: the session call that ends next
+// takes it, or ovf_device_error.  What a kernel-level caller's own data in device
+// memory does wrong goes to g_caller_error, which ovf_device_error alone takes: a
+// session that shares the device neither fails for it nor clears it.
 enum : int {
     DEVERR_NONE = 0,
     DEVERR_MBAR_TIMEOUT = 1,
@@ -64,8 +67,10 @@ enum : int {
 };
 // Defined once: the library is a single translation unit (csrc/ovf_lib.cu).
 __device__ int g_dev_error = 0;
+__device__ int g_caller_error = 0;
 
 __device__ __forceinline__ void raise_dev_error(int code) { atomicCAS(&g_dev_error, 0, code); }
+__device__ __forceinline__ void raise_caller_error(int code) { atomicCAS(&g_caller_error, 0, code); }
 
 // --------------------------------------------------------- PTX wrappers
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {

@@ -305,6 +305,7 @@ ovf_status q4_source(const char *what, const void *k_cache, const void *v_cache,
     s.rows = rows;
     s.n_seq = n_seq;
     s.KVH = n_kv_heads;
+    s.callers = true;
     *src = s;
     return OVF_OK;
 }

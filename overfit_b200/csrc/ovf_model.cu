@@ -1760,13 +1760,18 @@ int32_t ovf_session_position(const ovf_session *s) { return s ? s->pos : -1; }
 
 // Ends a synchronous call: moves the device error word into `slot` (read and
 // cleared in one atomic step, after the call's kernels), waits for the stream
-// and reports a bounded wait that gave up as OVF_ETIMEDOUT.
+// and reports a bounded wait that gave up as OVF_ETIMEDOUT.  (What a kernel-level
+// caller's data did wrong meanwhile lies in another word.)
 static ovf_status finish_call(cudaStream_t st, int *slot) {
     ovf_status r = launch_take_error(slot, st);
     if (r) return r;
     int code = 0;
     OVF_CUDA_TRY(cudaMemcpyAsync(&code, slot, sizeof(int), cudaMemcpyDeviceToHost, st));
     OVF_CUDA_TRY(cudaStreamSynchronize(st));
+    if (code == DEVERR_POSITION) {
+        set_error("a row's position does not fit its session's cache (code %d)", code);
+        return OVF_ESTATE;
+    }
     if (code) {
         set_error("device wait timed out (code %d)", code);
         return OVF_ETIMEDOUT;

@@ -114,6 +114,7 @@ struct Q4Source {
     const int32_t *positions, *counts;
     const float *cos, *sin;  // [max_ctx][hd / 2] or null
     int split_half, max_ctx, rows, n_seq, KVH, pos0;
+    bool callers;  // positions and counts are a kernel-level caller's data
 };
 
 struct Q4View {
@@ -123,7 +124,8 @@ struct Q4View {
 };
 
 // Sequence s; false if nothing is to be done for it.  Rows that do not fit
-// the cache set the error word and are left out.
+// the cache set the caller's error word (a session's, which the host has checked,
+// the library's own) and are left out.
 __device__ __forceinline__ bool q4_view(const Q4Source &p, int s, Q4View *w) {
     int max_ctx = p.max_ctx;
     if (p.seqs) {
@@ -145,7 +147,8 @@ __device__ __forceinline__ bool q4_view(const Q4Source &p, int s, Q4View *w) {
     w->count = p.counts ? min(max(p.counts[s], 0), p.rows) : p.rows;
     if (w->pos < 0 || w->count == 0) return false;
     if (w->pos > max_ctx - w->count) {
-        raise_dev_error(DEVERR_POSITION);
+        if (p.callers) raise_caller_error(DEVERR_POSITION);
+        else raise_dev_error(DEVERR_POSITION);
         return false;
     }
     return true;
