@@ -525,7 +525,9 @@ __global__ void __launch_bounds__(kAqThreads, Fused ? 2 : AqShape<NG, NT>::kCtas
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, s[nt][tile][i]);
 #pragma unroll
                 for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
-                const float zero = top == -INFINITY ? 0.0f : top, base = zero - kAqLift;  // (nothing attended: weights of 0)
+                // (nothing attended: weights of 0.  Rounded up, so that no weight passes 2^14: with scores of 2^25 and more
+                // the nearest float to top - 14 may lie 16 below top, whose weight of 2^16 fp16 does not hold)
+                const float zero = top == -INFINITY ? 0.0f : top, base = __fsub_ru(zero, kAqLift);
                 if (leaf > 0) {
                     const float keep = ex2(m[nt] - zero);
                     l[nt] *= keep;

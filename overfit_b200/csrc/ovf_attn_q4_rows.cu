@@ -18,8 +18,9 @@
 // small lo products first.
 //
 // The maximum that P refers to is raised only when a row's scores pass it by more
-// than 2^8; until then P is at most 2^(6 + 8 + 1), inside fp16, and O needs no
-// rescaling.  Weights are held times 2^6.
+// than 2^8; until then P is at most 2^(6 + 8), inside fp16, and O needs no
+// rescaling.  Weights are held times 2^6.  (Both steps from the maximum are rounded
+// so that the bound holds for scores of 2^24 and more, between whose floats lie more.)
 //
 // Codes lie in the pairs that their expansion yields: eight elements come out as
 // 0 4 1 5 2 6 3 7, along dimensions for K and along positions for V.  Q's columns
@@ -306,12 +307,12 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             *mine = top;
             ar_pair_sync(warp & 3);
             top = fmaxf(top, xch[(i & 1) * 2 * kArM + (half ^ 1) * kArM + row]);
-            const float m_before = m;
+            const float m_before = m, most = __fadd_rd(m, kArSlack);
             if (fresh) {
-                if (top > m + kArSlack || m == -INFINITY) m = top;
+                if (top > most || m == -INFINITY) m = top;
                 l *= m_before == m ? 1.0f : ex2(m_before - m);
             } else {
-                const bool raise = top > m + kArSlack || (m == -INFINITY && top > m);
+                const bool raise = top > most || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, raise)) {
                     // O so far, to the new maximum (this half of its columns)
                     wait(o_done, (i - 1) & 1);
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                     tmem_st_wait();
                 }
             }
-            const float base = (m == -INFINITY ? 0.0f : m) - kArLift;
+            const float base = __fsub_ru(m == -INFINITY ? 0.0f : m, kArLift);
             float2 sum = make_float2(0.0f, 0.0f);
             const float2 factor2 = make_float2(factor, factor), base2 = make_float2(-base, -base);
             // (P of 16 columns goes where those scores were: 8 columns of hi, 8 of lo parts)
