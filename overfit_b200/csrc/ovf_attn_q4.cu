@@ -47,7 +47,7 @@ static constexpr int kAqLeaf = 256;                // positions that the warps t
 static constexpr int kAqCounters = 64;             // ints at the start of the scratch, zero between calls
 static_assert(4 * kAqCounters == OVF_Q4_SCRATCH_ZEROS, "what a call finds zero and leaves zero");
 static constexpr int kAqWideTiles = 128;           // caches of more tiles have chunks of two leaves
-static constexpr float kAqLift = 14.0f;            // weights are held times 2^14: lo parts stay normal fp16 numbers
+static constexpr float kAqLift = 14.0f;            // weights are held times 2^14: a weight is off by 2^-22 of itself, or 2^-39 of the largest
 static_assert(kAqLeaf == kAqWarps * 2 * kQ4Tile, "two tiles a warp");
 
 // A call's shape in the template: NG groups of 32 dimensions, NT operands of 4

@@ -6,8 +6,8 @@
 //     S = Q K^T,  P = 2^(S - max),  O += P V,
 // Q, S, P and O in TMEM (Q and P as the left operand, from TMEM), K and V expanded
 // from their codes into shared memory in the UMMA layout.  As there, an fp32
-// operand enters as two fp16 numbers (hi + lo, 22 bits), here as two products into
-// one accumulator, and the cached values are fp16 numbers by definition.
+// operand enters as two fp16 numbers (hi + lo, 22 bits; small weights fewer, see below),
+// here as two products into one accumulator, and the cached values are fp16 numbers by definition.
 //
 // The tensor cores cut an accumulator's lower bits off at each addition, toward zero,
 // so that a long sum falls short (measured: 3e-7 of O per 128 positions, 1.9e-5 at
@@ -17,10 +17,16 @@
 // faster; at 1024 positions 0.95e-6 and 1.4e-6 (fp32 1.1e-6), so two.  S takes its
 // small lo products first.
 //
-// The maximum that P refers to is raised only when a row's scores pass it by more
-// than 2^8; until then P is at most 2^(6 + 8), inside fp16, and O needs no
-// rescaling.  Weights are held times 2^6.  (Both steps from the maximum are rounded
-// so that the bound holds for scores of 2^24 and more, between whose floats lie more.)
+// The maximum that P refers to is raised at each window's first tile, where O begins
+// anew, and inside a window only when a row's scores pass it by more than 2^3.5; until
+// then P is at most 2^(12 + 3.5), inside fp16, and O needs no rescaling.  (Both steps
+// from the maximum are rounded so that the bound holds for scores of 2^24 and more,
+// between whose floats lie more.)  Weights are held times 2^12, so that fp16's
+// smallest step is 2^-36 of the maximum's: what smaller weights lose is at most
+// 2^-37 a position, 1e-6 of the values at 131072 of them (with 2^6, and 2^8 in place of
+// 2^3.5, 6e-5, in all of one sign under a long flat tail; 1 % faster.  2^14 and 2^1.5
+// rescale so often that they take 4 % longer).  Weights are summed in two steps, of 16
+// tiles and of those sums, for the same reason.
 //
 // Codes lie in the pairs that their expansion yields: eight elements come out as
 // 0 4 1 5 2 6 3 7, along dimensions for K and along positions for V.  Q's columns
@@ -50,8 +56,9 @@ static constexpr int kArMma = 8 + kArExpand;
 static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
 static constexpr int kArWindow = 2;      // tiles that one accumulator in TMEM sums (a power of 2)
-static constexpr float kArLift = 6.0f;  // weights times 2^6
-static constexpr float kArSlack = 8.0f; // the maximum is raised when it is passed by 2^8
+static constexpr int kArSums = 16;      // tiles whose weights are summed before they are added to the others' (a power of 2)
+static constexpr float kArLift = 12.0f;  // weights times 2^12
+static constexpr float kArSlack = 3.5f;  // inside a window the maximum is raised when it is passed by 2^3.5
 
 template <int NG>
 struct ArSmem {
@@ -272,7 +279,8 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
     auto wait = [&](uint64_t *bar, int parity) { ok = ok && mbar_wait_bounded(bar, (uint32_t)parity); };
     if (warp < 8) {
         // ------------------------------------------------------- softmax
-        float m = -INFINITY, l = 0.0f, m_acc = -INFINITY;  // m_acc: what O of the earlier windows refers to
+        // l: the sum of the weights of up to kArSums tiles, l_acc: of those before; m_acc: what O of the earlier windows refers to
+        float m = -INFINITY, l = 0.0f, l_acc = 0.0f, m_acc = -INFINITY;
         float4 *acc = reinterpret_cast<float4 *>(sm + SM::acc_off) + half * (HD / 8) * kArM + row;
         for (int i = 0; i < nt; ++i) {
             const bool fresh = (i & (kArWindow - 1)) == 0;  // O begins anew with this tile
@@ -309,8 +317,14 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             top = fmaxf(top, xch[(i & 1) * 2 * kArM + (half ^ 1) * kArM + row]);
             const float m_before = m, most = __fadd_rd(m, kArSlack);
             if (fresh) {
-                if (top > most || m == -INFINITY) m = top;
-                l *= m_before == m ? 1.0f : ex2(m_before - m);
+                m = fmaxf(m, top);
+                if ((i & (kArSums - 1)) == 0) {
+                    l_acc += l;
+                    l = 0.0f;
+                }
+                const float k = m_before == m ? 1.0f : ex2(m_before - m);
+                l *= k;
+                l_acc *= k;
             } else {
                 const bool raise = top > most || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, raise)) {
@@ -319,6 +333,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
                     tc_fence_after();
                     const float k = raise ? ex2(m - top) : 1.0f;
                     l *= k;
+                    l_acc *= k;
                     if (raise) m = top;
 #pragma unroll
                     for (int c = 0; c < HD / 2; c += 16) {
@@ -387,6 +402,7 @@ __global__ void __launch_bounds__(kArThreads, 1) attention_q4_rows_kernel(const 
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[i & 1]);
         }
+        l += l_acc;
         // the rows' results (the slot of the last tile but one: its readers have passed a barrier since)
         xch[(nt & 1) * 2 * kArM + half * kArM + row] = l;
         wait(o_done, (nt - 1) & 1);

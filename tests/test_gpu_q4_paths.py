@@ -98,6 +98,33 @@ def normal(seed, *shape):
     return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
 
 
+# --------------------------------------------- attention_q4_rows_kernel
+@pytest.mark.parametrize("far", [26, 30, 31, 33, 36, 37])
+def test_one_large_weight_and_a_long_flat_tail(K, far):
+    """One position outweighs each of 65535 others by about 2^far: alone they are nothing, together 2^(16 - far) of the
+    output.  The others' keys are zero, so that their scores are, exactly, and the output is (T - 1) / (T + 1), of
+    values -1 and 1 and a tail T below 2^-9 that is off by less than 2^-16 of itself (the score's error).  The tensor cores cut
+    O by less than 2^-23 at each of the 32 additions of a window, and each of the 256 windows is added in fp32, off by
+    half a step of numbers below 1, 2^-25.  Weights are summed over 16 of the 512 tiles, these 32 sums to one, each
+    addition off by half a step of numbers above 1, 2^-24."""
+    ctx, rows, heads, kvh, hd = 65536, 320, 32, 4, 64
+    k, v = torch.zeros(1, ctx, kvh, hd, device="cuda"), torch.ones(1, ctx, kvh, hd, device="cuda")
+    k[:, 0], v[:, 0] = 2.0, -1.0
+    b = Long(K, k, v, heads)
+    assert (b.k[:, 1:] == 0).all() and (b.k[:, 0] > 1.9).all() and (b.v[:, 0] == -1).all() and (b.v[:, 1:] == 1).all()
+    # weights of 2^-0.9 times 2^-far: just below half a step where 2^-far is one
+    q = torch.full((1, rows, heads, hd), (far + 1.1) * np.log(2) / (b.k[0, 0, 0].sum().item() * hd ** -0.5), device="cuda")
+    got, scratch = b.run(q, [ctx - rows])
+    assert splits_of(scratch, 1, rows, heads, hd, ctx) == 1
+    for r in (0, 150, 319):
+        z, _ = b.scores(q, 0, ctx - rows, [r])
+        tail = (z - z.amax(-1, keepdim=True)).exp().sum(-1) - 1
+        assert (tail < 2.0 ** -9).all()
+        want = ((tail - 1) / (tail + 1)).view(1, heads, 1).expand(1, heads, hd)
+        tol = 2.0 ** -24 + 2 * 2.0 ** -9 * 2.0 ** -16 + 32 * 2.0 ** -23 + 256 * 2.0 ** -25 + 48 * 2.0 ** -24
+        torch.testing.assert_close(got[0, r:r + 1].double(), want, rtol=0, atol=tol)
+
+
 # --------------------------------------------- every kernel
 @pytest.mark.parametrize("rows,n", [(1, 2), (6, 2), (200, 4), (200, 8)])
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
