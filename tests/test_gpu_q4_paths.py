@@ -99,6 +99,128 @@ def normal(seed, *shape):
 
 
 # --------------------------------------------- attention_q4_rows_kernel
+# sequences, splits that they leave room for (148 SMs)
+MANY = [(4, "several"), (8, "one")]
+
+
+@pytest.mark.parametrize("n,kind", MANY)
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (8, 2, 64), (8, 2, 32)])
+def test_maxima_that_rise_within_a_window(K, n, kind, heads, kvh, hd):
+    """Keys that grow along the sequence: every tile of 128 passes the maximum of the last by more than 2^8 for most
+    rows, odd tiles (the second of a window) too; then they shrink.  Odd and even numbers of tiles, ends inside a tile."""
+    length, rows = 1500, 200
+    grow = 0.02 + 8.0 * (torch.arange(length, device="cuda") / 1200).clamp(max=1)
+    grow[1300:] *= 0.1
+    # (keys that all point the same way, so that a row's scores rise or fall together)
+    way = normal(hd, 1, 1, kvh, hd)
+    k = (way + 0.1 * normal(hd + 1, n, length, kvh, hd)) * grow[None, :, None, None]
+    b = Long(K, k, normal(hd + 2, n, length, kvh, hd), heads)
+    q = 3 * normal(hd + 3, n, rows, heads, hd) + 2.5 * way.view(1, 1, kvh, 1, hd).expand(n, rows, kvh, heads // kvh,
+                                                                                       hd).reshape(n, rows, heads, hd)
+    z, _ = b.scores(q, 0, 1100 - rows, [rows - 1])
+    top = z[..., :1024].unflatten(-1, (8, 128)).amax(-1) / np.log(2)
+    rise = top.diff(dim=-1)  # of tiles 1 .. 7
+    assert (rise[..., ::2] > 8).double().mean() > 0.5 and (rise[..., 1::2] > 8).double().mean() > 0.5
+    for end in (1500, 1409, 1280, 1100, 300):
+        at = [end - rows - 3 * s for s in range(n)]
+        got, scratch = b.run(q, at)
+        assert (splits_of(scratch, n, rows, heads, hd, b.ctx) > 1) == (kind == "several")
+        b.check(got, q, at, [0, 1, 77, 127, 128, rows - 1])
+
+
+@pytest.mark.parametrize("n,kind", MANY)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_bytes_behind_many_rows_do_not_matter(K, n, kind, hd):
+    """Stale bytes behind the last position (all ones: codes 15, D and M NaN) change no bit."""
+    length, rows, heads, kvh = 1203, 200, 8, 2
+    k, v, q = normal(1, n, length, kvh, hd), normal(2, n, length, kvh, hd), normal(3, n, rows, heads, hd)
+    at = [length - rows] * n
+    got = []
+    for fill in (0, 0xFF):
+        b = Long(K, k, v, heads, fill, ctx=1500)
+        out, scratch = b.run(q, at)
+        assert (splits_of(scratch, n, rows, heads, hd, b.ctx) > 1) == (kind == "several")
+        got.append(out)
+    assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1])
+    b.check(got[0], q, at, [0, 60, 199])
+
+
+@pytest.mark.parametrize("n,kind", MANY)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_a_bad_query_among_many_rows(K, n, kind, hd):
+    """NaN and infinities stay in the rows and heads that have them."""
+    length, rows, heads, kvh = 1300, 200, 8, 2
+    b = Long(K, normal(1, n, length, kvh, hd), normal(2, n, length, kvh, hd), heads)
+    q = normal(3, n, rows, heads, hd)
+    at = [length - rows] * n
+    clean, scratch = b.run(q, at)
+    assert (splits_of(scratch, n, rows, heads, hd, b.ctx) > 1) == (kind == "several")
+    bad = q.clone()
+    bad[0, 3, 1, 5], bad[1, 120, 7, 0], bad[2, 199, 0, 31] = torch.nan, torch.inf, -torch.inf
+    got, _ = b.run(bad, at)
+    hit = torch.zeros(n, rows, heads, dtype=torch.bool, device="cuda")
+    hit[0, 3, 1] = hit[1, 120, 7] = hit[2, 199, 0] = True
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("n,kind", MANY)
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_many_rows_appended_by_the_call(K, n, kind, hd):
+    """k_new / v_new: as an append and then the attention, in caches and output; ragged."""
+    heads, kvh, rows, ctx = 8, 2, 200, 1500
+    b = Long(K, normal(1, n, 1203, kvh, hd), normal(2, n, 1203, kvh, hd), heads, 0xFF, ctx=ctx)
+    k, v, q = (normal(3 + i, n, rows, h * hd) for i, h in enumerate((kvh, kvh, heads)))
+    pos = dev([1203 - 5 * s for s in range(n)], torch.int32)
+    counts = dev([rows - 17 * s for s in range(n)], torch.int32)
+    A = K.CachedAttentionKernel
+    got = []
+    for new in (False, True):
+        kc, vc, out = b.kc.clone(), b.vc.clone(), torch.full((n, rows, heads * hd), 7.0, device="cuda")
+        scratch = torch.full((A.q4_scratch_bytes(n, rows, heads, kvh, hd, ctx),), 0xFF, dtype=torch.uint8, device="cuda")
+        scratch[:256] = 0
+        if not new:
+            K.KvCacheQ4.append(k, v, kc, vc, pos, kvh, hd, ctx, row_counts=counts)
+        A.compute_q4(q, kc, vc, out, pos, heads, kvh, hd, ctx, 0.09, scratch, row_counts=counts,
+                     k_new=k if new else None, v_new=v if new else None)
+        torch.cuda.synchronize()
+        assert (used_scratch(scratch) > 256) == (kind == "several")
+        got.append((kc, vc, out))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    for s in range(n):
+        assert (got[0][2][s, rows - 17 * s:] == 7.0).all() and (got[0][2][s, :rows - 17 * s] != 7.0).any(-1).all()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(32, 8, 128), (14, 2, 64), (8, 4, 32)])
+def test_seventeen_rows(K, heads, kvh, hd):
+    """The fewest rows that this kernel takes: a row group that they fill in part, unequal sequences."""
+    n, rows, ctx = 6, 17, 4096
+    b = Long(K, normal(1, n, ctx, kvh, hd), normal(2, n, ctx, kvh, hd), heads)
+    q = normal(3, n, rows, heads, hd)
+    at = [ctx - rows, 0, 111, 2000, 128, ctx - rows]
+    got, scratch = b.run(q, at)
+    assert 1 < splits_of(scratch, n, rows, heads, hd, b.ctx) < 16
+    b.check(got, q, at, list(range(rows)))
+
+
+@pytest.mark.parametrize("n,kind", MANY)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_few_large_weights_of_many_rows(K, n, kind, hd):
+    """Rows whose queries are a position's key, many times as large: its weight, and those of a few near copies of it, are
+    all there is, and a score's error is theirs."""
+    length, rows, heads, kvh = 2048, 200, 8, 2
+    k = normal(1, n, length, kvh, hd)
+    k[:, 1::2] = k[:, 0::2] + 0.02 * normal(2, n, length // 2, kvh, hd)
+    b = Long(K, k, normal(3, n, length, kvh, hd), heads)
+    at = [length - rows] * n
+    pick = torch.randint(0, length - rows, (n, rows, heads), generator=torch.Generator(device="cuda").manual_seed(4),
+                         device="cuda")
+    head = torch.arange(heads, device="cuda") // (heads // kvh)
+    q = b.k[torch.arange(n, device="cuda")[:, None, None], pick, head].float() * 6
+    got, scratch = b.run(q, at)
+    assert (splits_of(scratch, n, rows, heads, hd, b.ctx) > 1) == (kind == "several")
+    b.check(got, q, at, [0, 5, 127, 128, 199])
+
+
 @pytest.mark.parametrize("far", [26, 30, 31, 33, 36, 37])
 def test_one_large_weight_and_a_long_flat_tail(K, far):
     """One position outweighs each of 65535 others by about 2^far: alone they are nothing, together 2^(16 - far) of the
@@ -123,6 +245,51 @@ def test_one_large_weight_and_a_long_flat_tail(K, far):
         want = ((tail - 1) / (tail + 1)).view(1, heads, 1).expand(1, heads, hd)
         tol = 2.0 ** -24 + 2 * 2.0 ** -9 * 2.0 ** -16 + 32 * 2.0 ** -23 + 256 * 2.0 ** -25 + 48 * 2.0 ** -24
         torch.testing.assert_close(got[0, r:r + 1].double(), want, rtol=0, atol=tol)
+
+
+# --------------------------------------------- the same bits on every path
+def bits(K, b, q, positions):
+    """Rows of a call one by one (joined in the attention's launch) against the whole call."""
+    whole, _ = b.run(q, positions)
+    for s in range(q.shape[0]):
+        one = Long.__new__(Long)
+        one.__dict__.update(b.__dict__)
+        size = b.kc.numel() // b.n
+        one.kc, one.vc = b.kc[s * size:(s + 1) * size].clone(), b.vc[s * size:(s + 1) * size].clone()
+        for r in range(q.shape[1]):
+            alone, _ = one.run(q[s:s + 1, r:r + 1], [positions[s] + r])
+            assert torch.equal(alone[0, 0], whole[s, r]), (s, r)
+    return whole
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(8, 2, 128), (14, 2, 64), (4, 2, 32), (4, 2, 256)])
+@pytest.mark.parametrize("ctx,rows", [(2500, 1), (2500, 5), (6000, 1), (6000, 3), (12288, 1)])
+def test_bits_of_a_second_launch(K, heads, kvh, hd, ctx, rows):
+    """A decode step alone joins its chunks in the attention's launch; in a call of more than 64 groups of rows a second
+    one does.  Chunks of 256 and of 512 positions, the last of 1 to all of theirs."""
+    n = 40
+    assert n * kvh > 64
+    g = torch.Generator().manual_seed(ctx + hd)
+    lengths = torch.randint(rows, ctx + 1, (n,), generator=g).tolist()
+    lengths[:4] = [ctx, rows, 513, 1024]
+    b = Long(K, normal(1, n, ctx, kvh, hd), normal(2, n, ctx, kvh, hd), heads)
+    q = normal(3, n, rows, heads, hd)
+    at = [length - rows for length in lengths]
+    whole = bits(K, b, q, at)
+    b.check(whole, q, at, list(range(rows)))
+
+
+@pytest.mark.parametrize("hd,split", [(128, 4), (64, 2), (32, 1), (256, 2)])
+def test_bits_of_some_of_the_heads(K, hd, split):
+    """The KV heads of a part of a model (a rank of a split one) alone give the bits that they have among all."""
+    n, ctx, kvh, group = 3, 3000, 4, 4
+    k, v, q = normal(1, n, ctx, kvh, hd), normal(2, n, ctx, kvh, hd), normal(3, n, 2, kvh * group, hd)
+    at = [2998, 700, 0]
+    whole, _ = Long(K, k, v, kvh * group).run(q, at)
+    for h in range(0, kvh, split):
+        part, _ = Long(K, k[:, :, h:h + split], v[:, :, h:h + split], split * group).run(
+            q[:, :, h * group:(h + split) * group], at)
+        assert torch.equal(part, whole[:, :, h * group:(h + split) * group])
 
 
 # --------------------------------------------- every kernel
