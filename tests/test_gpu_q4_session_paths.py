@@ -44,3 +44,38 @@ def test_a_callers_bad_position_is_not_a_sessions(K, engine, kv):
         assert device_error() == 4 and device_error() == 0
     s.close()
     other.close()
+
+
+def test_bits_of_a_batch_beside_a_long_session(engine):
+    """Alone, a session's step joins its chunks in the attention's launch; beside a session of more than 12288 positions
+    a kernel for many chunks joins every row, and beside many sessions one for few.  Chunks of 256 and of 512."""
+    shapes = [(700, 1000), (3000, 4096), (2700, 8192), (513, 5000), (40, 12288), (1100, 13000)]
+    V = engine.vocabulary_size
+    alone = [engine.create_session(c, "q4") for _, c in shapes]
+    batch = [engine.create_session(c, "q4") for _, c in shapes]
+    for i, (n, _) in enumerate(shapes):
+        for s in (alone[i], batch[i]):
+            s.prefill(prompt(n, V, i))
+    for step in range(3):
+        t = prompt(len(shapes), V, 50 + step)
+        am = engine.decode_batch(batch, t)
+        for i, s in enumerate(alone):
+            assert s.decode(t[i]) == am[i]
+            np.testing.assert_array_equal(batch[i].get_last_logits(), s.get_last_logits())
+    # 40 sessions (80 groups of rows), none of more than 12288 positions
+    more = [engine.create_session(600, "q4") for _ in range(35)]
+    for i, s in enumerate(more):
+        s.prefill(prompt(3 + 14 * i, V, 70 + i))
+    t = prompt(40, V, 90)
+    am = engine.decode_batch(batch[:5] + more, t)
+    for i, s in enumerate(alone[:5]):
+        assert s.decode(t[i]) == am[i]
+        np.testing.assert_array_equal(batch[i].get_last_logits(), s.get_last_logits())
+    # and a verify of 17 rows over chunks of 512 (two parts of it) against single steps
+    rows = prompt(17, V, 91)
+    am, lg = batch[2].verify(rows, want_logits=True)
+    for j, x in enumerate(rows):
+        assert alone[2].decode(x) == am[j]
+        np.testing.assert_array_equal(alone[2].get_last_logits(), lg[j])
+    for s in alone + batch + more:
+        s.close()
