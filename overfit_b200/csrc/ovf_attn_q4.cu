@@ -855,11 +855,11 @@ ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_n
     if (st) return st;
     OVF_CHECK_ARG(n_heads > 0 && n_heads <= 65535 && n_heads % n_kv_heads == 0,
                   "attention_q4: n_heads %d must be a multiple of n_kv_heads %d (at most 65535)", n_heads, n_kv_heads);
+    if (n_seq == 0 || rows == 0) return OVF_OK;
     OVF_CHECK_ARG(q && out && scratch, "attention_q4: null buffer");
     OVF_CHECK_ARG(aligned16(q) && aligned16(out) && aligned16(scratch), "attention_q4: buffers must be 16-byte aligned");
     OVF_CHECK_ARG(q != out, "attention_q4: the output must not be the query");
     OVF_CHECK_ARG(!k_new == !v_new, "attention_q4: k_new and v_new go together");
-    if (n_seq == 0 || rows == 0) return OVF_OK;
     OVF_CHECK_ARG((int64_t)rows * n_heads <= (1 << 22), "attention_q4: %d rows of %d heads in one call (at most 2^22 in all)",
                   rows, n_heads);
     // (as many partial results as an int counts: more need hundreds of GB of scratch)

@@ -287,7 +287,8 @@ ovf_status q4_source(const char *what, const void *k_cache, const void *v_cache,
     OVF_CHECK_ARG(n_kv_heads > 0 && n_kv_heads <= 1024, "%s: n_kv_heads %d outside [1, 1024]", what, n_kv_heads);
     OVF_CHECK_ARG(max_ctx > 0 && max_ctx <= (1 << 20), "%s: max_ctx %d outside [1, 2^20]", what, max_ctx);
     OVF_CHECK_ARG(rows >= 0 && rows <= max_ctx, "%s: %d rows do not fit max_ctx %d", what, rows, max_ctx);
-    OVF_CHECK_ARG(k_cache && v_cache && positions, "%s: null buffer", what);
+    // (a call without rows needs no buffers: empty arrays may have no address)
+    OVF_CHECK_ARG(n_seq == 0 || rows == 0 || (k_cache && v_cache && positions), "%s: null buffer", what);
     OVF_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache), "%s: caches must be 16-byte aligned", what);
     OVF_CHECK_ARG((int64_t)rows * n_kv_heads <= (1 << 22), "%s: %d rows of %d heads in one call (at most 2^22 in all)", what,
                   rows, n_kv_heads);
@@ -327,12 +328,11 @@ ovf_status ovf_kv_q4_append(const float *k, const float *v, void *k_cache, void 
     Q4Source src;
     ovf_status st = q4_source("kv_q4_append", k_cache, v_cache, positions, row_counts, n_seq, rows, n_kv_heads,
                               head_dim, max_ctx, rope_cos, rope_sin, split_half, &src);
-    if (st) return st;
+    if (st || n_seq == 0 || rows == 0) return st;
     OVF_CHECK_ARG(k && v, "kv_q4_append: null buffer");
     OVF_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(rope_cos) && aligned16(rope_sin),
                   "kv_q4_append: buffers must be 16-byte aligned");
     OVF_CHECK_ARG(k_cache != v_cache, "kv_q4_append: keys and values need caches of their own");
-    if (n_seq == 0 || rows == 0) return OVF_OK;
     return launch_kv_q4_append(src, head_dim, k, v, reinterpret_cast<cudaStream_t>(stream), false);
 }
 
@@ -343,10 +343,9 @@ ovf_status ovf_kv_q4_read(const void *k_cache, const void *v_cache, const int32_
     Q4Source src;
     ovf_status st = q4_source("kv_q4_read", k_cache, v_cache, positions, row_counts, n_seq, rows, n_kv_heads, head_dim,
                               max_ctx, nullptr, nullptr, 0, &src);
-    if (st) return st;
+    if (st || n_seq == 0 || rows == 0) return st;
     OVF_CHECK_ARG(k && v && k != v, "kv_q4_read: null buffer, or one for both sides");
     OVF_CHECK_ARG(aligned16(k) && aligned16(v), "kv_q4_read: buffers must be 16-byte aligned");
-    if (n_seq == 0 || rows == 0) return OVF_OK;
     return launch_kv_q4_read(src, head_dim, k, v, reinterpret_cast<cudaStream_t>(stream));
 }
 

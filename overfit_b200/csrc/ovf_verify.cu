@@ -592,11 +592,11 @@ extern "C" ovf_status ovf_verify_drafts(const float *logits, const float *draft_
     OVF_CHECK_ARG(n_seq >= 0 && n_seq <= 65535, "verify_drafts: n_seq %d outside [0, 65535]", n_seq);
     OVF_CHECK_ARG(max_drafts >= 0 && max_drafts <= 1023, "verify_drafts: max_drafts %d outside [0, 1023]", max_drafts);
     OVF_CHECK_ARG(vocab > 0 && vocab <= (1 << 24), "verify_drafts: vocab %d outside [1, 2^24]", vocab);
+    if (n_seq == 0) return OVF_OK;
     OVF_CHECK_ARG(logits && uniforms && temperatures && accepted && next_token, "verify_drafts: null buffer");
     OVF_CHECK_ARG(max_drafts == 0 || drafts, "verify_drafts: drafts are missing");
     OVF_CHECK_ARG(max_drafts > 0 || !draft_probs, "verify_drafts: probabilities without drafts");
     OVF_CHECK_ARG(accepted != next_token, "verify_drafts: one buffer for both results");
-    if (n_seq == 0) return OVF_OK;
     VerifyParams p{logits, draft_probs, uniforms, temperatures, drafts, draft_counts, accepted, next_token, max_drafts, vocab};
     return launch_verify_drafts(p, n_seq, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -79,3 +79,22 @@ def test_bits_of_a_batch_beside_a_long_session(engine):
         np.testing.assert_array_equal(alone[2].get_last_logits(), lg[j])
     for s in alone + batch + more:
         s.close()
+
+
+def test_calls_without_rows(K):
+    """No sequences, or no rows: nothing is done."""
+    A = K.CachedAttentionKernel
+    kc, vc = (torch.zeros(K.KvCacheQ4.bytes(2, 64, 32), dtype=torch.uint8, device="cuda") for _ in "kv")
+    scratch = torch.zeros(256, dtype=torch.uint8, device="cuda")
+    for n, rows in ((0, 1), (1, 0), (0, 0)):
+        pos = torch.zeros(n, dtype=torch.int32, device="cuda")
+        k, v, k2, v2 = (torch.zeros(n, rows, 128, device="cuda") for _ in range(4))
+        q, out = torch.zeros(n, rows, 256, device="cuda"), torch.zeros(n, rows, 256, device="cuda")
+        K.KvCacheQ4.append(k, v, kc, vc, pos, 2, 64, 32)
+        K.KvCacheQ4.read(kc, vc, pos, 2, 64, 32, k2, v2)
+        A.compute_q4(q, kc, vc, out, pos, 4, 2, 64, 32, 0.1, scratch)
+        A.compute_q4(q, kc, vc, out, pos, 4, 2, 64, 32, 0.1, scratch, k_new=k, v_new=v)
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    K.SpeculativeVerifier.verify(torch.zeros(0, 3, 100, device="cuda"), torch.zeros(0, 2, dtype=torch.int32, device="cuda"),
+                                 torch.zeros(0, 3, device="cuda"), torch.zeros(0, device="cuda"), empty, empty.clone())
+    assert device_error() == 0 and not kc.any() and not vc.any()
