@@ -324,11 +324,12 @@ class CudaLlamaSession:
             q = np.ascontiguousarray(np.asarray(draft_probs, dtype=np.float32))
             if q.shape != (n - 1, self.engine.cfg["vocab"]):
                 raise ValueError("draft_probs must be [tokens - 1, vocab]")
-        a, t = C.c_int32(), C.c_int32()
-        check(_lib.load().ovf_session_verify_sampled(self._h, toks.ctypes.data, n, None if q is None else q.ctypes.data,
-                                                     u.ctypes.data, float(temperature), C.byref(a), C.byref(t)),
-              "VerifySampled")
-        self._have_logits = False
+        a, t, at = C.c_int32(), C.c_int32(), self.current_position
+        status = _lib.load().ovf_session_verify_sampled(self._h, toks.ctypes.data, n, None if q is None else q.ctypes.data,
+                                                        u.ctypes.data, float(temperature), C.byref(a), C.byref(t))
+        if self.current_position != at:  # (a failed call's rows may be in the cache, too)
+            self._have_logits = False
+        check(status, "VerifySampled")
         return a.value, t.value
 
     def generate_speculative_sampled(self, history, rng, temperature: float, max_draft: int = 4, ngram_min: int = 1,

@@ -1,0 +1,61 @@
+"""The host side of sampled verification and speculative generation:
+the library's calls are faked."""
+import numpy as np
+import pytest
+
+import q4_reference as ref
+
+
+@pytest.fixture
+def engine():
+    from overfit_b200 import build, engine
+    build.build()
+    return engine
+
+
+class Fake:
+    """A library whose sampled verify gives `status`, and whose other session calls succeed."""
+
+    def __init__(self, status=0):
+        self.status, self.position, self.rows = status, 20, []
+
+    def ovf_session_position(self, h):
+        return self.position
+
+    def ovf_session_verify_sampled(self, h, tokens, n, probs, u, T, accepted, token):
+        self.rows.append(n)
+        self.position += 1
+        return self.status
+
+    def ovf_session_decode(self, h, token, logits, argmax):
+        self.position += 1
+        return 0
+
+    def ovf_last_error(self):
+        return b"no distribution"
+
+
+def session(engine, monkeypatch, fake, logits):
+    monkeypatch.setattr(engine._lib, "load", lambda: fake)
+    s = engine.CudaLlamaSession.__new__(engine.CudaLlamaSession)
+    s.engine = type("E", (), {"cfg": {"vocab": len(logits)}})()
+    s._h, s._logits, s._have_logits, s.max_context_length = 0, np.asarray(logits, np.float32), True, 1000
+    return s
+
+
+def test_a_failed_verify_leaves_no_logits(engine, monkeypatch):
+    """The rows behind which there is no distribution are in the cache: the logits of the step before are not the session's."""
+    from overfit_b200 import _lib
+    s = session(engine, monkeypatch, Fake(_lib.OVF_ESTATE), np.zeros(10))
+    with pytest.raises(engine.OverfitRuntimeError):
+        s.verify_sampled([1, 2], [0.5, 0.5], 1.0)
+    assert s.current_position == 21
+    with pytest.raises(engine.OverfitRuntimeError):
+        s.get_last_logits()
+
+
+def test_a_refused_verify_keeps_the_logits(engine, monkeypatch):
+    s = session(engine, monkeypatch, Fake(), np.arange(10))
+    with pytest.raises(ValueError):
+        s.verify_sampled([1, 2], [0.5], 1.0)
+    assert s.get_last_logits()[3] == 3
