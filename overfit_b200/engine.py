@@ -23,6 +23,8 @@ from . import _lib
 from ._lib import (TENSORS_PER_LAYER, TYPE_F32, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_0, ModelConfig, OverfitRuntimeError,
                    Tensor, check)
 
+VERIFY_MAX = 64  # rows of one verify forward
+
 LAYER_KEYS = ("attn_norm", "wq", "wk", "wv", "wo", "bq", "bk", "bv", "bo", "ffn_norm", "gate", "up", "down", "router")
 
 # Benchmark model shapes (random-init, synthetic).  eps follows the reference,
@@ -347,7 +349,7 @@ class CudaLlamaSession:
         z = self.get_last_logits().astype(np.float64) / temperature
         cum = np.cumsum(np.exp(z - z.max()))
         t0 = min(int(np.searchsorted(cum, rng.random() * cum[-1], side="right")), cum.size - 1)
-        draft = prompt_lookup_draft(list(history) + [t0], max_draft, ngram_min, ngram_max)
+        draft = prompt_lookup_draft(list(history) + [t0], min(max_draft, VERIFY_MAX - 1), ngram_min, ngram_max)
         if not draft or self.current_position + 1 + len(draft) + 1 > self.max_context_length:
             self.decode(t0)
             return [t0]
