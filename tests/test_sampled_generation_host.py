@@ -65,5 +65,5 @@ def test_drafts_of_any_length(engine, monkeypatch):
     """A verify takes 64 rows: a longer draft is cut, not refused."""
     fake = Fake()
     s = session(engine, monkeypatch, fake, np.r_[50.0, np.zeros(9)])
-    s.generate_speculative_sampled([0, 1, 2, 3, 4, 5, 6, 7, 8, 9] * 20, np.random.default_rng(0), 1.0, max_draft=200)
+    s.generate_speculative_sampled([0] + [1, 2, 3, 4, 5, 6, 7, 8, 9] * 20, np.random.default_rng(0), 1.0, max_draft=200)
     assert fake.rows == [64]
