@@ -341,14 +341,12 @@ class CudaLlamaSession:
         that accepts them against the target's distribution, and the token drawn
         behind them decoded, so that the session holds its logits.  Returns the
         committed tokens (>= 1), distributed as single sampled steps would be.
-        `rng`: a numpy Generator."""
+        `rng`: a numpy Generator.  Logits without a distribution raise."""
         if max_draft <= 0:
             raise ValueError("maxDraft must be positive")
         if not temperature > 0:
             raise ValueError("temperature must be positive (generate_speculative is the greedy form)")
-        z = self.get_last_logits().astype(np.float64) / temperature
-        cum = np.cumsum(np.exp(z - z.max()))
-        t0 = min(int(np.searchsorted(cum, rng.random() * cum[-1], side="right")), cum.size - 1)
+        t0 = draw_token(self.get_last_logits(), rng.random(), temperature)
         draft = prompt_lookup_draft(list(history) + [t0], min(max_draft, VERIFY_MAX - 1), ngram_min, ngram_max)
         if not draft or self.current_position + 1 + len(draft) + 1 > self.max_context_length:
             self.decode(t0)
@@ -449,6 +447,18 @@ class CudaLlamaSession:
             self.close()
         except Exception:
             pass
+
+
+def draw_token(logits, uniform: float, temperature: float) -> int:
+    """The first token whose cumulative probability passes `uniform`, as
+    ovf_verify_drafts draws it: 64 bits, logits of -infinity or of the lowest float
+    impossible, a temperature of more than 1e30 as 1e30."""
+    x = np.asarray(logits, dtype=np.float64)
+    top = x.max()
+    if not np.isfinite(top) or top == -np.finfo(np.float32).max:  # (the maximum of a row with NaN is NaN)
+        raise OverfitRuntimeError("the session's logits are no distribution")
+    cum = np.cumsum(np.exp((x - top) / min(float(temperature), 1e30)))
+    return int(np.searchsorted(cum, uniform * cum[-1], side="right"))  # (`uniform` below 1: inside)
 
 
 def prompt_lookup_draft(history, max_draft: int, ngram_min: int = 1, ngram_max: int = 3) -> list:
