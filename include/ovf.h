@@ -294,11 +294,11 @@ ovf_status ovf_attention_q4(const float *q, const float *k_new, const float *v_n
  * nothing has weight).  uniforms [n_seq][max_drafts + 1] in [0, 1);
  * temperatures [n_seq]: 0 or less is greedy (a draft is accepted iff it is its
  * row's first maximum, and the next token is that maximum), more than 1e30 is
- * 1e30.  Logits of -infinity or of the lowest float are impossible tokens; a
- * row that has no others, or a NaN or +infinity, accepts nothing and gives
- * token -1.  A draft outside the vocabulary is rejected.  draft_counts [n_seq]
- * or NULL (max_drafts each): negative marks an
- * unused place, whose results are left as they are.
+ * 1e30.  Logits of -infinity or of the lowest float are impossible tokens, and a
+ * weight below e^-690 of its row's largest counts as none; a row that has no
+ * other logits, or a NaN or +infinity, accepts nothing and gives token -1.  A draft
+ * outside the vocabulary is rejected.  draft_counts [n_seq] or NULL (max_drafts
+ * each): negative marks an unused place, whose results are left as they are.
  * accepted [n_seq]: drafts accepted; next_token [n_seq].  max_drafts 0 samples
  * plainly.  Probabilities and sums are formed in 64 bits. */
 ovf_status ovf_verify_drafts(const float *logits, const float *draft_probs, const int32_t *drafts,

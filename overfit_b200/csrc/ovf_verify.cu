@@ -40,15 +40,15 @@ static constexpr int kVfStep = 128;         // elements that a warp takes at onc
 // rows that a warp's run meets: the run is ceil(rows * steps / warps) steps of `steps` a row
 static constexpr int kVfSlots = kVfRows / kVfWarps + 2;  // (a cluster of one CTA)
 
-// e^x in 64 bits for x of -700 to 700, off by less than 2^-44: x = n ln 2 / 64 + r, the series of e^r to r^4
-// (|r| < 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64)
+// e^x in 64 bits for x of -700 to 700, off by less than 2^-43.8 (2^-44.4 for |x| < 40; the series' rest is 2^-44.5 at
+// most, the double of ln 2 / 64, n times, up to 2^-45.2): x = n ln 2 / 64 + r, the series of e^r to r^4 (|r| < 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64)
 // less i << 46 (the lanes of half a warp have a copy each, for indices are as good as random).  NaN stays NaN.
 // A branch for other x would double its time (3.8 clocks a warp and SM): its callers raise smaller logits to
 // a floor of weight e^-690 instead, in 32 bits.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
     const double shift = 0x1.8p52;  // its sum with a number ends in that number's nearest integer
     const double kd = fma(x, 64.0 / 0.693147180559945309417, shift), n = kd - shift;
-    const double r = fma(n, -0.693147180559945309417 / 64.0, x);  // (n < 2^17: off by less than 2^-46)
+    const double r = fma(n, -0.693147180559945309417 / 64.0, x);  // (|n| < 2^16)
     double y = fma(r, 1.0 / 24.0, 1.0 / 6.0);
     y = fma(y, r, 0.5);
     y = fma(y, r, 1.0);
