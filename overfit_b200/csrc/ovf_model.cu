@@ -1973,6 +1973,16 @@ ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, 
     return finish_call(s->stream, s->err_slot);
 }
 
+// The position becomes length; the session's logits stay what it generates from next if they are `kept`.
+static ovf_status truncate_session(ovf_session *s, int length, bool kept) {
+    ovf_status r = launch_truncate_step(s->step, length, s->tokens_log, kept, s->stream);
+    if (r) return r;
+    OVF_CUDA_TRY(cudaStreamSynchronize(s->stream));
+    s->pos = length;
+    s->n_logits = kept && s->n_logits > 0 ? 1 : 0;
+    return OVF_OK;
+}
+
 ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int32_t n, const float *draft_probs,
                                       const float *uniforms, float temperature, int32_t *accepted_out,
                                       int32_t *next_token_out) {
@@ -2010,7 +2020,7 @@ ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int
         s->needs_reset = true;
         return r;
     }
-    if ((r = ovf_session_truncate(s, base + 1 + result[0]))) return r;
+    if ((r = truncate_session(s, base + 1 + result[0], true))) return r;
     *accepted_out = result[0];
     *next_token_out = result[1];
     if (result[1] < 0) {
@@ -2027,11 +2037,7 @@ ovf_status ovf_session_truncate(ovf_session *s, int32_t length) {
     OVF_CHECK_ARG(s, "TruncateTo: null session");
     OVF_CHECK_ARG(length >= 0 && length <= s->pos, "TruncateTo %d must be in [0, CurrentLength=%d]", length, s->pos);
     DeviceGuard guard(s->m->device);
-    ovf_status r = launch_set_step_pos(s->step, length > 0 ? length - 1 : 0, length, s->stream);
-    if (r) return r;
-    OVF_CUDA_TRY(cudaStreamSynchronize(s->stream));
-    s->pos = length;
-    return OVF_OK;
+    return truncate_session(s, length, true);
 }
 
 static size_t kv_elem_bytes(const ovf_session *s) {

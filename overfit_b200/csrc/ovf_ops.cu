@@ -498,6 +498,21 @@ ovf_status launch_set_step_pos(DevStep *step, int cur, int next, cudaStream_t st
     return cuda_status(cudaGetLastError(), "set_step_pos");
 }
 
+// The state behind a truncation.  The log starts anew with its last token, if
+// that is `kept`: a session that is cut back again and again would write behind
+// the log's end otherwise.
+__global__ void truncate_step_kernel(DevStep *step, int length, int32_t *tokens_log, int kept) {
+    step->cur_pos = length > 0 ? length - 1 : 0;
+    step->next_pos = length;
+    if (step->n_generated > 0) tokens_log[0] = tokens_log[step->n_generated - 1];
+    step->n_generated = kept && step->n_generated > 0 ? 1 : 0;
+}
+
+ovf_status launch_truncate_step(DevStep *step, int length, int32_t *tokens_log, bool kept, cudaStream_t st) {
+    truncate_step_kernel<<<1, 1, 0, st>>>(step, length, tokens_log, kept);
+    return cuda_status(cudaGetLastError(), "truncate_step");
+}
+
 // --------------------------------------------------------------- SiLU * up
 // Runtime/CachedFeedForwardBlock.cs:464-472 + :309: h = (g*sigmoid(g))*u, for
 // gate/up pairs that cannot share one GEMV launch.
