@@ -450,7 +450,8 @@ ovf_status ovf_session_verify(ovf_session *s, const int32_t *tokens, int32_t n, 
  * [0, 1), one per draft and one for the next token.  The rows run as in
  * ovf_session_verify; the session's position becomes that behind the accepted
  * drafts, and *next_token_out (not decoded yet) is the token drawn there.
- * temperature 0 or less accepts greedily.  Host pointers.  A row of logits
+ * temperature 0 or less accepts greedily.  Host pointers.  The session holds no
+ * logits to generate from until the next prefill or decode.  A row of logits
  * without a distribution returns OVF_ESTATE, the accepted drafts standing. */
 ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int32_t n, const float *draft_probs,
                                       const float *uniforms, float temperature, int32_t *accepted_out,

@@ -2020,7 +2020,8 @@ ovf_status ovf_session_verify_sampled(ovf_session *s, const int32_t *tokens, int
         s->needs_reset = true;
         return r;
     }
-    if ((r = truncate_session(s, base + 1 + result[0], true))) return r;
+    // (the last row's logits and greedy token are a rejected draft's, or not what was drawn: nothing to generate from)
+    if ((r = truncate_session(s, base + 1 + result[0], false))) return r;
     *accepted_out = result[0];
     *next_token_out = result[1];
     if (result[1] < 0) {

@@ -60,3 +60,20 @@ def test_a_cut_keeps_the_token_that_comes_next(engine):
         got = s.generate_greedy(3)
         assert got[0] == token and s.current_position == cut + 3
     s.close()
+
+
+def test_nothing_is_generated_behind_a_sampled_verify(engine):
+    """The token that it drew is not decoded yet; the last row's greedy token is of rejected drafts."""
+    prompt = np.random.default_rng(3).integers(0, engine.vocabulary_size, 20).tolist()
+    s, twin = engine.create_session(60, "q4"), engine.create_session(60, "q4")
+    for x in (s, twin):
+        x.prefill(prompt)
+    accepted, token = s.verify_sampled([5, 6, 7], [0.9, 0.9, 0.5], 1.0)
+    with pytest.raises(ValueError):
+        s.generate_greedy(1)
+    for t in [5, 6, 7][:accepted + 1] + [token]:
+        want = twin.decode(t)
+    assert s.decode(token) == want
+    np.testing.assert_array_equal(s.generate_greedy(5), twin.generate_greedy(5))
+    s.close()
+    twin.close()
