@@ -34,8 +34,10 @@
 // of all sequences, so that unequal lengths cost nothing; a warp's next keys load
 // while it weights values, and its next values while it scores.
 // Measured, 32 heads over 8, 128 wide: one token at 2048 positions 9.5 us (latency);
-// 64 sessions of up to 8192, 96 us, 3.94 TB/s (60 % of the copy rate), bound by
-// instructions (2.4 of 4 a clock; half of the integer pipe takes codes apart).
+// 64 sessions of up to 8192, 97 us, 3.9 TB/s (60 % of the copy rate), bound by latency at
+// low occupancy: 2.2 of 4 instructions a clock, half of the integer pipe (taking codes
+// apart) and half of DRAM in use, 3.8 warps a scheduler, which wait for fixed latencies,
+// loads and instruction fetch.  <4, 1, false> is at its 128 registers and spills some.
 #include "ovf_attn_q4_rows.cu"
 #include "ovf_q4.cuh"
 
