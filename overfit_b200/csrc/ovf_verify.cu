@@ -371,10 +371,10 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
             drafted = vf_exp0(((double)row.x[row.out] - row.m) * inv, tab);
         }
         // The row's parts and their weights.  Without a distribution to take away they are the runs above and their
-        // sums (less a draft's, unless little were left: a difference of nearly equal sums would be inexact); else
-        // the row is passed once more.
+        // sums (less a draft's, unless little were left: a difference of nearly equal sums would be inexact, and a
+        // uniform so small asks for the least of what is left); else the row is passed once more.
         int parts, part0, per = 0;
-        const bool again = (k < n && p.probs) || drafted > 0.99 * sh.row_sum[k];
+        const bool again = (k < n && p.probs) || drafted > 0.99 * sh.row_sum[k] || (row.out >= 0 && last_u < 1e-8f);
         if (again) {
             if (k < n && p.probs) {
                 row.q = p.probs + ((size_t)s * p.max_drafts + k) * V;
@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
             if (lane >= o) before += y;
         }
         const double target = (double)last_u * __shfl_sync(0xFFFFFFFFu, before, 31);
-        before -= own;
+        before = __shfl_up_sync(0xFFFFFFFFu, before, 1);  // (not by a subtraction, which loses small weights before a large one)
+        if (lane == 0) before = 0.0;
         int part = 0x7FFFFFFF, last = -1;
         for (int i = 0; i < entries; ++i) {
             const double y = sh.all[i * 32 + lane];
@@ -465,6 +466,8 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
                     const double y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
                     if (lane >= o) incl += y;
                 }
+                double excl = __shfl_up_sync(0xFFFFFFFFu, incl, 1);
+                if (lane == 0) excl = 0.0;
                 __syncthreads();
                 if (lane == 31) sh.step[warp] = incl;
                 if (tid == 0) sh.token = 0x7FFFFFFF, sh.last = -1;
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kVfThreads, Ctas) verify_drafts_kernel(const V
                     if (w < warp) cum += sh.step[w];
                     base += sh.step[w];
                 }
-                cum += incl - four;
+                cum += excl;
                 unsigned hit = 0x7FFFFFFFu;
                 int any = -1;
 #pragma unroll
