@@ -56,9 +56,9 @@ static constexpr int kArMma = 8 + kArExpand;
 static constexpr int kArThreads = (kArMma + 1) * 32;
 static constexpr int kArStages = 2;
 static constexpr int kArWindow = 2;      // tiles that one accumulator in TMEM sums (a power of 2)
-static constexpr int kArSums = 16;      // tiles whose weights are summed before they are added to the others' (a power of 2)
-static constexpr float kArLift = 12.0f;  // weights times 2^12
-static constexpr float kArSlack = 3.5f;  // inside a window the maximum is raised when it is passed by 2^3.5
+static constexpr int kArSums = 16;       // tiles whose weights are summed before they are added to the others' (a power of 2)
+static constexpr float kArLift = 12.0f; // weights times 2^12
+static constexpr float kArSlack = 3.5f; // inside a window the maximum is raised when it is passed by 2^3.5
 
 template <int NG>
 struct ArSmem {

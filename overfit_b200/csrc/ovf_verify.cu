@@ -40,9 +40,10 @@ static constexpr int kVfStep = 128;         // elements that a warp takes at onc
 // rows that a warp's run meets: the run is ceil(rows * steps / warps) steps of `steps` a row
 static constexpr int kVfSlots = kVfRows / kVfWarps + 2;  // (a cluster of one CTA)
 
-// e^x in 64 bits for x of -700 to 700, off by less than 2^-43.8 (2^-44.4 for |x| < 40; the series' rest is 2^-44.5 at
-// most, the double of ln 2 / 64, n times, up to 2^-45.2): x = n ln 2 / 64 + r, the series of e^r to r^4 (|r| < 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64)
-// less i << 46 (the lanes of half a warp have a copy each, for indices are as good as random).  NaN stays NaN.
+// e^x in 64 bits for x of -700 to 700, off by less than 2^-43.8 (2^-44.4 for |x| < 40: the series' rest is 2^-44.5 at
+// most, the double of ln 2 / 64, n times, up to 2^-45.2).  x = n ln 2 / 64 + r, the series of e^r to r^4 (|r| <
+// 0.0055), and 2^(n / 64) from `tab`, this lane's column of the table: entry 16 i holds the bits of 2^(i / 64) less
+// i << 46 (the lanes of half a warp have a copy each, for indices are as good as random).  NaN stays NaN.
 // A branch for other x would double its time (3.8 clocks a warp and SM): its callers raise smaller logits to
 // a floor of weight e^-690 instead, in 32 bits.
 __device__ __forceinline__ double vf_exp(double x, const unsigned long long *tab) {
